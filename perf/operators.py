@@ -399,7 +399,7 @@ def _own(s):
     case, lib, stream = s["case"], s["lib"], torch.cuda.current_stream().cuda_stream
     if case["op"] == "plan":
         rc = lib.l3m_kv4_plan_dev(s["call"], stream)
-        out = [s["tables"], s["free"], s["n_free_out"][0], s["q_start"], s["kv_total"], s["slot"], s["pos"]]
+        out = [s["tables"], s["free"], s["n_free_out"], s["q_start"], s["kv_total"], s["slot"], s["pos"]]
     elif case["op"] == "attend":
         rc = lib.l3m_kv4_attend_dev(s["cache"], s["call"], stream)
         out = s["out"]
