@@ -106,6 +106,113 @@ L3M_API int l3m_expf_dev(const float *x, float *y, int n, void *stream);
 // on the current device over `steps` steps (64 .. 2^24) by one warp; synchronous. The decode's
 // chain-latency bound is its dependent steps per token times this.
 L3M_API int l3m_chain_cycles_dev(int steps, double *cycles_per_step);
+// ---- a paged key/value cache in 4 bits: its bookkeeping, its writer and its reader (no counterpart
+// in the reference, whose one sequence has one bf16 cache). Keys and values are held in the file
+// formats' 4-bit blocks, q4_0 or mxfp4, 32 values of one head of one token to a block; head_dim is
+// rounded up to whole blocks (the padding holds zeros). The unit is a tile of 16 tokens of one
+// head; with NG = ceil(head_dim / 32) it holds, in this order,
+//   key codes     [16 tokens][4 parts t][NG blocks j][4 bytes]: nibble i (low one first) is value 32*j + 8*t + i
+//   value codes   [16 tokens][8 parts g][NG blocks j][2 bytes]: nibble i is value 32*j + 4*g + i
+//   key scales    [16 tokens][NG] and value scales [16 tokens][NG]: f16 (q4_0) or e8m0 (mxfp4)
+// and tiles lie [page][kv head][page / 16]. value = (nibble - 8) * scale, or e2m1 * 2^(scale - 127).
+// A slot is page id * page + offset. Slots, lengths and positions are int32, addresses 64-bit.
+// All calls are asynchronous on the stream, allocate nothing, may be captured into a graph, and
+// read every length on the device. They return 0, or -1 with nothing launched.
+typedef struct {
+    void *data;                  // n_pages * l3m_kv4_page_bytes() bytes of device memory, 16-byte aligned
+    int   dtype;                 // L3M_DT_Q4_0 or L3M_DT_MXFP4
+    int   n_pages;               // n_pages * page < 2^31
+    int   page;                  // tokens per page, a multiple of 16, at most 4096
+    int   n_kv_heads, head_dim;  // head_dim a multiple of 8, 8 .. 256
+} l3m_kv4;
+L3M_API size_t l3m_kv4_page_bytes(int dtype, int n_kv_heads, int head_dim, int page);   // 0: no such cache
+
+// Bits that the calls below OR into their *status (device memory, NULL: not reported). The caller zeroes it.
+enum {
+    L3M_KV4_NO_PAGES = 1,        // plan: the free list ran out
+    L3M_KV4_BAD_LENGTH = 2,      // plan: a negative kv_len, a length beyond max_blocks * page, or a bad n_free
+    L3M_KV4_NO_ROOM = 4,         // plan: more new tokens than max_tokens
+    L3M_KV4_BAD_PAGE = 8,        // a page id or slot outside the cache was left out
+    L3M_KV4_BAD_POS = 16,        // qkv: a position outside the rotation table; its row was left out
+};
+
+// One step's bookkeeping. Request r holds kv_len[r] tokens in the pages tables[r][0 .. ceil(kv_len/page))
+// and brings new_len[r] tokens (0: it waits; below 0: it has ended and its pages return to the free list,
+// in request order, its table row left as it is). free_pages[0 .. *n_free) is a stack: new pages
+// come off its top, in request order. Writes the new table entries, the free list, *n_free_out,
+// q_start[0 .. n_req] (running sum of the new tokens), kv_total[r] (the length with the new tokens), and
+// for each new token its position and slot; rows behind the last one get -1. A request is left out (kv_total 0,
+// slots and positions -1, no pages taken) when its lengths are bad, when the pages wanted by it and the
+// requests before it exceed the free list and it wants some, or when its rows pass max_tokens; a status bit says so.
+typedef struct {
+    int n_req;                   // 0 .. 16384
+    int max_blocks;              // entries of a table row
+    int max_tokens;              // entries of slot and pos
+    int page, n_pages;
+    const int32_t *kv_len, *new_len;
+    int32_t *tables;             // [n_req][max_blocks]
+    int32_t *free_pages;         // [n_pages]
+    const int32_t *n_free;       // device memory, one value
+    int32_t *n_free_out;         // another one: it must not be n_free
+    int32_t *q_start;            // [n_req + 1]
+    int32_t *kv_total;           // [n_req], not kv_len
+    int32_t *slot, *pos;         // [max_tokens]
+    int32_t *status;
+} l3m_kv4_plan;
+L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream);
+
+// The prelude of attention, one pass over q, k and v: RMS norm of each query and key head over head_dim
+// (q_norm, k_norm: weights, NULL = no norm; x * w / sqrt(mean x^2 + eps)), then the rotation of its first rot_dim
+// values by pos[token] (rope_table[n_pos][rot_dim / 2][2]: cos, sin). Queries go to q_out. Keys go to
+// k_out (may be NULL) and, with a cache, keys and values to the cache's slot[token] in 4 bits (a negative slot:
+// not stored). A token with pos < 0 is padding: nothing of it is read or written. Tensors are
+// [n_tokens][heads][head_dim], heads contiguous, ld elements from token to token, so slices of one qkv matrix serve; q_out may be q
+// and k_out may be k. Codes and scales are those of exact arithmetic: as ggml's rule gives them for the
+// normed, rotated values in 64 bits (scales in f16: rounded to f32 first, at most 65504); a NaN is stored as 0. The tokens of a call
+// have different slots (the plan's do): where two share one, its row holds a mixture of both.
+typedef struct {
+    int   dtype;                 // of q, k, v, q_out and k_out: L3M_DT_F32 or L3M_DT_BF16
+    int   n_tokens, n_heads, n_kv_heads, head_dim;
+    int   rope;                  // 0 none, 1 adjacent pairs (2i, 2i + 1), 2 halves (i, i + rot_dim / 2)
+    int   rot_dim;               // even, at most head_dim
+    int   n_pos;
+    float eps;
+    const float *q_norm, *k_norm, *rope_table;
+    const int32_t *pos, *slot;   // slot: read with a cache only
+    const void *q, *k, *v;       // q with n_heads > 0; k; v with a cache only
+    int64_t q_ld, k_ld, v_ld;
+    void *q_out, *k_out;
+    int64_t q_out_ld, k_out_ld;
+    int32_t *status;
+} l3m_qkv;
+L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *stream);   // cache may be NULL
+// Reads cache rows back: k[i], v[i] ([n][n_kv_heads][head_dim], dtype L3M_DT_F32 or L3M_DT_BF16, either may be NULL) =
+// the values at slots[i]. A row whose slot lies outside the cache is left as it was.
+L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, const int32_t *slots, int n, void *stream);
+
+// Causal attention of a batch over the cache: request r's queries are rows q_start[r] .. q_start[r+1) of q, the
+// newest tokens of its kv_len[r] cached ones (kv_total of the plan, after l3m_qkv_rope_dev stored them). The query at position p sees
+// positions 0 .. p, with a window only those above p - window. A query that sees nothing (kv_len 0) gets
+// zeros; rows outside q_start's range stay as they were. Positions in pages with an id outside the cache are not seen. out may not overlap q.
+typedef struct {
+    int   dtype;                 // of q and out: L3M_DT_F32 or L3M_DT_BF16
+    int   n_heads;               // a multiple of n_kv_heads: query head h reads kv head h / (n_heads / n_kv_heads)
+    int   n_req, max_blocks;
+    int   max_q;                 // at least every request's number of queries
+    int   max_kv;                // at least every kv_len; at most max_blocks * page
+    int   window;                // 0: none
+    float scale;                 // of the scores, finite
+    const void *q;
+    void *out;
+    int64_t q_ld, out_ld;        // elements from token to token
+    const int32_t *q_start, *kv_len, *tables;
+    void  *scratch;              // l3m_kv4_attend_scratch() bytes of device memory, 16-byte aligned, in any state;
+    size_t scratch_bytes;        // calls that overlap need one each
+    int32_t *status;
+} l3m_kv4_attend;
+L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend *a);   // from the integer fields alone
+L3M_API int    l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, void *stream);
+
 // The last CUDA error this library saw, as text ("" if none).
 L3M_API const char *l3m_cuda_error(void);
 

@@ -34,6 +34,32 @@ class Vec(C.Structure):
     _fields_ = [("f32", C.c_void_p), ("bf16", C.c_void_p), ("q8", C.c_void_p), ("scale", C.c_void_p), ("sum", C.c_void_p)]
 
 
+class Kv4(C.Structure):
+    """l3m_kv4: a paged 4-bit key/value cache (include/l3m_kernels.h)."""
+    _fields_ = [("data", C.c_void_p), ("dtype", C.c_int), ("n_pages", C.c_int), ("page", C.c_int), ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class Kv4Plan(C.Structure):
+    """l3m_kv4_plan: one step's block tables, free list, slots and positions."""
+    _fields_ = [(f, C.c_int) for f in ("n_req", "max_blocks", "max_tokens", "page", "n_pages")] + \
+               [(f, C.c_void_p) for f in ("kv_len", "new_len", "tables", "free_pages", "n_free", "n_free_out", "q_start", "kv_total", "slot", "pos", "status")]
+
+
+class Qkv(C.Structure):
+    """l3m_qkv: query/key norm, rotation and the cache's write in one pass."""
+    _fields_ = [(f, C.c_int) for f in ("dtype", "n_tokens", "n_heads", "n_kv_heads", "head_dim", "rope", "rot_dim", "n_pos")] + [("eps", C.c_float)] + \
+               [(f, C.c_void_p) for f in ("q_norm", "k_norm", "rope_table", "pos", "slot", "q", "k", "v")] + \
+               [(f, C.c_int64) for f in ("q_ld", "k_ld", "v_ld")] + [("q_out", C.c_void_p), ("k_out", C.c_void_p)] + \
+               [("q_out_ld", C.c_int64), ("k_out_ld", C.c_int64), ("status", C.c_void_p)]
+
+
+class Kv4Attend(C.Structure):
+    """l3m_kv4_attend: attention of a batch over the cache."""
+    _fields_ = [(f, C.c_int) for f in ("dtype", "n_heads", "n_req", "max_blocks", "max_q", "max_kv", "window")] + [("scale", C.c_float)] + \
+               [("q", C.c_void_p), ("out", C.c_void_p), ("q_ld", C.c_int64), ("out_ld", C.c_int64)] + \
+               [(f, C.c_void_p) for f in ("q_start", "kv_len", "tables", "scratch")] + [("scratch_bytes", C.c_size_t), ("status", C.c_void_p)]
+
+
 GEMV = C.CFUNCTYPE(None, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(Vec))
 ATTEND = C.CFUNCTYPE(None, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int)
 
@@ -87,6 +113,12 @@ def lib():
         "l3m_attend_dev": (i, [vp, vp, vp, vp, i, i, i, vp]),
         "l3m_expf_dev": (i, [vp, vp, i, vp]),
         "l3m_chain_cycles_dev": (i, [i, C.POINTER(C.c_double)]),
+        "l3m_kv4_page_bytes": (sz, [i, i, i, i]),
+        "l3m_kv4_plan_dev": (i, [C.POINTER(Kv4Plan), vp]),
+        "l3m_qkv_rope_dev": (i, [C.POINTER(Kv4), C.POINTER(Qkv), vp]),
+        "l3m_kv4_load_dev": (i, [C.POINTER(Kv4), i, vp, vp, vp, i, vp]),
+        "l3m_kv4_attend_scratch": (sz, [C.POINTER(Kv4), C.POINTER(Kv4Attend)]),
+        "l3m_kv4_attend_dev": (i, [C.POINTER(Kv4), C.POINTER(Kv4Attend), vp]),
         "l3m_cuda_error": (C.c_char_p, []),
         "l3m_write_packed": (i, [C.c_char_p, C.c_char_p]),
     }

@@ -1,0 +1,715 @@
+// The paged 4-bit key/value cache: a step's bookkeeping (l3m_kv4_plan_dev), the pass that norms,
+// rotates and stores a step's queries, keys and values (l3m_qkv_rope_dev), and the read-back
+// (l3m_kv4_load_dev). Contracts in include/l3m_kernels.h, layout in kv4.cuh.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include <cfloat>
+#include <cmath>
+#include <cstdio>
+#include <type_traits>
+#include "kv4.cuh"
+
+using namespace l3m;
+
+extern "C" int l3m_error_msg(const char *msg);
+extern "C" int l3m_error_cuda(int e, const char *what);
+
+namespace {
+
+int refuse(const char *entry, const char *why) {
+    char msg[200];
+    snprintf(msg, sizeof msg, "%s: %s", entry, why);
+    return l3m_error_msg(msg);
+}
+
+int launched(const char *entry) {
+    const cudaError_t e = cudaGetLastError();
+    return e == cudaSuccess ? 0 : l3m_error_cuda(e, entry);
+}
+
+// ---- plan
+
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanMaxReq = 16384;
+
+struct PlanArgs {
+    l3m_kv4_plan a;
+};
+
+// Inclusive sum over the block; `total` gets the block's sum. ws: one value per warp, reused.
+__device__ long long block_scan(long long v, long long *ws, long long *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) ws[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        long long s = ws[lane];
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        ws[lane] = s;
+    }
+    __syncthreads();
+    if (warp) v += ws[warp - 1];
+    *total = ws[31];
+    __syncthreads();
+    return v;
+}
+
+// The last index i of sorted a[0..n) with a[i] <= x (a[0] <= x is the caller's promise).
+__device__ int last_not_above(const int *a, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Every CTA sums the requests' lengths for itself (a few microseconds at most: they fit one SM's
+// shared memory), so the CTAs need nothing from each other; then they share out the rows of slot and
+// pos, the new table entries and the returned pages. A page that comes off the stack above its old
+// top is one that an ended request returns in this call: it is read from that request's table row,
+// which nobody writes, not from the stack, which another CTA may still be writing.
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
+    const l3m_kv4_plan &a = p.a;
+    extern __shared__ int sh[];
+    const int n = a.n_req;
+    int *gone = sh, *used = sh + (n + 1), *start = sh + 2 * (n + 1);      // exclusive sums: pages returned, pages taken, rows
+    uint8_t *ok = (uint8_t *)(sh + 3 * (n + 1));
+    __shared__ long long ws[32];
+    __shared__ int left_s;
+    const int tid = threadIdx.x;
+    int status = 0;
+
+    const int free0 = *a.n_free;
+    const int old_top = min(max(free0, 0), a.n_pages);
+    if (free0 != old_top) status |= L3M_KV4_BAD_LENGTH;
+
+    // Pass 1: what ended requests return.
+    long long base = 0;
+    for (int c = 0; c < n; c += kPlanThreads) {
+        const int r = c + tid;
+        long long give = 0;
+        if (r < n) {
+            const long long kv = a.kv_len[r];
+            const long long held = (kv + a.page - 1) / a.page;
+            if (a.new_len[r] < 0 && kv >= 0 && held <= a.max_blocks) give = held;
+        }
+        long long sum;
+        const long long upto = block_scan(give, ws, &sum);
+        if (r < n) gone[r] = (int)min(base + upto - give, (long long)a.n_pages);
+        base += sum;
+    }
+    if (base > a.n_pages - old_top) {                                     // more pages than the pool has: the excess is dropped
+        status |= L3M_KV4_BAD_LENGTH;
+        base = a.n_pages - old_top;
+    }
+    const int n_gone = (int)base, top = old_top + n_gone;
+    if (tid == 0) {
+        gone[n] = n_gone;
+        left_s = top;
+    }
+
+    // Pass 2: what the others take.
+    long long rows = 0, pages = 0;
+    for (int c = 0; c < n; c += kPlanThreads) {
+        const int r = c + tid;
+        long long count = 0, need = 0, kv = 0;
+        int bad = 0, ended = 0;
+        if (r < n) {
+            kv = a.kv_len[r];
+            ended = a.new_len[r] < 0;
+            count = max(a.new_len[r], 0);
+            const long long held = (kv + a.page - 1) / a.page, after = (kv + count + a.page - 1) / a.page;
+            bad = kv < 0 || after > a.max_blocks || kv + count > 0x7fffffff;
+            if (!bad) need = after - held;
+        }
+        long long sum;
+        const long long rows_upto = block_scan(count, ws, &sum) + rows;
+        rows += sum;
+        const long long pages_upto = block_scan(need, ws, &sum) + pages;
+        pages += sum;
+        if (r < n) {
+            const bool pages_ok = need == 0 || pages_upto <= top, rows_ok = rows_upto <= a.max_tokens;
+            const bool served = !bad && !ended && pages_ok && rows_ok;
+            if (bad) status |= L3M_KV4_BAD_LENGTH;
+            if (!pages_ok) status |= L3M_KV4_NO_PAGES;
+            if (count && !rows_ok) status |= L3M_KV4_NO_ROOM;
+            used[r] = (int)min(pages_upto - need, 0x7fffffffLL);
+            start[r] = (int)min(rows_upto - count, 0x7fffffffLL);
+            ok[r] = served;
+            if (blockIdx.x == 0) {
+                a.q_start[r + 1] = (int)min(rows_upto, 0x7fffffffLL);
+                a.kv_total[r] = served ? (int)(kv + count) : 0;
+            }
+            if (served && need) atomicMin(&left_s, (int)(top - pages_upto));
+        }
+    }
+    if (tid == 0) {
+        used[n] = (int)min(pages, 0x7fffffffLL);
+        start[n] = (int)min(rows, 0x7fffffffLL);
+        if (blockIdx.x == 0) a.q_start[0] = 0;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+        if (tid == 0) *a.n_free_out = left_s;
+        if (status && a.status) atomicOr((int *)a.status, status);
+    }
+    const int taken = top - left_s;
+    const int step = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
+    auto returned = [&](int i) {                                          // the i-th returned page
+        const int r = last_not_above(gone, n, i);
+        return a.tables[(size_t)r * a.max_blocks + (i - gone[r])];
+    };
+    auto popped = [&](int i) {                                            // the i-th page off the stack
+        const int at = top - 1 - i;
+        return at < old_top ? a.free_pages[at] : returned(at - old_top);
+    };
+    for (int i = first; i < n_gone; i += step) a.free_pages[old_top + i] = returned(i);
+    for (int i = first; i < taken; i += step) {
+        const int r = last_not_above(used, n, i);
+        if (!ok[r]) continue;
+        const int block = (a.kv_len[r] + a.page - 1) / a.page + (i - used[r]);
+        a.tables[(size_t)r * a.max_blocks + block] = popped(i);
+    }
+    const int total = min(start[n], a.max_tokens);
+    for (int t = first; t < a.max_tokens; t += step) {
+        int pos = -1, slot = -1;
+        if (t < total) {
+            const int r = last_not_above(start, n, t);
+            if (ok[r]) {
+                const int kv = a.kv_len[r], held = (kv + a.page - 1) / a.page;
+                pos = kv + (t - start[r]);
+                const int block = pos / a.page;
+                const int id = block < held ? a.tables[(size_t)r * a.max_blocks + block] : popped(used[r] + block - held);
+                slot = id * a.page + (pos - block * a.page);
+            }
+        }
+        a.pos[t] = pos;
+        a.slot[t] = slot;
+    }
+}
+
+// ---- qkv
+
+constexpr int kQkvThreads = 256;
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f32(float *p, float x) { *p = x; }
+__device__ __forceinline__ void from_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+// 8 values at p: one or two 16-byte accesses where every row starts 16-byte aligned (vec), else one by one.
+__device__ __forceinline__ void load8(float *x, const float *p, bool vec) {
+    if (vec) {
+        const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
+        x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+        x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = p[e];
+    }
+}
+__device__ __forceinline__ void load8(float *x, const __nv_bfloat16 *p, bool vec) {
+    if (vec) {
+        const uint4 v = *(const uint4 *)p;
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            x[2 * e] = __uint_as_float(w[e] << 16);
+            x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = __bfloat162float(p[e]);
+    }
+}
+__device__ __forceinline__ void store8(float *p, const float *x, float f, bool vec) {
+    if (vec) {
+        ((float4 *)p)[0] = make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
+        ((float4 *)p)[1] = make_float4(x[4] * f, x[5] * f, x[6] * f, x[7] * f);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) p[e] = x[e] * f;
+    }
+}
+__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float *x, float f, bool vec) {
+    if (vec) {
+        __nv_bfloat162 h[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(x[2 * e] * f, x[2 * e + 1] * f);
+        *(uint4 *)p = *(const uint4 *)h;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) p[e] = __float2bfloat16_rn(x[e] * f);
+    }
+}
+
+struct QkvArgs {
+    l3m_qkv a;
+    Kv4Dev c;
+    int store, mx, vec;
+    int heads, chunks, per_chunk;         // rows per token; warps per token and the rows each takes
+};
+
+__device__ __forceinline__ double finite(double x) { return x != x ? 0.0 : fmin(fmax(x, -(double)FLT_MAX), (double)FLT_MAX); }
+
+// What a lane stores of its row: the codes of its 8 values and its block's scale bits.
+struct Held { unsigned codes, scale; };
+
+// The definition, in 64 bits, read again from memory: for the rows whose 32-bit values lie too near a border.
+// Every lane of the warp takes part (lanes without a row with src null).
+template <typename T, int LPR, int ROPE>
+__device__ __noinline__ Held exact_row(const T *src, const float *w, const float *turn, int D, int rot, float eps, int mx) {
+    const int lane = threadIdx.x & (LPR - 1), d0 = lane * 8, half = rot / 2;
+    const bool mine = src && d0 < D;
+    double u[8], ss = 0.0, f = 1.0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const int d = d0 + e;
+        double x = mine ? (double)to_f32(src[d]) : 0.0;
+        if (w) ss += x * x;
+        if (mine && w) x *= (double)w[d];
+        u[e] = x;
+        if (ROPE && mine && turn && d < rot) {
+            const int md = ROPE == 1 ? d ^ 1 : d < half ? d + half : d - half, i = ROPE == 1 ? d >> 1 : d < half ? d : d - half;
+            const bool second = ROPE == 1 ? (d & 1) != 0 : d >= half;
+            double m = (double)to_f32(src[md]);
+            if (w) m *= (double)w[md];
+            const double c = (double)turn[2 * i], s = (double)turn[2 * i + 1];
+            u[e] = second ? m * s + x * c : x * c - m * s;
+        }
+        u[e] = finite(u[e]);
+    }
+    for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (w) f = finite(1.0 / sqrt(ss / D + (double)eps));
+    double top = 0.0;
+    int at = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+        if (fabs(u[e]) > fabs(top)) {
+            top = u[e];
+            at = e;
+        }
+    at += (lane & 3) * 8;
+    for (int o = 1; o < 4; o <<= 1) {                                       // the first of equals over the block's 4 lanes
+        const double ot = __shfl_xor_sync(0xffffffffu, top, o);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (fabs(ot) > fabs(top) || (fabs(ot) == fabs(top) && oa < at)) {
+            top = ot;
+            at = oa;
+        }
+    }
+    Held r = {0, 0};
+    if (!mx) {
+        const double d = top / -8.0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double q = d != 0.0 ? floor(u[e] / d + 8.5) : 8.0;
+            r.codes |= (unsigned)(int)fmin(fmax(q, 0.0), 15.0) << (4 * e);
+        }
+        r.scale = top != 0.0 ? __half_as_ushort(__float2half_rn(fminf(fmaxf((float)(d * f), -65504.0f), 65504.0f))) : 0;
+    } else {
+        const double m = fabs(top * f);
+        const int e8 = m > 0.0 ? min(max(ilogb(m) + 125, 0), 254) : 0;
+        const double inv = ldexp(1.0, 127 - e8);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double y = u[e] * f, v = fabs(y) * inv;
+            const unsigned mag = (v > 0.25) + (v > 0.75) + (v > 1.25) + (v > 1.75) + (v > 2.5) + (v > 3.5) + (v > 5.0);
+            r.codes |= (mag | (y < 0.0 && mag ? 8u : 0u)) << (4 * e);
+        }
+        r.scale = (unsigned)e8;
+    }
+    return r;
+}
+
+// A row (a head of a token) is held by LPR lanes, 8 contiguous dims each, so 4 lanes hold a block. A warp
+// takes a run of one token's rows (queries, then keys, then values): position, rotation and slot are read once.
+//
+// Codes and scales have to be those of exact arithmetic, but a value next to a border between two codes may land
+// on either side of it in 32 bits. So u (the normed, rotated value before the row's factor, which
+// q4_0's codes do not depend on) is computed in 32 bits with a bound on its error, each decision with its
+// distance from the border, and where the distance is within the bound the row is redone in 64 bits (about 1% of the rows).
+// q4_0's test is exact for exact u: code >= b iff (b - 8.5) / 8 * |top| + u * sign(top) <= 0, one fma whose sign cannot
+// be rounded away; so values, which are neither normed nor rotated, never need 64 bits for it.
+template <typename T, int LPR, int ROPE>
+__global__ void __launch_bounds__(kQkvThreads) qkv_kernel(const QkvArgs p) {
+    const l3m_qkv &a = p.a;
+    __shared__ float mate_buf[ROPE == 2 ? kQkvThreads * 8 : 1];
+    constexpr int RPW = 32 / LPR;
+    const int wl = threadIdx.x & 31, lane = wl & (LPR - 1), sub = wl / LPR;
+    const int D = a.head_dim, d0 = lane * 8, half = ROPE ? a.rot_dim / 2 : 0;
+    const bool in = d0 < D;
+    float qw[8], kw[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        qw[e] = a.q_norm && in ? a.q_norm[d0 + e] : 1.0f;
+        kw[e] = a.k_norm && in ? a.k_norm[d0 + e] : 1.0f;
+    }
+    const bool partial = ROPE && a.rot_dim < D;
+    const int shift = ROPE == 2 && (half & 7) == 0 ? half >> 3 : 0;           // halves: the mate's lane is this far away; 0: through shared memory
+    const int mate_lane = (wl & ~(LPR - 1)) + (d0 < half ? lane + shift : d0 < 2 * half ? lane - shift : lane);
+    const long long items = (long long)a.n_tokens * p.chunks;
+    for (long long item = blockIdx.x * (kQkvThreads / 32) + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * (kQkvThreads / 32)) {
+        const int tok = (int)(item / p.chunks), first = (int)(item - (long long)tok * p.chunks) * p.per_chunk, end = min(first + p.per_chunk, p.heads);
+        const int pos = a.pos[tok];
+        if (pos < 0) continue;
+        if (ROPE && pos >= a.n_pos) {
+            if (a.status && wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_POS);
+            continue;
+        }
+        uint8_t *tile = nullptr;
+        int tr = 0;
+        if (p.store) {
+            const int slot = a.slot[tok];
+            if (slot >= p.c.n_pages * p.c.page) {
+                if (a.status && wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
+            } else if (slot >= 0) {
+                const int page = slot / p.c.page, off = slot - page * p.c.page;
+                tile = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
+                tr = off % kKvTile;
+            }
+        }
+        // cos and sin of this lane's dims; halves carry the sign of the mate's term in sin
+        float cs[8], sn[8];
+        const float *turn = ROPE ? a.rope_table + (size_t)pos * half * 2 : nullptr;
+        if (ROPE) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const int d = d0 + e;
+                if (d < 2 * half) {
+                    const int i = ROPE == 1 ? d >> 1 : d < half ? d : d - half;
+                    const float2 t = *(const float2 *)(turn + 2 * i);
+                    cs[e] = t.x;
+                    sn[e] = (ROPE == 1 ? e & 1 : d >= half) ? t.y : -t.y;
+                } else {
+                    cs[e] = 1.0f;
+                    sn[e] = 0.0f;
+                }
+            }
+        }
+        for (int hb = first; hb < end; hb += RPW) {
+            const int h = hb + sub;
+            const bool live = h < end;
+            const int kind = !live || h < a.n_heads ? 0 : h < p.heads - (p.store ? a.n_kv_heads : 0) ? 1 : 2;
+            const int hh = kind == 0 ? h : kind == 1 ? h - a.n_heads : h - (p.heads - a.n_kv_heads);
+            const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (size_t)tok * (kind == 0 ? a.q_ld : kind == 1 ? a.k_ld : a.v_ld) + (size_t)hh * D;
+            float u[8];
+            if (live && in) {
+                load8(u, src + d0, p.vec);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; e++) u[e] = 0.0f;
+            }
+            const float *w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+            float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value
+            if (a.q_norm || a.k_norm) {
+                float ss = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) ss = fmaf(u[e], u[e], ss);
+#pragma unroll
+                for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                if (w) {
+                    const float m = __fdiv_rn(ss, (float)D) + a.eps;
+                    f = __frcp_rn(__fsqrt_rn(m));
+#pragma unroll
+                    for (int e = 0; e < 8; e++) u[e] *= kind ? kw[e] : qw[e];
+                }
+            }
+            if (ROPE) {
+                float m[8];
+                if (ROPE == 1) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) m[e] = u[e ^ 1];
+                } else if (shift) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) m[e] = __shfl_sync(0xffffffffu, u[e], mate_lane);
+                } else {
+                    float *row = mate_buf + (threadIdx.x - lane) * 8;
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; e++) row[d0 + e] = u[e];
+                    __syncwarp();
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const int d = d0 + e;
+                        m[e] = d < half ? row[d + half] : d < 2 * half ? row[d - half] : 0.0f;
+                    }
+                }
+                if (kind < 2) {
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        size = fmaxf(size, fabsf(u[e]) + fabsf(m[e]));
+                        const float r = fmaf(m[e], sn[e], u[e] * cs[e]);
+                        u[e] = partial && d0 + e >= a.rot_dim ? u[e] : r;
+                    }
+                }
+            }
+            Held held = {0, 0};
+            const bool keep = live && kind && tile;
+            if (__any_sync(0xffffffffu, keep)) {
+                // The block's extremes; zero keeps a sum of zeros, anything not finite spoils it.
+                float hi = u[0], lo = u[0], zero = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    hi = fmaxf(hi, u[e]);
+                    lo = fminf(lo, u[e]);
+                    zero = fmaf(u[e], 0.0f, zero);
+                }
+#pragma unroll
+                for (int o = 1; o < 4; o <<= 1) {
+                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+                    size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
+                }
+                const float mag = fmaxf(hi, -lo);
+                // An upper bound on the error of u: three roundings of |a| + |b| at 2^-24 (the rotation), one of u (the weight).
+                const bool exact = kind == 2 || (!w && !(ROPE && a.rot_dim));
+                const float err = exact ? 0.0f : ROPE && a.rot_dim ? size * 0x1p-22f : mag * 0x1p-23f;
+                bool again = !(zero == 0.0f) || (mag < 0x1p-100f && (mag > 0.0f || err > 0.0f)) || mag > 0x1p120f;
+                if (!p.mx) {
+                    // opposite signs of one size: the sign of the first decides
+                    again |= mag > 0.0f && fabsf(hi + lo) <= 2.0f * err;
+                    const float top = hi >= -lo ? hi : lo, inv = __fdividef(-8.0f, top), sgn = hi >= -lo ? 1.0f : -1.0f;
+                    const float tol = exact ? -1.0f : 3.0f * err + mag * 0x1p-22f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float b = rintf(fmaf(u[e], inv, 8.5f));
+                        const float r = fmaf(fmaf(b, 0.125f, -1.0625f), mag, u[e] * sgn);
+                        again |= fabsf(r) <= tol;
+                        const int code = (int)b - (r <= 0.0f ? 0 : 1);
+                        held.codes |= (unsigned)min(max(code, 0), 15) << (4 * e);
+                    }
+                    const float s = top * -0.125f * f, rel = 0x1p-20f + __fdividef(2.0f * err, mag);
+                    const unsigned short s0 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f - rel), -65504.0f), 65504.0f)));
+                    const unsigned short s1 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f + rel), -65504.0f), 65504.0f)));
+                    if (exact) held.scale = __half_as_ushort(__float2half_rn(fminf(fmaxf(s, -65504.0f), 65504.0f)));
+                    else held.scale = s0;
+                    again |= !exact && s0 != s1;
+                    if (mag == 0.0f) held = {0x88888888u, 0};
+                } else {
+                    const float m = mag * f, rel = exact ? 0.0f : 0x1p-20f + __fdividef(2.0f * err, mag);
+                    const unsigned e0 = __float_as_uint(m * (1.0f - rel)) >> 23, e1 = __float_as_uint(m * (1.0f + rel)) >> 23;
+                    again |= mag > 0.0f && (e0 != e1 || e0 < 20u || e0 > 250u || f > 0x1p17f);   // far from either end, fi below is a normal number
+                    const float inv = mag > 0.0f ? __uint_as_float((256u - e0) << 23) : 0.0f;   // 2^(127 - e8), e8 = e0 - 2
+                    const float fi = f * inv, tol = exact ? -1.0f : (3.0f * err + mag * 0x1p-20f) * fi * 2.0f;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        const float v = fabsf(u[e]) * fi;                     // in [0, 8): the steps are 1/2 below 2, 1 below 4, 2 above
+                        const float r = fmaf(v, v < 2.0f ? 2.0f : v < 4.0f ? 1.0f : 0.5f, -0.5f), c = ceilf(r);
+                        again |= fabsf(r - rintf(r)) <= tol;
+                        const int code = min((int)c + (v < 2.0f ? 0 : v < 4.0f ? 2 : 4), 7);
+                        held.codes |= (unsigned)(code | (u[e] < 0.0f && code ? 8 : 0)) << (4 * e);
+                    }
+                    held.scale = mag > 0.0f ? e0 - 2 : 0;
+                }
+                again &= keep;
+                if (__any_sync(0xffffffffu, again)) {
+                    const Held h64 = exact_row<T, LPR, ROPE>(live ? src : nullptr, w, kind == 2 ? nullptr : turn, D, kind == 2 ? 0 : a.rot_dim, a.eps, p.mx);
+                    const unsigned blockmask = 0xfu << (wl & ~3);
+                    if (__ballot_sync(0xffffffffu, again) & blockmask) held = h64;
+                }
+            }
+            __syncwarp();                                                    // in place: every lane has read its row
+            if (live && in && kind == 0) store8((T *)a.q_out + (size_t)tok * a.q_out_ld + (size_t)hh * D + d0, u, f, p.vec);
+            if (live && in && kind == 1 && a.k_out) store8((T *)a.k_out + (size_t)tok * a.k_out_ld + (size_t)hh * D + d0, u, f, p.vec);
+            if (keep && lane < 4 * p.c.ng) {
+                const int j = lane >> 2, t = lane & 3, ng = p.c.ng;
+                uint8_t *at = tile + (size_t)hh * p.c.tiles * p.c.tile_bytes;
+                if (kind == 1) {
+                    *(uint32_t *)(at + tr * 16 * ng + (t * ng + j) * 4) = held.codes;
+                } else {
+                    uint16_t *v = (uint16_t *)(at + 256 * ng + tr * 16 * ng);
+                    v[2 * t * ng + j] = (uint16_t)held.codes;
+                    v[(2 * t + 1) * ng + j] = (uint16_t)(held.codes >> 16);
+                }
+                if (t == 0) {
+                    uint8_t *s = at + (kind == 1 ? p.c.k_scales() : p.c.v_scales()) + (tr * ng + j) * p.c.sb;
+                    if (p.mx) *s = (uint8_t)held.scale;
+                    else *(uint16_t *)s = (uint16_t)held.scale;
+                }
+            }
+        }
+    }
+}
+
+// ---- load
+
+struct LoadArgs {
+    Kv4Dev c;
+    int mx, n;
+    void *k, *v;
+    const int32_t *slots;
+};
+
+__device__ __forceinline__ float code_value(unsigned nib, int mx) {
+    if (!mx) return (float)(int)nib - 8.0f;
+    const float m = (float)((0xC8643210u >> (4 * (nib & 7))) & 15) * 0.5f;
+    return nib & 8 ? -m : m;
+}
+__device__ __forceinline__ float scale_value(const uint8_t *p, int mx) {
+    return mx ? (*p ? __uint_as_float((uint32_t)*p << 23) : __uint_as_float(0x00400000u)) : __half2float(*(const __half *)p);
+}
+
+// One thread per 8 values of one row.
+template <typename T>
+__global__ void __launch_bounds__(256) load_kernel(const LoadArgs p) {
+    const int parts = p.c.dim / 8;
+    const long long items = (long long)p.n * p.c.n_kv * parts * 2;
+    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < items; i += gridDim.x * 256LL) {
+        const int c = (int)(i % parts);
+        long long r = i / parts;
+        const int head = (int)(r % p.c.n_kv);
+        r /= p.c.n_kv;
+        const int row = (int)(r % p.n), is_v = (int)(r / p.n);
+        T *out = (T *)(is_v ? p.v : p.k);
+        const int slot = p.slots[row];
+        if (!out || slot < 0 || slot >= p.c.n_pages * p.c.page) continue;
+        const int page = slot / p.c.page, off = slot - page * p.c.page, tr = off % kKvTile, j = c >> 2, t = c & 3, ng = p.c.ng;
+        const uint8_t *tile = p.c.data + p.c.tile_at(page, head, off / kKvTile);
+        const uint8_t *codes = tile + (is_v ? 256 * ng : 0) + tr * 16 * ng;
+        uint32_t w;
+        if (is_v) w = ((const uint16_t *)codes)[2 * t * ng + j] | (uint32_t)((const uint16_t *)codes)[(2 * t + 1) * ng + j] << 16;
+        else w = ((const uint32_t *)codes)[t * ng + j];
+        const float s = scale_value(tile + (is_v ? p.c.v_scales() : p.c.k_scales()) + (tr * ng + j) * p.c.sb, p.mx);
+        T *dst = out + ((size_t)row * p.c.n_kv + head) * p.c.dim + c * 8;
+        for (int e = 0; e < 8; e++) from_f32(dst + e, code_value(w >> (4 * e) & 15, p.mx) * s);
+    }
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
+    return sms;
+}
+
+}  // namespace
+
+extern "C" {
+
+L3M_API size_t l3m_kv4_page_bytes(int dtype, int n_kv_heads, int head_dim, int page) {
+    l3m_kv4 c = {nullptr, dtype, 0, page, n_kv_heads, head_dim};
+    if (kv4_shape_error(&c)) return 0;
+    const Kv4Dev d = kv4_dev(&c);
+    return (size_t)d.tile_bytes * d.tiles * d.n_kv;
+}
+
+L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream) {
+    const char *me = "l3m_kv4_plan_dev";
+    if (!a) return refuse(me, "arguments are required");
+    if (a->n_req < 0 || a->n_req > kPlanMaxReq) return refuse(me, "n_req must be 0 to 16384");
+    if (a->page < kKvTile || a->page > 4096 || a->page % kKvTile) return refuse(me, "page must be a multiple of 16 from 16 to 4096");
+    if (a->max_blocks < 0 || a->max_tokens < 0 || a->n_pages < 0 || (int64_t)a->n_pages * a->page > 0x7fffffff)
+        return refuse(me, "max_blocks, max_tokens and n_pages must not be negative, n_pages * page below 2^31");
+    if (!a->n_free || !a->n_free_out || !a->q_start || (a->n_pages && !a->free_pages) || (a->max_tokens && (!a->slot || !a->pos)) ||
+        (a->n_req && (!a->kv_len || !a->new_len || !a->kv_total || (a->max_blocks && !a->tables))))
+        return refuse(me, "a pointer is missing");
+    if (a->n_free == a->n_free_out || (a->n_req && (a->kv_total == a->kv_len || a->kv_total == a->new_len)))
+        return refuse(me, "n_free_out must not be n_free, nor kv_total kv_len or new_len");
+    if (((uintptr_t)a->kv_len | (uintptr_t)a->new_len | (uintptr_t)a->tables | (uintptr_t)a->free_pages | (uintptr_t)a->n_free | (uintptr_t)a->n_free_out |
+         (uintptr_t)a->q_start | (uintptr_t)a->kv_total | (uintptr_t)a->slot | (uintptr_t)a->pos | (uintptr_t)a->status) & 3)
+        return refuse(me, "a pointer is not aligned to its type");
+    PlanArgs p = {*a};
+    const size_t smem = (size_t)3 * (a->n_req + 1) * 4 + a->n_req;
+    const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e != cudaSuccess) return l3m_error_cuda(e, me);
+    const int grid = std::max(1, std::min(sm_count(), (a->max_tokens + kPlanThreads - 1) / kPlanThreads));
+    plan_kernel<<<grid, kPlanThreads, smem, (cudaStream_t)stream>>>(p);
+    return launched(me);
+}
+
+L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *stream) {
+    const char *me = "l3m_qkv_rope_dev";
+    if (!a) return refuse(me, "arguments are required");
+    if (a->dtype != L3M_DT_F32 && a->dtype != L3M_DT_BF16) return refuse(me, "dtype must be f32 or bf16");
+    if (a->n_tokens < 0 || a->n_heads < 0 || a->n_kv_heads < 0 || a->n_heads > 65535 || a->n_kv_heads > 65535) return refuse(me, "bad token or head counts");
+    if (a->head_dim < 8 || a->head_dim > 256 || a->head_dim % 8) return refuse(me, "head_dim must be a multiple of 8 from 8 to 256");
+    if (a->rope < 0 || a->rope > 2) return refuse(me, "rope must be 0, 1 or 2");
+    if (a->rope && (a->rot_dim < 0 || a->rot_dim % 2 || a->rot_dim > a->head_dim || a->n_pos < 0 || (a->rot_dim && a->n_pos && !a->rope_table)))
+        return refuse(me, "the rotation needs an even rot_dim up to head_dim and a table of n_pos rows");
+    if (!(a->eps >= 0.0f) || std::isinf(a->eps)) return refuse(me, "eps must be finite and not negative");
+    if (cache) {
+        if (const char *why = kv4_error(cache)) return refuse(me, why);
+        if (cache->n_kv_heads != a->n_kv_heads || cache->head_dim != a->head_dim) return refuse(me, "the cache has another n_kv_heads or head_dim");
+        if (a->n_kv_heads && a->n_tokens && (!a->k || !a->v || !a->slot)) return refuse(me, "a cache needs k, v and slot");
+    }
+    if (!a->n_tokens || !(a->n_heads + a->n_kv_heads)) return 0;
+    if (!a->pos) return refuse(me, "pos is required");
+    if (a->n_heads && (!a->q || !a->q_out)) return refuse(me, "q and q_out are required");
+    if (!cache && a->k_out && !a->k) return refuse(me, "k_out needs k");
+    const int64_t qw = (int64_t)a->n_heads * a->head_dim, kw = (int64_t)a->n_kv_heads * a->head_dim;
+    const bool with_k = a->n_kv_heads && a->k && (cache || a->k_out), with_v = cache && a->n_kv_heads;
+    if ((a->n_heads && (a->q_ld < qw || a->q_out_ld < qw)) || (with_k && (a->k_ld < kw || (a->k_out && a->k_out_ld < kw))) || (with_v && a->v_ld < kw))
+        return refuse(me, "a token stride is smaller than its heads");
+    const uintptr_t mask = a->dtype == L3M_DT_F32 ? 3 : 1;
+    if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->k_out) & mask) ||
+        (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm | (uintptr_t)a->rope_table | (uintptr_t)a->pos | (uintptr_t)a->slot) & 3))
+        return refuse(me, "a pointer is not aligned to its type");
+    const int kv_rows = (with_k ? a->n_kv_heads : 0) + (with_v ? a->n_kv_heads : 0), heads = a->n_heads + kv_rows;
+    if (!heads) return 0;
+    if (a->rope && ((uintptr_t)a->rope_table & 7)) return refuse(me, "rope_table must be 8-byte aligned");
+    QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, heads, 1, heads};
+    if (cache) p.c = kv4_dev(cache);
+    // 16-byte accesses where every row of every tensor starts on 16 bytes.
+    const int per16 = a->dtype == L3M_DT_F32 ? 4 : 8;
+    uintptr_t at = 0;
+    int64_t ld = 0;
+    if (a->n_heads) at |= (uintptr_t)a->q | (uintptr_t)a->q_out, ld |= a->q_ld | a->q_out_ld;
+    if (with_k) at |= (uintptr_t)a->k, ld |= a->k_ld;
+    if (with_k && a->k_out) at |= (uintptr_t)a->k_out, ld |= a->k_out_ld;
+    if (with_v) at |= (uintptr_t)a->v, ld |= a->v_ld;
+    p.vec = !(at & 15) && ld % per16 == 0;
+    const int rope = a->rope && a->rot_dim ? a->rope : 0;
+    const int ng = (a->head_dim + kKvBlock - 1) / kKvBlock, lpr = ng == 1 ? 4 : ng == 2 ? 8 : ng <= 4 ? 16 : 32;
+    // One warp per token takes all its rows when there are tokens enough to fill the GPU; else its rows are shared out.
+    const int sms = sm_count(), groups = (heads * lpr + 31) / 32;
+    const long long want = (32LL * sms + a->n_tokens - 1) / a->n_tokens;
+    p.chunks = (int)std::min<long long>(std::max(1LL, want), groups);
+    p.per_chunk = (groups + p.chunks - 1) / p.chunks * (32 / lpr);
+    p.chunks = (heads + p.per_chunk - 1) / p.per_chunk;
+    const long long warps = (long long)a->n_tokens * p.chunks;
+    const int grid = (int)std::min<long long>(8LL * sms, (warps + kQkvThreads / 32 - 1) / (kQkvThreads / 32));
+    const cudaStream_t s = (cudaStream_t)stream;
+    auto go = [&](auto t, auto r) {
+        typedef decltype(t) T;
+        constexpr int R = decltype(r)::value;
+        if (lpr == 4) qkv_kernel<T, 4, R><<<grid, kQkvThreads, 0, s>>>(p);
+        else if (lpr == 8) qkv_kernel<T, 8, R><<<grid, kQkvThreads, 0, s>>>(p);
+        else if (lpr == 16) qkv_kernel<T, 16, R><<<grid, kQkvThreads, 0, s>>>(p);
+        else qkv_kernel<T, 32, R><<<grid, kQkvThreads, 0, s>>>(p);
+    };
+    auto by_rope = [&](auto t) {
+        if (rope == 0) go(t, std::integral_constant<int, 0>{});
+        else if (rope == 1) go(t, std::integral_constant<int, 1>{});
+        else go(t, std::integral_constant<int, 2>{});
+    };
+    if (a->dtype == L3M_DT_F32) by_rope(float{});
+    else by_rope(__nv_bfloat16{});
+    return launched(me);
+}
+
+L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, const int32_t *slots, int n, void *stream) {
+    const char *me = "l3m_kv4_load_dev";
+    if (const char *why = kv4_error(cache)) return refuse(me, why);
+    if (dtype != L3M_DT_F32 && dtype != L3M_DT_BF16) return refuse(me, "dtype must be f32 or bf16");
+    if (n < 0) return refuse(me, "n must not be negative");
+    if (n == 0 || (!k && !v)) return 0;
+    if (!slots) return refuse(me, "slots are required");
+    if (((uintptr_t)k | (uintptr_t)v) & (dtype == L3M_DT_F32 ? 3 : 1) || (uintptr_t)slots & 3) return refuse(me, "a pointer is not aligned to its type");
+    const LoadArgs p = {kv4_dev(cache), cache->dtype == L3M_DT_MXFP4, n, k, v, slots};
+    const long long items = (long long)n * cache->n_kv_heads * (cache->head_dim / 8) * 2;
+    const int grid = (int)std::min<long long>(16LL * sm_count(), (items + 255) / 256);
+    if (dtype == L3M_DT_F32) load_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+    else load_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
+    return launched(me);
+}
+
+}  // extern "C"
