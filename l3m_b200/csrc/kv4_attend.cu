@@ -23,67 +23,840 @@ int refuse(const char *entry, const char *why) {
 struct AttendArgs {
     l3m_kv4_attend a;
     Kv4Dev c;
-    int mx;
+    int group, row_tiles;                 // query heads per kv head; row tiles of a request with max_q queries
+    int split;                            // 1: workers share all tiles out evenly, 0: a worker takes whole segments
+    float *part;                          // [workers][2] partial results of [rows][Dp + 2] floats: values, then reference and sum
+    int4 *desc;                           // [workers]: the segment whose last piece the worker did and where it began
 };
 
-__device__ __forceinline__ float to_f32(float x) { return x; }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f32(float *p, float x) { *p = x; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+// ---- warp pieces
 
-__device__ __forceinline__ float code_value(unsigned nib, int mx) {
-    if (!mx) return (float)(int)nib - 8.0f;
-    const float m = (float)((0xC8643210u >> (4 * (nib & 7))) & 15) * 0.5f;
-    return nib & 8 ? -m : m;
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+    return d;
 }
-__device__ __forceinline__ float scale_value(const uint8_t *p, int mx) {
-    return mx ? (*p ? __uint_as_float((uint32_t)*p << 23) : __uint_as_float(0x00400000u)) : __half2float(*(const __half *)p);
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+// Two floats rounded to f16 (lo in the low half).
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t v) {
+    const __half2 h = *(const __half2 *)&v;
+    return __half22float2(h);
+}
+// The 8x8 f16 matrix held as accumulators are (row lane / 4, columns 2 * (lane % 4)), transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+    uint32_t d;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(v));
+    return d;
+}
+__device__ __forceinline__ void mma(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+// Two e2m1 codes (a byte, the low nibble first) as f16.
+__device__ __forceinline__ uint32_t e2m1_pair(uint32_t byte) {
+    uint32_t d;
+    asm("{ .reg .b8 c, z0, z1, z2;\n mov.b32 {c, z0, z1, z2}, %1;\n cvt.rn.f16x2.e2m1x2 %0, c; }" : "=r"(d) : "r"(byte));
+    return d;
 }
 
-// One warp per query row, one cached token at a time: lane l holds dims l + 32 j. The softmax runs with the
-// row's running maximum and sum.
-template <typename T>
-__global__ void __launch_bounds__(256) attend_rows(const AttendArgs p) {
-    const l3m_kv4_attend &a = p.a;
-    const int lane = threadIdx.x & 31;
-    const long long rows = (long long)a.max_q * a.n_req * a.n_heads;
-    for (long long i = blockIdx.x * 8LL + (threadIdx.x >> 5); i < rows; i += gridDim.x * 8LL) {
-        const int h = (int)(i % a.n_heads);
-        const int r = (int)(i / a.n_heads % a.n_req), q = (int)(i / a.n_heads / a.n_req);
-        const int start = a.q_start[r], nq = a.q_start[r + 1] - start;
-        if (q >= nq) continue;
-        const int kv = min(max(a.kv_len[r], 0), a.max_kv), pos = kv - nq + q;
-        const int lo = a.window ? max(0, pos - a.window + 1) : 0;
-        const int kh = h / (a.n_heads / p.c.n_kv), ng = p.c.ng, jt = (lane >> 3) * ng, gt = (lane >> 2) * ng;
-        const T *qp = (const T *)a.q + (size_t)(start + q) * a.q_ld + (size_t)h * p.c.dim;
-        float x[8], o[8] = {}, m = -INFINITY, l = 0.0f;
-        for (int j = 0; j < ng; j++) x[j] = lane + 32 * j < p.c.dim ? to_f32(qp[lane + 32 * j]) * a.scale : 0.0f;
-        for (int t = lo; t <= pos; t++) {
-            const int id = a.tables[(size_t)r * a.max_blocks + t / p.c.page], off = t % p.c.page, tr = off % kKvTile;
-            if (id < 0 || id >= p.c.n_pages) {
-                if (a.status && lane == 0) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
-                continue;
-            }
-            const uint8_t *tile = p.c.data + p.c.tile_at(id, kh, off / kKvTile);
-            float s = 0.0f;
-            for (int j = 0; j < ng; j++) {
-                const uint8_t b = tile[tr * 16 * ng + (jt + j) * 4 + (lane & 7) / 2];
-                s = fmaf(x[j], code_value(lane & 1 ? b >> 4 : b & 15, p.mx) * scale_value(tile + p.c.k_scales() + (tr * ng + j) * p.c.sb, p.mx), s);
-            }
-            for (int d = 16; d; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
-            const float mn = fmaxf(m, s), fix = m == -INFINITY ? 0.0f : expf(m - mn), w = expf(s - mn);
-            m = mn;
-            l = fmaf(l, fix, w);
-            for (int j = 0; j < ng; j++) {
-                const uint8_t b = tile[256 * ng + tr * 16 * ng + (gt + j) * 2 + (lane & 3) / 2];
-                const float v = code_value(lane & 1 ? b >> 4 : b & 15, p.mx) * scale_value(tile + p.c.v_scales() + (tr * ng + j) * p.c.sb, p.mx);
-                o[j] = fmaf(w, v, o[j] * fix);
+// N 32-bit words from shared memory in the widest accesses that N words' alignment allows.
+template <int N> __device__ __forceinline__ void lds_words(uint32_t *w, const uint8_t *p) {
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 4; i++) {
+            const uint4 v = ((const uint4 *)p)[i];
+            w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+        }
+    } else if constexpr (N % 2 == 0) {
+#pragma unroll
+        for (int i = 0; i < N / 2; i++) {
+            const uint2 v = ((const uint2 *)p)[i];
+            w[2 * i] = v.x; w[2 * i + 1] = v.y;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i] = ((const uint32_t *)p)[i];
+    }
+}
+// N 16-bit values, two to a word.
+template <int N> __device__ __forceinline__ void lds_halves(uint32_t *w, const uint8_t *p) {
+    if constexpr (N % 2 == 0) {
+        lds_words<N / 2>(w, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; i += 2) w[i / 2] = ((const uint16_t *)p)[i] | (i + 1 < N ? (uint32_t)((const uint16_t *)p)[i + 1] << 16 : 0u);
+    }
+}
+// N bytes, four to a word.
+template <int N> __device__ __forceinline__ void lds_bytes(uint32_t *w, const uint8_t *p) {
+    if constexpr (N % 4 == 0) {
+        lds_words<N / 4>(w, p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < (N + 3) / 4; i++) w[i] = 0;
+#pragma unroll
+        for (int i = 0; i < N; i++) w[i / 4] |= (uint32_t)p[i] << (8 * (i % 4));
+    }
+}
+// Halves h of a (low) and of b (high).
+__device__ __forceinline__ uint32_t pair_of(const uint32_t *a, const uint32_t *b, int h) { return prmt(a[h / 2], b[h / 2], h % 2 ? 0x7632 : 0x5410); }
+
+__device__ __forceinline__ float load_f32(const float *p) { return *p; }
+__device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store_f32(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
+
+constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kStages = 4;               // tiles of a warp's ring
+constexpr int kMaxSms = 160;
+constexpr float kFloor = -1e30f;         // the reference of a row that has seen nothing
+
+// Resident CTAs per SM that the registers of a variant allow.
+constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 2 ? 4 : ng * nt <= 4 ? 3 : 2; }
+
+struct Segment { int r, h, rt; };
+
+// One piece of a segment (request r, kv head h, row tile rt): cache tiles [a, b), by the CTA's warps. Scores are
+// computed transposed, S^T = K Q^T (16 tokens x 8 rows a product), so that a decode step's few rows pad to 8, not 16, and
+// O^T = V^T P^T follows from it with one 8x8 transposition per 8 tokens. Each warp keeps its own softmax reference and
+// sums over its tiles a + warp, a + warp + 4, ...; the warps are joined at the end.
+//
+// Codes go into the products as the integers they are, so that the cache's values suffer no rounding. For q4_0 and bf16 results a
+// nibble in the low byte of a half is an f16 subnormal, n * 2^-24 (or n * 2^-20 four bits higher): one mask, no conversion. Its offset
+// of 8 is taken off the sum instead: scores start at -8 sum(q), and the sum of P times scale, which the values' offset multiplies,
+// comes from one more product with ones. Float results use n - 8 itself (one more f16 operation), so that nothing cancels.
+// A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
+// them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
+// split in two f16 for float ones.
+template <typename T, int MX, int NG, int NT>
+struct Worker {
+    static constexpr bool PREC = sizeof(T) == 4;
+    static constexpr bool SUBN = !PREC && !MX;
+    static constexpr int NR = 8 * NT, DP = 32 * NG, SB = MX ? 1 : 2;
+    static constexpr int TB = NG * (512 + 32 * SB);
+    static constexpr int RING = kStages * TB;
+    static constexpr int SMEM = kWarps * RING > kWarps * NR * (DP + 4) * 4 ? kWarps * RING : kWarps * NR * (DP + 4) * 4;
+    static constexpr int QP = PREC ? 2 : 1;
+    static constexpr int SW = MX ? (NG + 3) / 4 : (NG + 1) / 2;              // words of a row's scales
+
+    const AttendArgs &p;
+    uint8_t *smem;
+    int warp, lane, g, t;
+    uint32_t q[QP][NT][NG][4];            // B fragments of the rows: [high, low part][row][block][2 steps x 2]
+    float c0[SUBN ? NT : 1][SUBN ? NG : 1][2];
+    float mult[NT][2];
+    int pos[NT][2];
+    float ref[NT][2], sum[NT][2];
+    float o[NT][NG][2][4];
+    float w[SUBN ? NT : 1][SUBN ? NG : 1][4];
+    int vexp, eref;
+
+    __device__ Worker(const AttendArgs &args, uint8_t *sm) : p(args), smem(sm) {
+        warp = threadIdx.x >> 5;
+        lane = threadIdx.x & 31;
+        g = lane >> 2;
+        t = lane & 3;
+    }
+    // Row r of a 16-token product is token tau(r): a warp's reads of keys (rows g) and of values (tokens of k = 2t, 2t + 1) then spread over the banks.
+    __device__ static int tau(int r) { return (r & 8) | (r & 1 ? 4 + (((r >> 1) & 3) ^ 1) : (r >> 1) & 3); }
+
+    __device__ __forceinline__ void load_rows(int start, int nq, int kv, int h, int rt) {
+        float m8[NT], cs[NT][NG];
+        const float log2e = 1.4426950408889634f;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            const int row = rt * NR + n * 8 + g, i = row / p.group, head = h * p.group + row - i * p.group;
+            const T *src = (const T *)p.a.q + (size_t)(start + i) * p.a.q_ld + (size_t)head * p.c.dim;
+            float x[NG][8], top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NG; j++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const int d = 32 * j + 8 * t;
+                    x[j][e] = i < nq && d < p.c.dim ? load_f32(src + d + e) : 0.0f;
+                    top = fmaxf(top, fabsf(x[j][e]));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int up = top > 0.0f ? 9 - max(min(ilogbf(top), 127), -149) : 0;      // |x| * 2^up < 2^10
+            m8[n] = ldexpf(p.a.scale * log2e, (SUBN ? 24 : 0) - up);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                float s = 0.0f;
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    // q4_0: nibbles k and k + 4 make a pair; mxfp4: the two of a byte
+                    const float a = ldexpf(x[j][MX ? 2 * k : k], up), b = ldexpf(x[j][MX ? 2 * k + 1 : k + 4], up);
+                    const float down = SUBN && (k & 1) ? 0.0625f : 1.0f;
+                    q[0][n][j][k] = pack_f16(a * down, b * down);
+                    const float2 back = unpack_f16(q[0][n][j][k]);
+                    if (PREC) q[QP - 1][n][j][k] = pack_f16(a - back.x, b - back.y);
+                    s += SUBN && (k & 1) ? (back.x + back.y) * 16.0f : back.x + back.y;
+                }
+                cs[n][j] = s;
             }
         }
-        T *op = (T *)a.out + (size_t)(start + q) * a.out_ld + (size_t)h * p.c.dim;
-        for (int j = 0; j < ng; j++)
-            if (lane + 32 * j < p.c.dim) from_f32(op + lane + 32 * j, l > 0.0f ? o[j] / l : 0.0f);
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int j = 0; j < NG && SUBN; j++) {
+                cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 1);
+                cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 2);
+                c0[n][j][0] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t) * -0x1p-21f;
+                c0[n][j][1] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t + 4) * -0x1p-21f;
+            }
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                mult[n][c] = __shfl_sync(0xffffffffu, m8[n], 8 * t + 4 * c);
+                const int i = (rt * NR + n * 8 + 2 * t + c) / p.group;
+                pos[n][c] = i < nq ? kv - nq + i : -1;
+                ref[n][c] = kFloor;
+                sum[n][c] = 0.0f;
+            }
+#pragma unroll
+            for (int j = 0; j < NG; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    o[n][j][0][e] = o[n][j][1][e] = 0.0f;
+                    if (SUBN) w[n][j][e] = 0.0f;
+                }
+        }
+        vexp = PREC && !MX ? -16 : 0;                                              // P itself is held in f16 for bf16 results: 2^14 at most
+        eref = 15;
     }
+
+    __device__ __forceinline__ void scale_rows(int n, float f0, float f1) {
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+#pragma unroll
+            for (int m = 0; m < 2; m++) {
+                o[n][j][m][0] *= f0; o[n][j][m][1] *= f1;
+                o[n][j][m][2] *= f0; o[n][j][m][3] *= f1;
+            }
+            if (SUBN) {
+                w[n][j][0] *= f0; w[n][j][1] *= f1;
+            }
+        }
+    }
+
+    // One tile in shared memory. edge: some row does not see some of its tokens, which begin at tok0; [lo_any, hi_any) is seen by some row.
+    template <bool EDGE> __device__ __forceinline__ void tile(const uint8_t *sm, int tok0, int lo_any, int hi_any) {
+        // ---- scores
+        const int ra = tau(g);
+        uint32_t ka[NG], kb[NG], sa[SW], sb[SW];
+        lds_words<NG>(ka, sm + ra * 16 * NG + t * 4 * NG);
+        lds_words<NG>(kb, sm + (ra + 8) * 16 * NG + t * 4 * NG);
+        const uint8_t *ks = sm + 512 * NG, *vs = ks + 16 * NG * SB;
+        if (MX) {
+            lds_bytes<NG>(sa, ks + ra * NG);
+            lds_bytes<NG>(sb, ks + (ra + 8) * NG);
+        } else {
+            lds_halves<NG>(sa, ks + ra * NG * 2);
+            lds_halves<NG>(sb, ks + (ra + 8) * NG * 2);
+        }
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            uint32_t fa[4], fb[4];
+            codes4(fa, ka[j]);
+            codes4(fb, kb[j]);
+            float da, db;
+            if (MX) {
+                da = __uint_as_float((sa[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
+                db = __uint_as_float((sb[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
+            } else {
+                const float2 a2 = unpack_f16(sa[j / 2]), b2 = unpack_f16(sb[j / 2]);
+                da = j % 2 ? a2.y : a2.x;
+                db = j % 2 ? b2.y : b2.x;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float acc[4];
+                if (SUBN) {
+                    acc[0] = acc[2] = c0[SUBN ? n : 0][SUBN ? j : 0][0];
+                    acc[1] = acc[3] = c0[SUBN ? n : 0][SUBN ? j : 0][1];
+                } else {
+                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                }
+                if (PREC) {
+                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[QP - 1][n][j][0], q[QP - 1][n][j][1]);
+                    mma(acc, fa[2], fb[2], fa[3], fb[3], q[QP - 1][n][j][2], q[QP - 1][n][j][3]);
+                }
+                mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                mma(acc, fa[2], fb[2], fa[3], fb[3], q[0][n][j][2], q[0][n][j][3]);
+                s[n][0] = fmaf(acc[0], da, s[n][0]);
+                s[n][1] = fmaf(acc[1], da, s[n][1]);
+                s[n][2] = fmaf(acc[2], db, s[n][2]);
+                s[n][3] = fmaf(acc[3], db, s[n][3]);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s[n][e] *= mult[n][e & 1];
+                if (EDGE) {
+                    const int tok = tok0 + ra + (e & 2 ? 8 : 0), at = pos[n][e & 1];
+                    if (tok > at || (p.a.window && tok <= at - p.a.window)) s[n][e] = -INFINITY;
+                }
+            }
+        // ---- the values' scales: of this lane's tokens as P's transposed pairs want them, or (float results) as the scores lie
+        uint32_t v0[SW], v1[SW], v2[SW], v3[SW];
+        const int t0 = PREC ? ra : t, t1 = 4 + (t ^ 1);
+        auto scales = [&](uint32_t *x, int row) {
+            if (MX) lds_bytes<NG>(x, vs + row * NG);
+            else lds_halves<NG>(x, vs + row * NG * 2);
+            if (EDGE) {
+                const int tok = tok0 + row;
+                const bool gone = tok < lo_any || tok >= hi_any;
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    if (!MX) {                                               // infinities and NaN that some row does not see must not meet its zeros
+                        if ((x[i] & 0x7c00u) == 0x7c00u) x[i] &= 0xffff0000u;
+                        if ((x[i] & 0x7c000000u) == 0x7c000000u) x[i] &= 0x0000ffffu;
+                    }
+                    if (gone) x[i] = 0;
+                }
+            }
+        };
+        scales(v0, t0);
+        if (!PREC) scales(v1, t1);
+        scales(v2, t0 + 8);
+        if (!PREC) scales(v3, t1 + 8);
+        // ---- does the reference still hold? P <= 2^lim, |scale| < 2^(vexp + 1) (mxfp4: scales are taken relative to eref, vexp stays)
+        bool move = false;
+        if (MX) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int i = 0; i < SW; i++) {
+                top = __vmaxu4(top, __vmaxu4(v0[i], v2[i]));
+                if (!PREC) top = __vmaxu4(top, __vmaxu4(v1[i], v3[i]));
+            }
+            const uint32_t two = __vmaxu4(top, top >> 16);
+            move = (int)max(two & 0xff, two >> 8 & 0xff) > eref;
+        } else {
+            uint32_t any = 0;
+            if (PREC) {
+#pragma unroll
+                for (int i = 0; i < SW; i++) any = __vmaxu2(any, __vmaxu2(v0[i] & 0x7fff7fffu, v2[i] & 0x7fff7fffu));
+                move = (int)max(any >> 10 & 31, any >> 26) - 15 > vexp;
+            } else {
+#pragma unroll
+                for (int i = 0; i < SW; i++) any |= v0[i] | v1[i] | v2[i] | v3[i];
+                move = (any & 0x40004000u) && vexp < 16;
+            }
+        }
+        float lim = 14.0f - (float)vexp;
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+            move |= fmaxf(s[n][0], s[n][2]) > ref[n][0] + lim;
+            move |= fmaxf(s[n][1], s[n][3]) > ref[n][1] + lim;
+        }
+        if (__any_sync(0xffffffffu, move)) {
+            int top = 0;
+#pragma unroll
+            for (int i = 0; i < SW; i++) {
+                const uint32_t all[4] = {v0[i], v2[i], PREC ? 0u : v1[i], PREC ? 0u : v3[i]};
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    if (MX) {
+                        top = max(max(top, (int)(all[k] & 0xff)), max((int)(all[k] >> 8 & 0xff), max((int)(all[k] >> 16 & 0xff), (int)(all[k] >> 24))));
+                    } else {
+                        top = max(top, max((int)(all[k] >> 10 & 31), (int)(all[k] >> 26 & 31)));
+                    }
+                }
+            }
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+            float shrink = 1.0f;
+            if (MX) {
+                if (top > eref) {
+                    shrink = top - eref > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (top - eref)) << 23);
+                    eref = top;
+                }
+            } else {
+                vexp = max(vexp, top - 15);
+                lim = 14.0f - (float)vexp;
+            }
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                float f[2];
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float m = fmaxf(s[n][c], s[n][c + 2]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    f[c] = 1.0f;
+                    if (m > ref[n][c] + lim) {
+                        const float to = m - lim + 4.0f;                     // room for 2^4 before the next move
+                        f[c] = ex2(ref[n][c] - to);
+                        ref[n][c] = to;
+                    }
+                    sum[n][c] *= f[c];
+                }
+                scale_rows(n, f[0] * shrink, f[1] * shrink);
+            }
+        }
+        // ---- probabilities
+        uint32_t pb[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[n][e] = ex2(s[n][e] - ref[n][e & 1]);
+            sum[n][0] += s[n][0] + s[n][2];
+            sum[n][1] += s[n][1] + s[n][3];
+            if (!PREC) {
+                pb[n][0] = transpose8(pack_f16(s[n][0], s[n][1]));
+                pb[n][1] = transpose8(pack_f16(s[n][2], s[n][3]));
+            }
+        }
+        // ---- values
+        uint32_t c[4][(NG + 1) / 2];
+        const uint8_t *vc = sm + 256 * NG + g * 2 * NG;
+        lds_halves<NG>(c[0], vc + t * 16 * NG);
+        lds_halves<NG>(c[1], vc + t1 * 16 * NG);
+        lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
+        lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
+#pragma unroll
+        for (int j = 0; j < NG; j++) {
+            uint32_t fa[4], fb[4];
+            value4(fa, c[0], c[1], j);
+            value4(fb, c[2], c[3], j);
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                if (PREC) {
+                    float d0, d1;
+                    if (MX) {
+                        d0 = rel_f32(v0[j / 4] >> (8 * (j % 4)) & 0xff);
+                        d1 = rel_f32(v2[j / 4] >> (8 * (j % 4)) & 0xff);
+                    } else {
+                        const float2 a2 = unpack_f16(v0[j / 2]), b2 = unpack_f16(v2[j / 2]);
+                        d0 = j % 2 ? a2.y : a2.x;
+                        d1 = j % 2 ? b2.y : b2.x;
+                    }
+                    const float x0 = s[n][0] * d0, x1 = s[n][1] * d0, x2 = s[n][2] * d1, x3 = s[n][3] * d1;
+                    const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
+                    const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
+                    const uint32_t l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y)), l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
+                    const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {                            // a tile's sum by itself: the accumulator of a product is truncated, not rounded
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
+                        mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n][j][m][e] += acc[e];
+                    }
+                } else {
+                    uint32_t d0, d1;
+                    if (MX) {
+                        d0 = rel_f16(v0[j / 4], v1[j / 4], j % 4);
+                        d1 = rel_f16(v2[j / 4], v3[j / 4], j % 4);
+                    } else {
+                        d0 = pair_of(v0, v1, j);
+                        d1 = pair_of(v2, v3, j);
+                    }
+                    const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
+                    mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
+                    mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
+                    if (SUBN) mma(w[SUBN ? n : 0][SUBN ? j : 0], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b0, b1);
+                }
+            }
+        }
+    }
+    // A word's 8 codes as four pairs.
+    __device__ __forceinline__ static void codes4(uint32_t *f, uint32_t x) {
+        if (MX) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) f[k] = e2m1_pair(x >> (8 * k));
+        } else {
+            const uint32_t y = x >> 8;
+            f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
+            f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
+            if (PREC) whole(f);
+        }
+    }
+    // Block j's 4 codes of two tokens as four pairs of the same dim.
+    __device__ __forceinline__ static void value4(uint32_t *f, const uint32_t *a, const uint32_t *b, int j) {
+        if (MX) {
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                const uint32_t x = e2m1_pair(a[j / 2] >> (16 * (j % 2) + 8 * k)), y = e2m1_pair(b[j / 2] >> (16 * (j % 2) + 8 * k));
+                f[2 * k] = prmt(x, y, 0x5410);
+                f[2 * k + 1] = prmt(x, y, 0x7632);
+            }
+        } else {
+            const uint32_t x = pair_of(a, b, j), y = x >> 8;
+            f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
+            f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
+            if (PREC) whole(f);
+        }
+    }
+    // n -> n - 8 in f16: 1024 + n (or 1024 + 16 n) is a number whose last bits are n.
+    __device__ __forceinline__ static void whole(uint32_t *f) {
+        const __half2 off = __halves2half2(__ushort_as_half(0xe408), __ushort_as_half(0xe408));   // -1032
+        const __half2 s16 = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));   // 1/16
+        const __half2 o16 = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));   // -72
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            uint32_t x = f[k] | 0x64006400u;
+            const __half2 h = *(const __half2 *)&x;
+            const __half2 r = k % 2 ? __hfma2(h, s16, o16) : __hadd2(h, off);
+            f[k] = *(const uint32_t *)&r;
+        }
+    }
+    // mxfp4 scales relative to eref: 2^(e - eref).
+    __device__ __forceinline__ float rel_f32(uint32_t e) const { return __uint_as_float((uint32_t)max((int)e - eref + 127, 0) << 23); }
+    __device__ __forceinline__ uint32_t rel_f16(uint32_t a, uint32_t b, int k) const {
+        const uint32_t x = prmt(a >> (8 * k), b >> (8 * k), 0x5410) & 0x00ff00ffu, base = (uint32_t)(eref - 15) * 0x10001u;
+        return (__vmaxs2(x, base) - base) << 10;
+    }
+
+    // Cache tiles [a, b) of request r's head h into the rows' sums.
+    __device__ __forceinline__ void run(int r, int h, int rt, int nq, int kv, int a, int b) {
+        const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
+        const int i0 = rt * NR / p.group, i1 = min((rt * NR + NR - 1) / p.group, nq - 1);
+        const int first = kv - nq + i0, last = kv - nq + i1;                 // the rows' positions
+        const int lo_any = p.a.window ? first - p.a.window + 1 : 0, hi_any = last + 1;
+        const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;   // seen by every row
+        uint8_t *ring = smem + warp * RING;
+        const int n = a + warp < b ? (b - a - warp + kWarps - 1) / kWarps : 0;    // this warp's tiles
+        long long at = -1;                                                        // lane i: where its tile 32 * (k / 32) + i lies
+        auto locate = [&](int k) {
+            at = -1;
+            if (k + lane < n) {
+                const int tl = a + warp + (k + lane) * kWarps, blk = tl / p.c.tiles, id = table[blk];
+                if (id >= 0 && id < p.c.n_pages) at = (long long)p.c.tile_at(id, h, tl - blk * p.c.tiles);
+                else if (p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
+            }
+        };
+        uint32_t good = 0;                                                        // which of the ring's tiles are there
+        auto fetch = [&](int k) {
+            if (k < n) {
+                if (k % 32 == 0) locate(k);
+                const long long from = __shfl_sync(0xffffffffu, at, k % 32);
+                const int st = k % kStages;
+                good = from < 0 ? good & ~(1u << st) : good | 1u << st;
+                if (from >= 0) {
+                    const uint8_t *src = p.c.data + from;
+                    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + st * TB);
+#pragma unroll
+                    for (int c = 0; c < TB; c += 512)
+                        if (c + 512 <= TB || c + lane * 16 < TB)
+                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c + lane * 16), "l"(src + c + lane * 16) : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        for (int k = 0; k < kStages - 1; k++) fetch(k);
+        for (int k = 0; k < n; k++) {
+            fetch(k + kStages - 1);
+            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            __syncwarp();
+            const int st = k % kStages;
+            if (good >> st & 1) {
+                const int tok0 = (a + warp + k * kWarps) * kKvTile;
+                if (tok0 >= whole_lo && tok0 + kKvTile <= whole_hi) tile<false>(ring + st * TB, tok0, lo_any, hi_any);
+                else tile<true>(ring + st * TB, tok0, lo_any, hi_any);
+            }
+            __syncwarp();
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+
+    // The warps' results joined; the rows' outputs, or a partial result.
+    __device__ __forceinline__ void finish(int start, int nq, int h, int rt, float *part) {
+        float *buf = (float *)smem;                                          // [warp][row][DP + 4]: values, reference, sum
+        constexpr int LD = DP + 4;
+        __syncthreads();                                                     // every warp is done with the ring
+#pragma unroll
+        for (int n = 0; n < NT; n++) {
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                float s = sum[n][c];
+                s += __shfl_xor_sync(0xffffffffu, s, 4);
+                s += __shfl_xor_sync(0xffffffffu, s, 8);
+                s += __shfl_xor_sync(0xffffffffu, s, 16);
+                float *row = buf + (warp * NR + n * 8 + 2 * t + c) * LD;
+                if (g == 0) {
+                    row[DP] = ref[n][c];
+                    row[DP + 1] = s;
+                }
+                const float unit = MX ? __uint_as_float((uint32_t)eref << 23) : 1.0f;
+#pragma unroll
+                for (int j = 0; j < NG; j++) {
+                    float v[4] = {o[n][j][0][c], o[n][j][0][2 + c], o[n][j][1][c], o[n][j][1][2 + c]};
+                    if (SUBN) {
+                        const float off = w[SUBN ? n : 0][SUBN ? j : 0][c] * 8.0f;
+                        v[0] = fmaf(v[0], 0x1p24f, -off); v[1] = fmaf(v[1], 0x1p20f, -off);
+                        v[2] = fmaf(v[2], 0x1p24f, -off); v[3] = fmaf(v[3], 0x1p20f, -off);
+                    }
+                    if (MX) v[0] *= unit, v[1] *= unit, v[2] *= unit, v[3] *= unit;
+                    *(float4 *)(row + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
+                }
+            }
+        }
+        __syncthreads();
+        constexpr int PER = DP / 4;
+        for (int i = threadIdx.x; i < NR * PER; i += kThreads) {
+            const int row = i / PER, d = (i - row * PER) * 4;
+            float m = kFloor, l = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < kWarps; k++) m = fmaxf(m, buf[(k * NR + row) * LD + DP]);
+#pragma unroll
+            for (int k = 0; k < kWarps; k++) {
+                const float *from = buf + (k * NR + row) * LD;
+                const float f = ex2(from[DP] - m);
+                const float4 x = *(const float4 *)(from + d);
+                l = fmaf(from[DP + 1], f, l);
+                v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            }
+            if (part) {
+                float *to = part + row * (DP + 4);
+                *(float4 *)(to + d) = v;
+                if (d == 0) *(float2 *)(to + DP) = make_float2(m, l);
+            } else {
+                put(start, nq, h, rt, row, d, v, l);
+            }
+        }
+        __syncthreads();                                                     // the buffer is the next piece's ring
+    }
+
+    __device__ __forceinline__ void put(int start, int nq, int h, int rt, int row8, int d, float4 v, float l) const {
+        const int row = rt * NR + row8, i = row / p.group;
+        if (i >= nq || d >= p.c.dim) return;
+        T *dst = (T *)p.a.out + (size_t)(start + i) * p.a.out_ld + (size_t)(h * p.group + row - i * p.group) * p.c.dim + d;
+        const float f = l != 0.0f ? 1.0f / l : 0.0f;
+        store_f32(dst, v.x * f);
+        store_f32(dst + 1, v.y * f);
+        store_f32(dst + 2, v.z * f);
+        store_f32(dst + 3, v.w * f);
+    }
+};
+
+struct Request { int start, nq, kv, lo, tiles, rts; };            // cache tiles [lo, lo + tiles), row tiles
+
+__device__ __forceinline__ Request request_of(const AttendArgs &p, int r, int nr) {
+    Request q;
+    q.start = p.a.q_start[r];
+    q.nq = max(p.a.q_start[r + 1] - q.start, 0);
+    q.kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
+    const int lo = p.a.window ? max(0, q.kv - q.nq - p.a.window + 1) : 0;
+    q.lo = lo / kKvTile;
+    q.tiles = max(1, (q.kv + kKvTile - 1) / kKvTile - q.lo);     // one at least: a request whose queries see nothing has rows to write
+    q.rts = (q.nq * p.group + nr - 1) / nr;
+    return q;
+}
+
+__device__ long long block_sum_scan(long long v, long long *ws, long long *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) ws[warp] = v;
+    __syncthreads();
+    long long all = 0;
+    for (int k = 0; k < kWarps; k++) {
+        if (k < warp) v += ws[k];
+        all += ws[k];
+    }
+    *total = all;
+    __syncthreads();
+    return v;
+}
+
+template <typename T, int MX, int NG, int NT>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(const AttendArgs p) {
+    typedef Worker<T, MX, NG, NT> W;
+    extern __shared__ __align__(16) uint8_t smem[];
+    W w(p, smem);
+    const int n_req = p.a.n_req, heads = p.c.n_kv;
+    // All segments' cache tiles in one line, request by request, head by head, row tile by row tile: a worker's share is [u0, u1).
+    // Not split, the line is of segments (the same number for each request), and a worker takes every gridDim.x-th.
+    __shared__ long long ws[kWarps];
+    __shared__ long long found_at;
+    __shared__ int found;
+    const int per_req = heads * p.row_tiles;
+    long long share = 1, u0 = blockIdx.x, u1 = (long long)n_req * per_req, at = 0;
+    int r = 0;
+    if (p.split) {
+        long long total = 0;
+        for (int c = 0; c < n_req; c += kThreads) {
+            const int i = c + threadIdx.x;
+            long long n = 0, sum;
+            if (i < n_req) {
+                const Request q = request_of(p, i, W::NR);
+                n = (long long)q.tiles * q.rts * heads;
+            }
+            block_sum_scan(n, ws, &sum);
+            total += sum;
+        }
+        share = (total + gridDim.x - 1) / gridDim.x;
+        share = max((share + kWarps - 1) / kWarps * kWarps, (long long)p.split);
+        u0 = share * blockIdx.x;
+        u1 = min(u0 + share, total);
+        long long base = 0;
+        for (int c = 0; c < n_req && u0 < u1; c += kThreads) {
+            const int i = c + threadIdx.x;
+            long long n = 0, sum;
+            if (i < n_req) {
+                const Request q = request_of(p, i, W::NR);
+                n = (long long)q.tiles * q.rts * heads;
+            }
+            const long long upto = base + block_sum_scan(n, ws, &sum);
+            if (upto - n <= u0 && u0 < upto) {
+                found = i;
+                found_at = upto - n;
+            }
+            base += sum;
+            if (u0 < base) break;
+        }
+        __syncthreads();
+        if (u0 < u1) {
+            r = found;
+            at = found_at;
+        }
+    }
+    int4 desc = make_int4(-1, 0, 0, 0);
+    while (u0 < u1) {
+        if (!p.split) {
+            r = (int)(u0 / per_req);
+            at = (long long)r * per_req;
+        }
+        const Request q = request_of(p, r, W::NR);
+        int x, off = 0, len = q.tiles, rts = p.row_tiles;
+        if (p.split) {
+            const long long n = (long long)q.tiles * q.rts * heads;
+            if (u0 >= at + n) {
+                at += n;
+                r++;
+                continue;
+            }
+            x = (int)((u0 - at) / q.tiles);
+            off = (int)(u0 - at - (long long)x * q.tiles);
+            len = (int)min((long long)(q.tiles - off), u1 - u0);
+            rts = q.rts;
+        } else {
+            x = (int)(u0 - at);
+        }
+        const int h = x / rts, rt = x - h * rts;
+        if (rt < q.rts) {
+            const int last = q.kv - q.nq + min((rt * W::NR + W::NR - 1) / p.group, q.nq - 1), top = last >= 0 ? last / kKvTile + 1 : 0;
+            const bool begins = off == 0, ends = off + len == q.tiles;
+            w.load_rows(q.start, q.nq, q.kv, h, rt);
+            w.run(r, h, rt, q.nq, q.kv, q.lo + off, min(q.lo + off + len, top));
+            w.finish(q.start, q.nq, h, rt, begins && ends ? nullptr : p.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * W::NR * (W::DP + 4));
+            if (!begins && ends) desc = make_int4((int)((u0 - off) / share), r, h, rt);
+        }
+        u0 += p.split ? len : gridDim.x;
+    }
+    if (p.split && threadIdx.x == 0) p.desc[blockIdx.x] = desc;
+}
+
+// The pieces of the segments that several workers shared: CTA (w, row) joins a row of the segment that ends in worker w.
+template <typename T, int MX, int NG, int NT>
+__global__ void __launch_bounds__(kThreads) join_kernel(const AttendArgs p) {
+    typedef Worker<T, MX, NG, NT> W;
+    constexpr int LD = W::DP + 4, SIZE = W::NR * LD;
+    const int4 d = p.desc[blockIdx.x];
+    if (d.x < 0) return;
+    const int row = blockIdx.y, own = blockIdx.x;
+    auto piece = [&](int k) { return p.part + ((size_t)k * 2 + (k == d.x ? 1 : 0)) * SIZE + row * LD; };
+    __shared__ float red[kWarps];
+    float m = kFloor;
+    for (int k = d.x + threadIdx.x; k <= own; k += kThreads) m = fmaxf(m, piece(k)[W::DP]);
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    for (int k = 0; k < kWarps; k++) m = fmaxf(m, red[k]);
+    for (int at = threadIdx.x * 4; at < W::DP; at += kThreads * 4) {
+        float l = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int k = d.x; k <= own; k++) {
+            const float *from = piece(k);
+            const float2 ml = *(const float2 *)(from + W::DP);
+            const float4 x = *(const float4 *)(from + at);
+            const float f = ex2(ml.x - m);
+            l = fmaf(ml.y, f, l);
+            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+        }
+        const Request q = request_of(p, d.y, W::NR);
+        W w(p, nullptr);
+        w.put(q.start, q.nq, d.z, d.w, row, at, v, l);
+    }
+}
+
+constexpr int kSplitFrom = 512;           // cached tokens from which segments are shared out
+constexpr int kLeastShare = 16;           // tiles of a worker's share
+
+int row_blocks(const l3m_kv4 *c, const l3m_kv4_attend *a) {
+    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
+    return rows > 8 && (c->head_dim + 31) / 32 <= 4 ? 2 : 1;
+}
+
+size_t part_floats(int nr, int ng) { return (size_t)2 * nr * (32 * ng + 4); }
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) return 148;
+    return std::min(sms, kMaxSms);
+}
+
+template <typename T, int MX, int NG, int NT>
+cudaError_t launch(AttendArgs p, cudaStream_t s) {
+    typedef Worker<T, MX, NG, NT> W;
+    cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, MX, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM);
+    if (e != cudaSuccess) return e;
+    const int workers = sm_count() * ctas_per_sm(NG, NT);
+    p.row_tiles = (int)(((long long)p.a.max_q * p.group + W::NR - 1) / W::NR);
+    p.split = p.a.max_kv > kSplitFrom ? kLeastShare : 0;
+    p.desc = (int4 *)p.a.scratch;
+    p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * ctas_per_sm(NG, NT) * sizeof(int4));
+    const long long segs = (long long)p.a.n_req * p.c.n_kv * p.row_tiles;
+    const int grid = p.split ? workers : (int)std::min<long long>(segs, 1 << 20);
+    attend_kernel<T, MX, NG, NT><<<grid, kThreads, W::SMEM, s>>>(p);
+    if (p.split) join_kernel<T, MX, NG, NT><<<dim3(workers, W::NR), kThreads, 0, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T, int MX, int NT>
+cudaError_t by_blocks(const AttendArgs &p, cudaStream_t s) {
+    switch (p.c.ng) {
+    case 1: return launch<T, MX, 1, NT>(p, s);
+    case 2: return launch<T, MX, 2, NT>(p, s);
+    case 3: return launch<T, MX, 3, NT>(p, s);
+    case 4: return launch<T, MX, 4, NT>(p, s);
+    default: break;
+    }
+    if constexpr (NT == 1) {
+        switch (p.c.ng) {
+        case 5: return launch<T, MX, 5, 1>(p, s);
+        case 6: return launch<T, MX, 6, 1>(p, s);
+        case 7: return launch<T, MX, 7, 1>(p, s);
+        default: return launch<T, MX, 8, 1>(p, s);
+        }
+    }
+    return cudaErrorInvalidValue;
 }
 
 const char *attend_error(const l3m_kv4 *c, const l3m_kv4_attend *a) {
@@ -102,7 +875,9 @@ extern "C" {
 
 L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend *a) {
     if (attend_error(cache, a)) return 0;
-    return 16;
+    if (a->max_kv <= kSplitFrom) return 16;
+    const int ng = (cache->head_dim + kKvBlock - 1) / kKvBlock, nt = row_blocks(cache, a);
+    return (size_t)kMaxSms * ctas_per_sm(ng, nt) * (sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
 }
 
 L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, void *stream) {
@@ -117,12 +892,17 @@ L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, vo
     if (((uintptr_t)a->q | (uintptr_t)a->out) & (a->dtype == L3M_DT_F32 ? 3 : 1) || ((uintptr_t)a->q_start | (uintptr_t)a->kv_len | (uintptr_t)a->tables) & 3)
         return refuse(me, "a pointer is not aligned to its type");
     if (!a->scratch || a->scratch_bytes < l3m_kv4_attend_scratch(cache, a) || ((uintptr_t)a->scratch & 15)) return refuse(me, "scratch is too small or not 16-byte aligned");
-    const AttendArgs p = {*a, kv4_dev(cache), cache->dtype == L3M_DT_MXFP4};
-    const long long rows = (long long)a->max_q * a->n_req * a->n_heads;
-    const int grid = (int)std::min<long long>(148 * 16, (rows + 7) / 8);
-    if (a->dtype == L3M_DT_F32) attend_rows<float><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    else attend_rows<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    const cudaError_t e = cudaGetLastError();
+    AttendArgs p = {*a, kv4_dev(cache), a->n_heads / cache->n_kv_heads, 0, 0, nullptr, nullptr};
+    const int mx = cache->dtype == L3M_DT_MXFP4, two = row_blocks(cache, a) == 2;
+    const cudaStream_t s = (cudaStream_t)stream;
+    cudaError_t e;
+    if (a->dtype == L3M_DT_F32) {
+        if (mx) e = two ? by_blocks<float, 1, 2>(p, s) : by_blocks<float, 1, 1>(p, s);
+        else e = two ? by_blocks<float, 0, 2>(p, s) : by_blocks<float, 0, 1>(p, s);
+    } else {
+        if (mx) e = two ? by_blocks<__nv_bfloat16, 1, 2>(p, s) : by_blocks<__nv_bfloat16, 1, 1>(p, s);
+        else e = two ? by_blocks<__nv_bfloat16, 0, 2>(p, s) : by_blocks<__nv_bfloat16, 0, 1>(p, s);
+    }
     return e == cudaSuccess ? 0 : l3m_error_cuda(e, me);
 }
 
