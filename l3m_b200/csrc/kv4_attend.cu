@@ -62,6 +62,12 @@ __device__ __forceinline__ void mma(float *c, uint32_t a0, uint32_t a1, uint32_t
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// The same with the accumulators starting at c.
+__device__ __forceinline__ void mma(float *d, const float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
     return *(const uint32_t *)&r;
@@ -115,6 +121,8 @@ template <int N> __device__ __forceinline__ void lds_bytes(uint32_t *w, const ui
 // Halves h of a (low) and of b (high).
 __device__ __forceinline__ uint32_t pair_of(const uint32_t *a, const uint32_t *b, int h) { return prmt(a[h / 2], b[h / 2], h % 2 ? 0x7632 : 0x5410); }
 
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }   // 2^e, -126 <= e <= 127
+
 __device__ __forceinline__ float load_f32(const float *p) { return *p; }
 __device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfloat162float(*p); }
 __device__ __forceinline__ void store_f32(float *p, float x) { *p = x; }
@@ -126,7 +134,7 @@ constexpr int kMaxSms = 160;
 constexpr float kFloor = -1e30f;         // the reference of a row that has seen nothing
 
 // Resident CTAs per SM that the registers of a variant allow.
-constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 2 ? 4 : ng * nt <= 4 ? 3 : 2; }
+constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 4 ? 4 : ng * nt <= 5 ? 3 : 2; }
 
 struct Segment { int r, h, rt; };
 
@@ -157,12 +165,12 @@ struct Worker {
     uint8_t *smem;
     int warp, lane, g, t;
     uint32_t q[QP][NT][NG][4];            // B fragments of the rows: [high, low part][row][block][2 steps x 2]
-    float c0[SUBN ? NT : 1][SUBN ? NG : 1][2];
+    float c0[SUBN ? NT : 1][SUBN ? NG : 1][4];
     float mult[NT][2];
     int pos[NT][2];
     float ref[NT][2], sum[NT][2];
     float o[NT][NG][2][4];
-    float w[SUBN ? NT : 1][SUBN ? NG : 1][4];
+    float w[SUBN ? NT : 1][SUBN ? (NG + 1) / 2 : 1][4];                       // two blocks' sums of P times scale: rows 0-7 block 2i, rows 8-15 block 2i + 1
     int vexp, eref;
 
     __device__ Worker(const AttendArgs &args, uint8_t *sm) : p(args), smem(sm) {
@@ -193,19 +201,32 @@ struct Worker {
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int up = top > 0.0f ? 9 - max(min(ilogbf(top), 127), -149) : 0;      // |x| * 2^up < 2^10
+            const float up0 = exp2i(up / 2), up1 = exp2i(up - up / 2);
             m8[n] = ldexpf(p.a.scale * log2e, (SUBN ? 24 : 0) - up);
 #pragma unroll
             for (int j = 0; j < NG; j++) {
                 float s = 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    // q4_0: nibbles k and k + 4 make a pair; mxfp4: the two of a byte
-                    const float a = ldexpf(x[j][MX ? 2 * k : k], up), b = ldexpf(x[j][MX ? 2 * k + 1 : k + 4], up);
-                    const float down = SUBN && (k & 1) ? 0.0625f : 1.0f;
-                    q[0][n][j][k] = pack_f16(a * down, b * down);
-                    const float2 back = unpack_f16(q[0][n][j][k]);
-                    if (PREC) q[QP - 1][n][j][k] = pack_f16(a - back.x, b - back.y);
-                    s += SUBN && (k & 1) ? (back.x + back.y) * 16.0f : back.x + back.y;
+                for (int e = 0; e < 8; e++) x[j][e] = x[j][e] * up0 * up1;
+                if (SUBN) {
+                    // The fragments hold nibbles 2k and 2k + 4 ... as r = n0 and y = n0 + 16 n1, so q0 n0 + q1 n1 = (q0 - q1 / 16) r + q1 / 16 y.
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        q[0][n][j][2 * k + 1] = pack_f16(x[j][2 * k + 1] * 0.0625f, x[j][2 * k + 5] * 0.0625f);
+                        const float2 y = unpack_f16(q[0][n][j][2 * k + 1]);
+                        q[0][n][j][2 * k] = pack_f16(x[j][2 * k] - y.x, x[j][2 * k + 4] - y.y);
+                        const float2 r = unpack_f16(q[0][n][j][2 * k]);
+                        s += r.x + r.y + 17.0f * (y.x + y.y);
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        // q4_0: nibbles k and k + 4 make a pair; mxfp4: the two of a byte
+                        const float a = x[j][MX ? 2 * k : k], b = x[j][MX ? 2 * k + 1 : k + 4];
+                        q[0][n][j][k] = pack_f16(a, b);
+                        const float2 back = unpack_f16(q[0][n][j][k]);
+                        if (PREC) q[QP - 1][n][j][k] = pack_f16(a - back.x, b - back.y);
+                    }
                 }
                 cs[n][j] = s;
             }
@@ -216,8 +237,8 @@ struct Worker {
             for (int j = 0; j < NG && SUBN; j++) {
                 cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 1);
                 cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 2);
-                c0[n][j][0] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t) * -0x1p-21f;
-                c0[n][j][1] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t + 4) * -0x1p-21f;
+                c0[n][j][0] = c0[n][j][2] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t) * -0x1p-21f;
+                c0[n][j][1] = c0[n][j][3] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t + 4) * -0x1p-21f;
             }
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -232,7 +253,7 @@ struct Worker {
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     o[n][j][0][e] = o[n][j][1][e] = 0.0f;
-                    if (SUBN) w[n][j][e] = 0.0f;
+                    if (SUBN) w[n][j / 2][e] = 0.0f;
                 }
         }
         vexp = PREC && !MX ? -16 : 0;                                              // P itself is held in f16 for bf16 results: 2^14 at most
@@ -248,7 +269,7 @@ struct Worker {
                 o[n][j][m][2] *= f0; o[n][j][m][3] *= f1;
             }
             if (SUBN) {
-                w[n][j][0] *= f0; w[n][j][1] *= f1;
+                w[n][j / 2][j % 2 * 2] *= f0; w[n][j / 2][j % 2 * 2 + 1] *= f1;
             }
         }
     }
@@ -288,17 +309,17 @@ struct Worker {
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float acc[4];
-                if (SUBN) {
-                    acc[0] = acc[2] = c0[SUBN ? n : 0][SUBN ? j : 0][0];
-                    acc[1] = acc[3] = c0[SUBN ? n : 0][SUBN ? j : 0][1];
-                } else {
-                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-                }
                 if (PREC) {
+                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
                     mma(acc, fa[0], fb[0], fa[1], fb[1], q[QP - 1][n][j][0], q[QP - 1][n][j][1]);
                     mma(acc, fa[2], fb[2], fa[3], fb[3], q[QP - 1][n][j][2], q[QP - 1][n][j][3]);
+                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                } else if (SUBN) {
+                    mma(acc, c0[SUBN ? n : 0][SUBN ? j : 0], fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                } else {
+                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
                 }
-                mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
                 mma(acc, fa[2], fb[2], fa[3], fb[3], q[0][n][j][2], q[0][n][j][3]);
                 s[n][0] = fmaf(acc[0], da, s[n][0]);
                 s[n][1] = fmaf(acc[1], da, s[n][1]);
@@ -306,16 +327,15 @@ struct Worker {
                 s[n][3] = fmaf(acc[3], db, s[n][3]);
             }
         }
+        if (EDGE) {
 #pragma unroll
-        for (int n = 0; n < NT; n++)
+            for (int n = 0; n < NT; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                s[n][e] *= mult[n][e & 1];
-                if (EDGE) {
+                for (int e = 0; e < 4; e++) {
                     const int tok = tok0 + ra + (e & 2 ? 8 : 0), at = pos[n][e & 1];
                     if (tok > at || (p.a.window && tok <= at - p.a.window)) s[n][e] = -INFINITY;
                 }
-            }
+        }
         // ---- the values' scales: of this lane's tokens as P's transposed pairs want them, or (float results) as the scores lie
         uint32_t v0[SW], v1[SW], v2[SW], v3[SW];
         const int t0 = PREC ? ra : t, t1 = 4 + (t ^ 1);
@@ -362,12 +382,15 @@ struct Worker {
                 move = (any & 0x40004000u) && vexp < 16;
             }
         }
-        float lim = 14.0f - (float)vexp;
+        float lim = 14.0f - (float)vexp, z[NT][4], high = kFloor;                                       // the exponents of P
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-            move |= fmaxf(s[n][0], s[n][2]) > ref[n][0] + lim;
-            move |= fmaxf(s[n][1], s[n][3]) > ref[n][1] + lim;
-        }
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                z[n][e] = EDGE && s[n][e] == -INFINITY ? -INFINITY : fmaf(s[n][e], mult[n][e & 1], -ref[n][e & 1]);
+                high = fmaxf(high, z[n][e]);
+            }
+        move |= high > lim;
         if (__any_sync(0xffffffffu, move)) {
             int top = 0;
 #pragma unroll
@@ -392,23 +415,25 @@ struct Worker {
                 }
             } else {
                 vexp = max(vexp, top - 15);
-                lim = 14.0f - (float)vexp;
+                lim = 14.0f - (float)vexp;                                   // raising vexp lowers it
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float f[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    float m = fmaxf(s[n][c], s[n][c + 2]);
+                    float m = fmaxf(EDGE && s[n][c] == -INFINITY ? -INFINITY : s[n][c] * mult[n][c], EDGE && s[n][c + 2] == -INFINITY ? -INFINITY : s[n][c + 2] * mult[n][c]);
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     f[c] = 1.0f;
-                    if (m > ref[n][c] + lim) {
+                    if (m - ref[n][c] > lim) {
                         const float to = m - lim + 4.0f;                     // room for 2^4 before the next move
                         f[c] = ex2(ref[n][c] - to);
                         ref[n][c] = to;
                     }
+                    z[n][c] = EDGE && s[n][c] == -INFINITY ? -INFINITY : fmaf(s[n][c], mult[n][c], -ref[n][c]);
+                    z[n][c + 2] = EDGE && s[n][c + 2] == -INFINITY ? -INFINITY : fmaf(s[n][c + 2], mult[n][c], -ref[n][c]);
                     sum[n][c] *= f[c];
                 }
                 scale_rows(n, f[0] * shrink, f[1] * shrink);
@@ -419,7 +444,7 @@ struct Worker {
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[n][e] = ex2(s[n][e] - ref[n][e & 1]);
+            for (int e = 0; e < 4; e++) s[n][e] = ex2(z[n][e]);
             sum[n][0] += s[n][0] + s[n][2];
             sum[n][1] += s[n][1] + s[n][3];
             if (!PREC) {
@@ -476,7 +501,11 @@ struct Worker {
                     const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
                     mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
                     mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
-                    if (SUBN) mma(w[SUBN ? n : 0][SUBN ? j : 0], 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, 0x3c003c00u, b0, b1);
+                    if (SUBN) {
+                        constexpr uint32_t one = 0x3c003c00u;
+                        const uint32_t up = j % 2 ? 0 : one, down = j % 2 ? one : 0;
+                        mma(w[SUBN ? n : 0][SUBN ? j / 2 : 0], up, down, up, down, b0, b1);
+                    }
                 }
             }
         }
@@ -487,10 +516,15 @@ struct Worker {
 #pragma unroll
             for (int k = 0; k < 4; k++) f[k] = e2m1_pair(x >> (8 * k));
         } else {
-            const uint32_t y = x >> 8;
-            f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
-            f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
-            if (PREC) whole(f);
+            if (SUBN) {                                                      // r and y of the low bytes, then of the high ones
+                f[1] = prmt(x, 0, 0x4240); f[0] = f[1] & 0x000f000fu;
+                f[3] = prmt(x, 0, 0x4341); f[2] = f[3] & 0x000f000fu;
+            } else {
+                const uint32_t y = x >> 8;
+                f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
+                f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
+                whole(f);
+            }
         }
     }
     // Block j's 4 codes of two tokens as four pairs of the same dim.
@@ -503,10 +537,16 @@ struct Worker {
                 f[2 * k + 1] = prmt(x, y, 0x7632);
             }
         } else {
-            const uint32_t x = pair_of(a, b, j), y = x >> 8;
-            f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
-            f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
-            if (PREC) whole(f);
+            if (SUBN) {                                                      // y = n0 + 16 n1 and 16 n1 of the low bytes, then of the high ones
+                const uint32_t lo = j % 2 ? 0x0602 : 0x0400, x = a[j / 2], y = b[j / 2];
+                f[0] = prmt(x, y, lo) & 0x00ff00ffu; f[1] = f[0] & 0x00f000f0u;
+                f[2] = prmt(x, y, lo + 0x0101) & 0x00ff00ffu; f[3] = f[2] & 0x00f000f0u;
+            } else {
+                const uint32_t x = pair_of(a, b, j), y = x >> 8;
+                f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
+                f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
+                whole(f);
+            }
         }
     }
     // n -> n - 8 in f16: 1024 + n (or 1024 + 16 n) is a number whose last bits are n.
@@ -604,9 +644,9 @@ struct Worker {
                 for (int j = 0; j < NG; j++) {
                     float v[4] = {o[n][j][0][c], o[n][j][0][2 + c], o[n][j][1][c], o[n][j][1][2 + c]};
                     if (SUBN) {
-                        const float off = w[SUBN ? n : 0][SUBN ? j : 0][c] * 8.0f;
-                        v[0] = fmaf(v[0], 0x1p24f, -off); v[1] = fmaf(v[1], 0x1p20f, -off);
-                        v[2] = fmaf(v[2], 0x1p24f, -off); v[3] = fmaf(v[3], 0x1p20f, -off);
+                        const float off = w[SUBN ? n : 0][SUBN ? j / 2 : 0][j % 2 * 2 + c] * 8.0f;
+                        v[0] = fmaf(v[0] - v[1], 0x1p24f, -off); v[1] = fmaf(v[1], 0x1p20f, -off);
+                        v[2] = fmaf(v[2] - v[3], 0x1p24f, -off); v[3] = fmaf(v[3], 0x1p20f, -off);
                     }
                     if (MX) v[0] *= unit, v[1] *= unit, v[2] *= unit, v[3] *= unit;
                     *(float4 *)(row + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
@@ -770,39 +810,67 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
         u0 += p.split ? len : gridDim.x;
     }
     if (p.split && threadIdx.x == 0) p.desc[blockIdx.x] = desc;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the join may take this CTA's place
 }
 
-// The pieces of the segments that several workers shared: CTA (w, row) joins a row of the segment that ends in worker w.
+// The pieces of the segments that several workers shared, joined: CTA (w, y) does `rows` rows of the segment that ends
+// in worker w. Its threads are [part][row][4 dims]: with few rows they take the pieces apart as well.
+constexpr int kJoinThreads = 512;
+
 template <typename T, int MX, int NG, int NT>
-__global__ void __launch_bounds__(kThreads) join_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs p, int rows) {
     typedef Worker<T, MX, NG, NT> W;
-    constexpr int LD = W::DP + 4, SIZE = W::NR * LD;
+    constexpr int LD = W::DP + 4, SIZE = W::NR * LD, PER = W::DP / 4;
+    __shared__ float4 sv[kJoinThreads];
+    __shared__ float2 sml[kJoinThreads];
+    asm volatile("griddepcontrol.wait;" ::: "memory");                      // the workers are done and their pieces visible
     const int4 d = p.desc[blockIdx.x];
     if (d.x < 0) return;
-    const int row = blockIdx.y, own = blockIdx.x;
-    auto piece = [&](int k) { return p.part + ((size_t)k * 2 + (k == d.x ? 1 : 0)) * SIZE + row * LD; };
-    __shared__ float red[kWarps];
-    float m = kFloor;
-    for (int k = d.x + threadIdx.x; k <= own; k += kThreads) m = fmaxf(m, piece(k)[W::DP]);
-    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-    __syncthreads();
-    for (int k = 0; k < kWarps; k++) m = fmaxf(m, red[k]);
-    for (int at = threadIdx.x * 4; at < W::DP; at += kThreads * 4) {
-        float l = 0.0f;
+    const int items = rows * PER, parts = max(1, kJoinThreads / items), n = blockIdx.x - d.x + 1;
+    for (int base = 0; base < items; base += kJoinThreads) {                 // one turn where parts > 1
+        const int it = parts > 1 ? threadIdx.x % items : base + threadIdx.x, part = parts > 1 ? threadIdx.x / items : 0;
+        const int row = blockIdx.y * rows + it / PER, at = it % PER * 4;
+        const bool on = it < items && part < parts;
+        auto piece = [&](int k) { return p.part + ((size_t)(d.x + k) * 2 + (k == 0 ? 1 : 0)) * SIZE + (size_t)row * LD; };
+        float m = kFloor, l = 0.0f;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (on) {
 #pragma unroll 8
-        for (int k = d.x; k <= own; k++) {
-            const float *from = piece(k);
-            const float2 ml = *(const float2 *)(from + W::DP);
-            const float4 x = *(const float4 *)(from + at);
-            const float f = ex2(ml.x - m);
-            l = fmaf(ml.y, f, l);
-            v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            for (int k = part; k < n; k += parts) m = fmaxf(m, piece(k)[W::DP]);
+#pragma unroll 4
+            for (int k = part; k < n; k += parts) {
+                const float *from = piece(k);
+                const float2 ml = *(const float2 *)(from + W::DP);
+                const float4 x = *(const float4 *)(from + at);
+                const float f = ex2(ml.x - m);
+                l = fmaf(ml.y, f, l);
+                v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            }
         }
-        const Request q = request_of(p, d.y, W::NR);
-        W w(p, nullptr);
-        w.put(q.start, q.nq, d.z, d.w, row, at, v, l);
+        if (parts > 1) {
+            sv[threadIdx.x] = v;
+            sml[threadIdx.x] = make_float2(m, l);
+            __syncthreads();
+            if (on && part == 0) {
+                float top = m;
+                for (int k = 1; k < parts; k++) top = fmaxf(top, sml[k * items + it].x);
+                float f = ex2(m - top);
+                l *= f;
+                v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+                for (int k = 1; k < parts; k++) {
+                    const float2 ml = sml[k * items + it];
+                    const float4 x = sv[k * items + it];
+                    f = ex2(ml.x - top);
+                    l = fmaf(ml.y, f, l);
+                    v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+                }
+            }
+        }
+        if (on && part == 0) {
+            const Request q = request_of(p, d.y, W::NR);
+            W w(p, nullptr);
+            w.put(q.start, q.nq, d.z, d.w, row, at, v, l);
+        }
     }
 }
 
@@ -835,8 +903,20 @@ cudaError_t launch(AttendArgs p, cudaStream_t s) {
     const long long segs = (long long)p.a.n_req * p.c.n_kv * p.row_tiles;
     const int grid = p.split ? workers : (int)std::min<long long>(segs, 1 << 20);
     attend_kernel<T, MX, NG, NT><<<grid, kThreads, W::SMEM, s>>>(p);
-    if (p.split) join_kernel<T, MX, NG, NT><<<dim3(workers, W::NR), kThreads, 0, s>>>(p);
-    return cudaGetLastError();
+    e = cudaGetLastError();
+    if (e != cudaSuccess || !p.split) return e;
+    // Its CTAs may start while the last workers run (each waits for them); a row per CTA where a segment has many pieces.
+    const int rows = workers > 8 * segs ? 1 : W::NR;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(workers, W::NR / rows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, join_kernel<T, MX, NG, NT>, p, rows);
 }
 
 template <typename T, int MX, int NT>
