@@ -26,7 +26,7 @@ struct AttendArgs {
     int group, row_tiles;                 // query heads per kv head; row tiles of a request with max_q queries
     int split;                            // 1: workers share all tiles out evenly, 0: a worker takes whole segments
     float *part;                          // [workers][2] partial results of [rows][Dp + 2] floats: values, then reference and sum
-    int4 *desc;                           // [workers]: the segment whose last piece the worker did and where it began
+    int4 *desc;                           // [workers][2]: the segment whose last piece the worker did: where it began, head, row tile; its request's first row and rows
 };
 
 // ---- warp pieces
@@ -61,12 +61,6 @@ __device__ __forceinline__ void mma(float *c, uint32_t a0, uint32_t a1, uint32_t
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The same with the accumulators starting at c.
-__device__ __forceinline__ void mma(float *d, const float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
-        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
 }
 __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
@@ -129,7 +123,7 @@ __device__ __forceinline__ void store_f32(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
 constexpr int kWarps = 4, kThreads = 32 * kWarps;
-constexpr int kStages = 4;               // tiles of a warp's ring
+constexpr int kStages = 4;               // tiles of a warp's ring: two pairs
 constexpr int kMaxSms = 160;
 constexpr float kFloor = -1e30f;         // the reference of a row that has seen nothing
 
@@ -159,13 +153,14 @@ struct Worker {
     static constexpr int RING = kStages * TB;
     static constexpr int SMEM = kWarps * RING > kWarps * NR * (DP + 4) * 4 ? kWarps * RING : kWarps * NR * (DP + 4) * 4;
     static constexpr int QP = PREC ? 2 : 1;
+    static constexpr int NG2 = NG + NG % 2;                                  // blocks, in pairs
     static constexpr int SW = MX ? (NG + 3) / 4 : (NG + 1) / 2;              // words of a row's scales
 
     const AttendArgs &p;
     uint8_t *smem;
     int warp, lane, g, t;
     uint32_t q[QP][NT][NG][4];            // B fragments of the rows: [high, low part][row][block][2 steps x 2]
-    float c0[SUBN ? NT : 1][SUBN ? NG : 1][4];
+    uint32_t c0[SUBN ? NT : 1][2];        // the offset's part of the scores as a B fragment: -sum(q) / 2^8 of block k, and its rest, against the keys' scales
     float mult[NT][2];
     int pos[NT][2];
     float ref[NT][2], sum[NT][2];
@@ -233,12 +228,25 @@ struct Worker {
         }
 #pragma unroll
         for (int n = 0; n < NT; n++) {
+            if (SUBN) {
 #pragma unroll
-            for (int j = 0; j < NG && SUBN; j++) {
-                cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 1);
-                cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 2);
-                c0[n][j][0] = c0[n][j][2] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t) * -0x1p-21f;
-                c0[n][j][1] = c0[n][j][3] = __shfl_sync(0xffffffffu, cs[n][j], 8 * t + 4) * -0x1p-21f;
+                for (int j = 0; j < NG; j++) {
+                    cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 1);
+                    cs[n][j] += __shfl_xor_sync(0xffffffffu, cs[n][j], 2);
+                }
+                // k = 0 .. NG2 - 1: the blocks' high parts, k = NG2 .. 2 NG2 - 1: what f16 leaves of them
+                float k4[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int k = 2 * t + (i & 1) + (i & 2 ? 8 : 0);
+                    float hi = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < NG; j++) hi = k % NG2 == j && k < 2 * NG2 ? cs[n][j] * -0x1p-8f : hi;
+                    const float rest = hi - __half2float(__float2half_rn(hi));
+                    k4[i] = k < NG2 ? hi : rest;
+                }
+                c0[SUBN ? n : 0][0] = pack_f16(k4[0], k4[1]);
+                c0[SUBN ? n : 0][1] = pack_f16(k4[2], k4[3]);
             }
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -274,137 +282,164 @@ struct Worker {
         }
     }
 
-    // One tile in shared memory. edge: some row does not see some of its tokens, which begin at tok0; [lo_any, hi_any) is seen by some row.
-    template <bool EDGE> __device__ __forceinline__ void tile(const uint8_t *sm, int tok0, int lo_any, int hi_any) {
+    // U tiles in shared memory, neighbours in the context. EDGE: some row does not see some of their tokens, which begin at tok0;
+    // [lo_any, hi_any) is seen by some row.
+    template <bool EDGE, int U> __device__ __forceinline__ void step(const uint8_t *sm, int tok0, int lo_any, int hi_any) {
+        const int ra = tau(g), t0 = PREC ? ra : t, t1 = 4 + (t ^ 1);
+        constexpr int KS = 512 * NG, VS = KS + 16 * NG * SB;
         // ---- scores
-        const int ra = tau(g);
-        uint32_t ka[NG], kb[NG], sa[SW], sb[SW];
-        lds_words<NG>(ka, sm + ra * 16 * NG + t * 4 * NG);
-        lds_words<NG>(kb, sm + (ra + 8) * 16 * NG + t * 4 * NG);
-        const uint8_t *ks = sm + 512 * NG, *vs = ks + 16 * NG * SB;
-        if (MX) {
-            lds_bytes<NG>(sa, ks + ra * NG);
-            lds_bytes<NG>(sb, ks + (ra + 8) * NG);
-        } else {
-            lds_halves<NG>(sa, ks + ra * NG * 2);
-            lds_halves<NG>(sb, ks + (ra + 8) * NG * 2);
-        }
-        float s[NT][4];
+        float s[U][NT][4];
 #pragma unroll
-        for (int n = 0; n < NT; n++) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            uint32_t fa[4], fb[4];
-            codes4(fa, ka[j]);
-            codes4(fb, kb[j]);
-            float da, db;
+        for (int u = 0; u < U; u++) {
+            const uint8_t *tl = sm + u * TB;
+            uint32_t ka[NG], kb[NG], sa[SW], sb[SW];
+            lds_words<NG>(ka, tl + ra * 16 * NG + t * 4 * NG);
+            lds_words<NG>(kb, tl + (ra + 8) * 16 * NG + t * 4 * NG);
             if (MX) {
-                da = __uint_as_float((sa[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
-                db = __uint_as_float((sb[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
+                lds_bytes<NG>(sa, tl + KS + ra * NG);
+                lds_bytes<NG>(sb, tl + KS + (ra + 8) * NG);
             } else {
-                const float2 a2 = unpack_f16(sa[j / 2]), b2 = unpack_f16(sb[j / 2]);
-                da = j % 2 ? a2.y : a2.x;
-                db = j % 2 ? b2.y : b2.x;
+                lds_halves<NG>(sa, tl + KS + ra * NG * 2);
+                lds_halves<NG>(sb, tl + KS + (ra + 8) * NG * 2);
             }
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                float acc[4];
-                if (PREC) {
-                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[QP - 1][n][j][0], q[QP - 1][n][j][1]);
-                    mma(acc, fa[2], fb[2], fa[3], fb[3], q[QP - 1][n][j][2], q[QP - 1][n][j][3]);
-                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
-                } else if (SUBN) {
-                    mma(acc, c0[SUBN ? n : 0][SUBN ? j : 0], fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
-                } else {
-                    acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
-                    mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                s[u][n][0] = s[u][n][1] = s[u][n][2] = s[u][n][3] = 0.0f;
+                if (SUBN) {
+                    // A: the scales of rows g and g + 8, columns 2t, 2t + 1 (+ 8): blocks 2t % NG2 and the next
+                    uint32_t f[4] = {0, 0, 0, 0};
+                    if constexpr (NG % 2 == 0) {
+                        const uint8_t *row = tl + KS + ra * NG * 2;
+                        if (t < NG) f[0] = *(const uint32_t *)(row + t % (NG / 2) * 4), f[1] = *(const uint32_t *)(row + 16 * NG + t % (NG / 2) * 4);
+                        if (NG > 4 && t + 4 < NG) f[2] = *(const uint32_t *)(row + (t + 4) % (NG / 2) * 4), f[3] = *(const uint32_t *)(row + 16 * NG + (t + 4) % (NG / 2) * 4);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < SW; i++) {
+                            const bool lo = t < NG2 && t % (NG2 / 2) == i, hi = t + 4 < NG2 && (t + 4) % (NG2 / 2) == i;
+                            f[0] = lo ? sa[i] : f[0]; f[1] = lo ? sb[i] : f[1];
+                            f[2] = hi ? sa[i] : f[2]; f[3] = hi ? sb[i] : f[3];
+                        }
+                    }
+                    mma(s[u][n], f[0], f[1], f[2], f[3], c0[SUBN ? n : 0][0], c0[SUBN ? n : 0][1]);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) s[u][n][e] *= 0x1p-13f;       // 8 * 2^-24 * 2^8
                 }
-                mma(acc, fa[2], fb[2], fa[3], fb[3], q[0][n][j][2], q[0][n][j][3]);
-                s[n][0] = fmaf(acc[0], da, s[n][0]);
-                s[n][1] = fmaf(acc[1], da, s[n][1]);
-                s[n][2] = fmaf(acc[2], db, s[n][2]);
-                s[n][3] = fmaf(acc[3], db, s[n][3]);
+            }
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                uint32_t fa[4], fb[4];
+                codes4(fa, ka[j]);
+                codes4(fb, kb[j]);
+                float da, db;
+                if (MX) {
+                    da = __uint_as_float((sa[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
+                    db = __uint_as_float((sb[j / 4] >> (8 * (j % 4)) & 0xff) << 23);
+                } else {
+                    const float2 a2 = unpack_f16(sa[j / 2]), b2 = unpack_f16(sb[j / 2]);
+                    da = j % 2 ? a2.y : a2.x;
+                    db = j % 2 ? b2.y : b2.x;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    float acc[4];
+                    if (PREC) {
+                        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                        mma(acc, fa[0], fb[0], fa[1], fb[1], q[QP - 1][n][j][0], q[QP - 1][n][j][1]);
+                        mma(acc, fa[2], fb[2], fa[3], fb[3], q[QP - 1][n][j][2], q[QP - 1][n][j][3]);
+                        mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                    } else {
+                        acc[0] = acc[1] = acc[2] = acc[3] = 0.0f;
+                        mma(acc, fa[0], fb[0], fa[1], fb[1], q[0][n][j][0], q[0][n][j][1]);
+                    }
+                    mma(acc, fa[2], fb[2], fa[3], fb[3], q[0][n][j][2], q[0][n][j][3]);
+                    s[u][n][0] = fmaf(acc[0], da, s[u][n][0]);
+                    s[u][n][1] = fmaf(acc[1], da, s[u][n][1]);
+                    s[u][n][2] = fmaf(acc[2], db, s[u][n][2]);
+                    s[u][n][3] = fmaf(acc[3], db, s[u][n][3]);
+                }
+            }
+            if (EDGE) {
+#pragma unroll
+                for (int n = 0; n < NT; n++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int tok = tok0 + u * kKvTile + ra + (e & 2 ? 8 : 0), at = pos[n][e & 1];
+                        if (tok > at || (p.a.window && tok <= at - p.a.window)) s[u][n][e] = -INFINITY;
+                    }
             }
         }
-        if (EDGE) {
+        // ---- the values' scales: of this lane's tokens as P's transposed pairs want them, or (float results) as the scores lie
+        uint32_t v[U][4][SW];
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (PREC && k % 2) {
+#pragma unroll
+                    for (int i = 0; i < SW; i++) v[u][k][i] = 0;
+                    continue;
+                }
+                const int row = (k % 2 ? t1 : t0) + (k / 2) * 8;
+                if (MX) lds_bytes<NG>(v[u][k], sm + u * TB + VS + row * NG);
+                else lds_halves<NG>(v[u][k], sm + u * TB + VS + row * NG * 2);
+                if (EDGE) {
+                    const int tok = tok0 + u * kKvTile + row;
+                    const bool gone = tok < lo_any || tok >= hi_any;
+#pragma unroll
+                    for (int i = 0; i < SW; i++) {
+                        uint32_t &x = v[u][k][i];
+                        if (!MX) {                                           // infinities and NaN that some row does not see must not meet its zeros
+                            if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u;
+                            if ((x & 0x7c000000u) == 0x7c000000u) x &= 0x0000ffffu;
+                        }
+                        if (gone) x = 0;
+                    }
+                }
+            }
+        // ---- does the reference still hold? P <= 2^lim, |scale| < 2^(vexp + 1) (mxfp4: scales are taken relative to eref, vexp stays)
+        bool move;
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int k = 0; k < 4; k += PREC ? 2 : 1)
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    if (MX) any = __vmaxu4(any, v[u][k][i]);
+                    else if (PREC) any = __vmaxu2(any, v[u][k][i] & 0x7fff7fffu);
+                    else any |= v[u][k][i];
+                }
+        if (MX) {
+            any = __vmaxu4(any, any >> 16);
+            move = (int)max(any & 0xff, any >> 8 & 0xff) > eref;
+        } else if (PREC) {
+            move = (int)max(any >> 10 & 31, any >> 26) - 15 > vexp;
+        } else {
+            move = (any & 0x40004000u) && vexp < 16;
+        }
+        float lim = 14.0f - (float)vexp, z[U][NT][4], high = kFloor;         // the exponents of P
+#pragma unroll
+        for (int u = 0; u < U; u++)
 #pragma unroll
             for (int n = 0; n < NT; n++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int tok = tok0 + ra + (e & 2 ? 8 : 0), at = pos[n][e & 1];
-                    if (tok > at || (p.a.window && tok <= at - p.a.window)) s[n][e] = -INFINITY;
+                    z[u][n][e] = EDGE && s[u][n][e] == -INFINITY ? -INFINITY : fmaf(s[u][n][e], mult[n][e & 1], -ref[n][e & 1]);
+                    high = fmaxf(high, z[u][n][e]);
                 }
-        }
-        // ---- the values' scales: of this lane's tokens as P's transposed pairs want them, or (float results) as the scores lie
-        uint32_t v0[SW], v1[SW], v2[SW], v3[SW];
-        const int t0 = PREC ? ra : t, t1 = 4 + (t ^ 1);
-        auto scales = [&](uint32_t *x, int row) {
-            if (MX) lds_bytes<NG>(x, vs + row * NG);
-            else lds_halves<NG>(x, vs + row * NG * 2);
-            if (EDGE) {
-                const int tok = tok0 + row;
-                const bool gone = tok < lo_any || tok >= hi_any;
-#pragma unroll
-                for (int i = 0; i < SW; i++) {
-                    if (!MX) {                                               // infinities and NaN that some row does not see must not meet its zeros
-                        if ((x[i] & 0x7c00u) == 0x7c00u) x[i] &= 0xffff0000u;
-                        if ((x[i] & 0x7c000000u) == 0x7c000000u) x[i] &= 0x0000ffffu;
-                    }
-                    if (gone) x[i] = 0;
-                }
-            }
-        };
-        scales(v0, t0);
-        if (!PREC) scales(v1, t1);
-        scales(v2, t0 + 8);
-        if (!PREC) scales(v3, t1 + 8);
-        // ---- does the reference still hold? P <= 2^lim, |scale| < 2^(vexp + 1) (mxfp4: scales are taken relative to eref, vexp stays)
-        bool move = false;
-        if (MX) {
-            uint32_t top = 0;
-#pragma unroll
-            for (int i = 0; i < SW; i++) {
-                top = __vmaxu4(top, __vmaxu4(v0[i], v2[i]));
-                if (!PREC) top = __vmaxu4(top, __vmaxu4(v1[i], v3[i]));
-            }
-            const uint32_t two = __vmaxu4(top, top >> 16);
-            move = (int)max(two & 0xff, two >> 8 & 0xff) > eref;
-        } else {
-            uint32_t any = 0;
-            if (PREC) {
-#pragma unroll
-                for (int i = 0; i < SW; i++) any = __vmaxu2(any, __vmaxu2(v0[i] & 0x7fff7fffu, v2[i] & 0x7fff7fffu));
-                move = (int)max(any >> 10 & 31, any >> 26) - 15 > vexp;
-            } else {
-#pragma unroll
-                for (int i = 0; i < SW; i++) any |= v0[i] | v1[i] | v2[i] | v3[i];
-                move = (any & 0x40004000u) && vexp < 16;
-            }
-        }
-        float lim = 14.0f - (float)vexp, z[NT][4], high = kFloor;                                       // the exponents of P
-#pragma unroll
-        for (int n = 0; n < NT; n++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                z[n][e] = EDGE && s[n][e] == -INFINITY ? -INFINITY : fmaf(s[n][e], mult[n][e & 1], -ref[n][e & 1]);
-                high = fmaxf(high, z[n][e]);
-            }
         move |= high > lim;
         if (__any_sync(0xffffffffu, move)) {
             int top = 0;
 #pragma unroll
-            for (int i = 0; i < SW; i++) {
-                const uint32_t all[4] = {v0[i], v2[i], PREC ? 0u : v1[i], PREC ? 0u : v3[i]};
+            for (int u = 0; u < U; u++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    if (MX) {
-                        top = max(max(top, (int)(all[k] & 0xff)), max((int)(all[k] >> 8 & 0xff), max((int)(all[k] >> 16 & 0xff), (int)(all[k] >> 24))));
-                    } else {
-                        top = max(top, max((int)(all[k] >> 10 & 31), (int)(all[k] >> 26 & 31)));
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int i = 0; i < SW; i++) {
+                        const uint32_t x = v[u][k][i];
+                        if (MX) top = max(max(top, (int)(x & 0xff)), max((int)(x >> 8 & 0xff), max((int)(x >> 16 & 0xff), (int)(x >> 24))));
+                        else top = max(top, max((int)(x >> 10 & 31), (int)(x >> 26 & 31)));
                     }
-                }
-            }
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             float shrink = 1.0f;
@@ -422,89 +457,98 @@ struct Worker {
                 float f[2];
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
-                    float m = fmaxf(EDGE && s[n][c] == -INFINITY ? -INFINITY : s[n][c] * mult[n][c], EDGE && s[n][c + 2] == -INFINITY ? -INFINITY : s[n][c + 2] * mult[n][c]);
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int e = c; e < 4; e += 2)
+                            if (!(EDGE && s[u][n][e] == -INFINITY)) m = fmaxf(m, s[u][n][e] * mult[n][c]);
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
                     f[c] = 1.0f;
                     if (m - ref[n][c] > lim) {
-                        const float to = m - lim + 4.0f;                     // room for 2^4 before the next move
+                        const float to = m - lim + 2.0f;                     // room for 2^2 before the next move: more costs P bits where scales are small
                         f[c] = ex2(ref[n][c] - to);
                         ref[n][c] = to;
                     }
-                    z[n][c] = EDGE && s[n][c] == -INFINITY ? -INFINITY : fmaf(s[n][c], mult[n][c], -ref[n][c]);
-                    z[n][c + 2] = EDGE && s[n][c + 2] == -INFINITY ? -INFINITY : fmaf(s[n][c + 2], mult[n][c], -ref[n][c]);
+#pragma unroll
+                    for (int u = 0; u < U; u++)
+#pragma unroll
+                        for (int e = c; e < 4; e += 2) z[u][n][e] = EDGE && s[u][n][e] == -INFINITY ? -INFINITY : fmaf(s[u][n][e], mult[n][c], -ref[n][c]);
                     sum[n][c] *= f[c];
                 }
                 scale_rows(n, f[0] * shrink, f[1] * shrink);
             }
         }
-        // ---- probabilities
-        uint32_t pb[NT][2];
+        // ---- probabilities and values
 #pragma unroll
-        for (int n = 0; n < NT; n++) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[n][e] = ex2(z[n][e]);
-            sum[n][0] += s[n][0] + s[n][2];
-            sum[n][1] += s[n][1] + s[n][3];
-            if (!PREC) {
-                pb[n][0] = transpose8(pack_f16(s[n][0], s[n][1]));
-                pb[n][1] = transpose8(pack_f16(s[n][2], s[n][3]));
-            }
-        }
-        // ---- values
-        uint32_t c[4][(NG + 1) / 2];
-        const uint8_t *vc = sm + 256 * NG + g * 2 * NG;
-        lds_halves<NG>(c[0], vc + t * 16 * NG);
-        lds_halves<NG>(c[1], vc + t1 * 16 * NG);
-        lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
-        lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
-#pragma unroll
-        for (int j = 0; j < NG; j++) {
-            uint32_t fa[4], fb[4];
-            value4(fa, c[0], c[1], j);
-            value4(fb, c[2], c[3], j);
+        for (int u = 0; u < U; u++) {
+            uint32_t pb[NT][2];
 #pragma unroll
             for (int n = 0; n < NT; n++) {
-                if (PREC) {
-                    float d0, d1;
-                    if (MX) {
-                        d0 = rel_f32(v0[j / 4] >> (8 * (j % 4)) & 0xff);
-                        d1 = rel_f32(v2[j / 4] >> (8 * (j % 4)) & 0xff);
-                    } else {
-                        const float2 a2 = unpack_f16(v0[j / 2]), b2 = unpack_f16(v2[j / 2]);
-                        d0 = j % 2 ? a2.y : a2.x;
-                        d1 = j % 2 ? b2.y : b2.x;
-                    }
-                    const float x0 = s[n][0] * d0, x1 = s[n][1] * d0, x2 = s[n][2] * d1, x3 = s[n][3] * d1;
-                    const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
-                    const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
-                    const uint32_t l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y)), l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
-                    const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
 #pragma unroll
-                    for (int m = 0; m < 2; m++) {                            // a tile's sum by itself: the accumulator of a product is truncated, not rounded
-                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                        mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
-                        mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+                for (int e = 0; e < 4; e++) z[u][n][e] = ex2(z[u][n][e]);
+                sum[n][0] += z[u][n][0] + z[u][n][2];
+                sum[n][1] += z[u][n][1] + z[u][n][3];
+                if (!PREC) {
+                    pb[n][0] = transpose8(pack_f16(z[u][n][0], z[u][n][1]));
+                    pb[n][1] = transpose8(pack_f16(z[u][n][2], z[u][n][3]));
+                }
+            }
+            uint32_t c[4][(NG + 1) / 2];
+            const uint8_t *vc = sm + u * TB + 256 * NG + g * 2 * NG;
+            lds_halves<NG>(c[0], vc + t * 16 * NG);
+            lds_halves<NG>(c[1], vc + t1 * 16 * NG);
+            lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
+            lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) o[n][j][m][e] += acc[e];
-                    }
-                } else {
-                    uint32_t d0, d1;
-                    if (MX) {
-                        d0 = rel_f16(v0[j / 4], v1[j / 4], j % 4);
-                        d1 = rel_f16(v2[j / 4], v3[j / 4], j % 4);
+            for (int j = 0; j < NG; j++) {
+                uint32_t fa[4], fb[4];
+                value4(fa, c[0], c[1], j);
+                value4(fb, c[2], c[3], j);
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    if (PREC) {
+                        float d0, d1;
+                        if (MX) {
+                            d0 = rel_f32(v[u][0][j / 4] >> (8 * (j % 4)) & 0xff);
+                            d1 = rel_f32(v[u][2][j / 4] >> (8 * (j % 4)) & 0xff);
+                        } else {
+                            const float2 a2 = unpack_f16(v[u][0][j / 2]), b2 = unpack_f16(v[u][2][j / 2]);
+                            d0 = j % 2 ? a2.y : a2.x;
+                            d1 = j % 2 ? b2.y : b2.x;
+                        }
+                        const float x0 = z[u][n][0] * d0, x1 = z[u][n][1] * d0, x2 = z[u][n][2] * d1, x3 = z[u][n][3] * d1;
+                        const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
+                        const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
+                        const uint32_t l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y)), l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
+                        const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
+#pragma unroll
+                        for (int m = 0; m < 2; m++) {                        // a tile's sum by itself: the accumulator of a product is truncated, not rounded
+                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
+                            mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+#pragma unroll
+                            for (int e = 0; e < 4; e++) o[n][j][m][e] += acc[e];
+                        }
                     } else {
-                        d0 = pair_of(v0, v1, j);
-                        d1 = pair_of(v2, v3, j);
-                    }
-                    const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
-                    mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
-                    mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
-                    if (SUBN) {
-                        constexpr uint32_t one = 0x3c003c00u;
-                        const uint32_t up = j % 2 ? 0 : one, down = j % 2 ? one : 0;
-                        mma(w[SUBN ? n : 0][SUBN ? j / 2 : 0], up, down, up, down, b0, b1);
+                        uint32_t d0, d1;
+                        if (MX) {
+                            d0 = rel_f16(v[u][0][j / 4], v[u][1][j / 4], j % 4);
+                            d1 = rel_f16(v[u][2][j / 4], v[u][3][j / 4], j % 4);
+                        } else {
+                            d0 = pair_of(v[u][0], v[u][1], j);
+                            d1 = pair_of(v[u][2], v[u][3], j);
+                        }
+                        const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
+                        mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
+                        mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
+                        if (SUBN) {
+                            constexpr uint32_t one = 0x3c003c00u;
+                            const uint32_t up = j % 2 ? 0 : one, down = j % 2 ? one : 0;
+                            mma(w[SUBN ? n : 0][SUBN ? j / 2 : 0], up, down, up, down, b0, b1);
+                        }
                     }
                 }
             }
@@ -517,7 +561,7 @@ struct Worker {
             for (int k = 0; k < 4; k++) f[k] = e2m1_pair(x >> (8 * k));
         } else {
             if (SUBN) {                                                      // r and y of the low bytes, then of the high ones
-                f[1] = prmt(x, 0, 0x4240); f[0] = f[1] & 0x000f000fu;
+                f[1] = x & 0x00ff00ffu; f[0] = x & 0x000f000fu;
                 f[3] = prmt(x, 0, 0x4341); f[2] = f[3] & 0x000f000fu;
             } else {
                 const uint32_t y = x >> 8;
@@ -538,9 +582,9 @@ struct Worker {
             }
         } else {
             if (SUBN) {                                                      // y = n0 + 16 n1 and 16 n1 of the low bytes, then of the high ones
-                const uint32_t lo = j % 2 ? 0x0602 : 0x0400, x = a[j / 2], y = b[j / 2];
-                f[0] = prmt(x, y, lo) & 0x00ff00ffu; f[1] = f[0] & 0x00f000f0u;
-                f[2] = prmt(x, y, lo + 0x0101) & 0x00ff00ffu; f[3] = f[2] & 0x00f000f0u;
+                const uint32_t x = pair_of(a, b, j);
+                f[0] = x & 0x00ff00ffu; f[1] = x & 0x00f000f0u;
+                f[2] = prmt(x, 0, 0x4341); f[3] = f[2] & 0x00f000f0u;
             } else {
                 const uint32_t x = pair_of(a, b, j), y = x >> 8;
                 f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
@@ -570,51 +614,60 @@ struct Worker {
     }
 
     // Cache tiles [a, b) of request r's head h into the rows' sums.
-    __device__ __forceinline__ void run(int r, int h, int rt, int nq, int kv, int a, int b) {
+    __device__ __forceinline__ void run(int r, int h, int rt, int start, int nq, int kv, int a, int b) {
         const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
         const int i0 = rt * NR / p.group, i1 = min((rt * NR + NR - 1) / p.group, nq - 1);
         const int first = kv - nq + i0, last = kv - nq + i1;                 // the rows' positions
         const int lo_any = p.a.window ? first - p.a.window + 1 : 0, hi_any = last + 1;
         const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;   // seen by every row
         uint8_t *ring = smem + warp * RING;
-        const int n = a + warp < b ? (b - a - warp + kWarps - 1) / kWarps : 0;    // this warp's tiles
-        long long at = -1;                                                        // lane i: where its tile 32 * (k / 32) + i lies
+        const int pairs = (b - a + 1) / 2, n = warp < pairs ? (pairs - warp + kWarps - 1) / kWarps : 0;      // this warp's pairs of tiles: warp, warp + 4, ...
+        int where = -1;                                                      // lane i: the number in the cache of tile i % 2 of pair 16 * (k / 16) + i / 2
         auto locate = [&](int k) {
-            at = -1;
-            if (k + lane < n) {
-                const int tl = a + warp + (k + lane) * kWarps, blk = tl / p.c.tiles, id = table[blk];
-                if (id >= 0 && id < p.c.n_pages) at = (long long)p.c.tile_at(id, h, tl - blk * p.c.tiles);
+            const int tl = a + 2 * (warp + (k + lane / 2) * kWarps) + lane % 2;
+            where = -1;
+            if (tl < b) {
+                const int blk = tl / p.c.tiles, id = table[blk];
+                if (id >= 0 && id < p.c.n_pages) where = (id * p.c.n_kv + h) * p.c.tiles + tl - blk * p.c.tiles;
                 else if (p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
             }
         };
-        uint32_t good = 0;                                                        // which of the ring's tiles are there
+        uint32_t good = 0;                                                   // which of the ring's tiles are there
         auto fetch = [&](int k) {
             if (k < n) {
-                if (k % 32 == 0) locate(k);
-                const long long from = __shfl_sync(0xffffffffu, at, k % 32);
-                const int st = k % kStages;
-                good = from < 0 ? good & ~(1u << st) : good | 1u << st;
-                if (from >= 0) {
-                    const uint8_t *src = p.c.data + from;
-                    const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + st * TB);
+                if (k % 16 == 0) locate(k);
+                const int st = k % 2 * 2;
+                good &= ~(3u << st);
 #pragma unroll
-                    for (int c = 0; c < TB; c += 512)
-                        if (c + 512 <= TB || c + lane * 16 < TB)
-                            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c + lane * 16), "l"(src + c + lane * 16) : "memory");
+                for (int u = 0; u < 2; u++) {
+                    const int from = __shfl_sync(0xffffffffu, where, k % 16 * 2 + u);
+                    if (from >= 0) {
+                        good |= 1u << (st + u);
+                        const uint8_t *src = p.c.data + (size_t)from * TB + lane * 16;
+                        const uint32_t dst = (uint32_t)__cvta_generic_to_shared(ring + (st + u) * TB) + lane * 16;
+#pragma unroll
+                        for (int c = 0; c < TB; c += 512)
+                            if (c + 512 <= TB || c + lane * 16 < TB)
+                                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + c), "l"(src + c) : "memory");
+                    }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-        for (int k = 0; k < kStages - 1; k++) fetch(k);
+        fetch(0);                                                            // under way while the rows are read
+        load_rows(start, nq, kv, h, rt);
         for (int k = 0; k < n; k++) {
-            fetch(k + kStages - 1);
-            asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 1) : "memory");
+            fetch(k + 1);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
             __syncwarp();
-            const int st = k % kStages;
-            if (good >> st & 1) {
-                const int tok0 = (a + warp + k * kWarps) * kKvTile;
-                if (tok0 >= whole_lo && tok0 + kKvTile <= whole_hi) tile<false>(ring + st * TB, tok0, lo_any, hi_any);
-                else tile<true>(ring + st * TB, tok0, lo_any, hi_any);
+            const int st = k % 2 * 2, tok0 = (a + 2 * (warp + k * kWarps)) * kKvTile;
+            const uint32_t both = good >> st & 3;
+            if (both == 3 && tok0 >= whole_lo && tok0 + 2 * kKvTile <= whole_hi) {
+                step<false, 2>(ring + st * TB, tok0, lo_any, hi_any);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < 2; u++)
+                    if (both >> u & 1) step<true, 1>(ring + (st + u) * TB, tok0 + u * kKvTile, lo_any, hi_any);
             }
             __syncwarp();
         }
@@ -730,6 +783,8 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
     extern __shared__ __align__(16) uint8_t smem[];
     W w(p, smem);
     const int n_req = p.a.n_req, heads = p.c.n_kv;
+    asm volatile("griddepcontrol.wait;" ::: "memory");                      // what ran before on the stream is done and visible
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the join's CTAs take this one's place as it ends, and wait for all
     // All segments' cache tiles in one line, request by request, head by head, row tile by row tile: a worker's share is [u0, u1).
     // Not split, the line is of segments (the same number for each request), and a worker takes every gridDim.x-th.
     __shared__ long long ws[kWarps];
@@ -751,7 +806,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
             total += sum;
         }
         share = (total + gridDim.x - 1) / gridDim.x;
-        share = max((share + kWarps - 1) / kWarps * kWarps, (long long)p.split);
+        share = max((share + 2 * kWarps - 1) / (2 * kWarps) * (2 * kWarps), (long long)p.split);
         u0 = share * blockIdx.x;
         u1 = min(u0 + share, total);
         long long base = 0;
@@ -776,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
             at = found_at;
         }
     }
-    int4 desc = make_int4(-1, 0, 0, 0);
+    int4 desc = make_int4(-1, 0, 0, 0), desc2 = make_int4(0, 0, 0, 0);
     while (u0 < u1) {
         if (!p.split) {
             r = (int)(u0 / per_req);
@@ -802,15 +857,19 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
         if (rt < q.rts) {
             const int last = q.kv - q.nq + min((rt * W::NR + W::NR - 1) / p.group, q.nq - 1), top = last >= 0 ? last / kKvTile + 1 : 0;
             const bool begins = off == 0, ends = off + len == q.tiles;
-            w.load_rows(q.start, q.nq, q.kv, h, rt);
-            w.run(r, h, rt, q.nq, q.kv, q.lo + off, min(q.lo + off + len, top));
+            w.run(r, h, rt, q.start, q.nq, q.kv, q.lo + off, min(q.lo + off + len, top));
             w.finish(q.start, q.nq, h, rt, begins && ends ? nullptr : p.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * W::NR * (W::DP + 4));
-            if (!begins && ends) desc = make_int4((int)((u0 - off) / share), r, h, rt);
+            if (!begins && ends) {
+                desc = make_int4((int)((u0 - off) / share), h, rt, 0);
+                desc2 = make_int4(q.start, q.nq, 0, 0);
+            }
         }
         u0 += p.split ? len : gridDim.x;
     }
-    if (p.split && threadIdx.x == 0) p.desc[blockIdx.x] = desc;
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");          // the join may take this CTA's place
+    if (p.split && threadIdx.x == 0) {
+        p.desc[2 * blockIdx.x] = desc;
+        p.desc[2 * blockIdx.x + 1] = desc2;
+    }
 }
 
 // The pieces of the segments that several workers shared, joined: CTA (w, y) does `rows` rows of the segment that ends
@@ -824,7 +883,7 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs p, 
     __shared__ float4 sv[kJoinThreads];
     __shared__ float2 sml[kJoinThreads];
     asm volatile("griddepcontrol.wait;" ::: "memory");                      // the workers are done and their pieces visible
-    const int4 d = p.desc[blockIdx.x];
+    const int4 d = p.desc[2 * blockIdx.x], d2 = p.desc[2 * blockIdx.x + 1];
     if (d.x < 0) return;
     const int items = rows * PER, parts = max(1, kJoinThreads / items), n = blockIdx.x - d.x + 1;
     for (int base = 0; base < items; base += kJoinThreads) {                 // one turn where parts > 1
@@ -835,16 +894,32 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs p, 
         float m = kFloor, l = 0.0f;
         float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         if (on) {
-#pragma unroll 8
-            for (int k = part; k < n; k += parts) m = fmaxf(m, piece(k)[W::DP]);
-#pragma unroll 4
-            for (int k = part; k < n; k += parts) {
-                const float *from = piece(k);
-                const float2 ml = *(const float2 *)(from + W::DP);
-                const float4 x = *(const float4 *)(from + at);
-                const float f = ex2(ml.x - m);
-                l = fmaf(ml.y, f, l);
-                v.x = fmaf(x.x, f, v.x); v.y = fmaf(x.y, f, v.y); v.z = fmaf(x.z, f, v.z); v.w = fmaf(x.w, f, v.w);
+            for (int k = part; k < n; k += 4 * parts) {                      // four pieces' loads at a time
+                float2 ml[4];
+                float4 x[4];
+                float to = m;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    ml[i] = make_float2(kFloor, 0.0f);
+                    x[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (k + i * parts < n) {
+                        const float *from = piece(k + i * parts);
+                        ml[i] = *(const float2 *)(from + W::DP);
+                        x[i] = *(const float4 *)(from + at);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; i++) to = fmaxf(to, ml[i].x);
+                float f = ex2(m - to);
+                m = to;
+                l *= f;
+                v.x *= f; v.y *= f; v.z *= f; v.w *= f;
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    f = ex2(ml[i].x - m);
+                    l = fmaf(ml[i].y, f, l);
+                    v.x = fmaf(x[i].x, f, v.x); v.y = fmaf(x[i].y, f, v.y); v.z = fmaf(x[i].z, f, v.z); v.w = fmaf(x[i].w, f, v.w);
+                }
             }
         }
         if (parts > 1) {
@@ -867,9 +942,8 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs p, 
             }
         }
         if (on && part == 0) {
-            const Request q = request_of(p, d.y, W::NR);
             W w(p, nullptr);
-            w.put(q.start, q.nq, d.z, d.w, row, at, v, l);
+            w.put(d2.x, d2.y, d.y, d.z, row, at, v, l);
         }
     }
 }
@@ -899,23 +973,26 @@ cudaError_t launch(AttendArgs p, cudaStream_t s) {
     p.row_tiles = (int)(((long long)p.a.max_q * p.group + W::NR - 1) / W::NR);
     p.split = p.a.max_kv > kSplitFrom ? kLeastShare : 0;
     p.desc = (int4 *)p.a.scratch;
-    p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * ctas_per_sm(NG, NT) * sizeof(int4));
+    p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * ctas_per_sm(NG, NT) * 2 * sizeof(int4));
     const long long segs = (long long)p.a.n_req * p.c.n_kv * p.row_tiles;
     const int grid = p.split ? workers : (int)std::min<long long>(segs, 1 << 20);
-    attend_kernel<T, MX, NG, NT><<<grid, kThreads, W::SMEM, s>>>(p);
-    e = cudaGetLastError();
-    if (e != cudaSuccess || !p.split) return e;
-    // Its CTAs may start while the last workers run (each waits for them); a row per CTA where a segment has many pieces.
-    const int rows = workers > 8 * segs ? 1 : W::NR;
+    // Both launches are programmatic: their CTAs may come up while what precedes them drains, and wait for it.
     cudaLaunchAttribute early;
     early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(workers, W::NR / rows);
-    cfg.blockDim = dim3(kJoinThreads);
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(kThreads);
+    cfg.dynamicSmemBytes = W::SMEM;
     cfg.stream = s;
     cfg.attrs = &early;
     cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, attend_kernel<T, MX, NG, NT>, p);
+    if (e != cudaSuccess || !p.split) return e;
+    const int rows = workers > 8 * segs ? 1 : W::NR;                         // a row per CTA where a segment has many pieces
+    cfg.gridDim = dim3(workers, W::NR / rows);
+    cfg.blockDim = dim3(kJoinThreads);
+    cfg.dynamicSmemBytes = 0;
     return cudaLaunchKernelEx(&cfg, join_kernel<T, MX, NG, NT>, p, rows);
 }
 
@@ -957,7 +1034,7 @@ L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend
     if (attend_error(cache, a)) return 0;
     if (a->max_kv <= kSplitFrom) return 16;
     const int ng = (cache->head_dim + kKvBlock - 1) / kKvBlock, nt = row_blocks(cache, a);
-    return (size_t)kMaxSms * ctas_per_sm(ng, nt) * (sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
+    return (size_t)kMaxSms * ctas_per_sm(ng, nt) * (2 * sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
 }
 
 L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, void *stream) {
