@@ -66,10 +66,10 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
     const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
     return *(const uint32_t *)&r;
 }
-// Two e2m1 codes (a byte, the low nibble first) as f16.
-__device__ __forceinline__ uint32_t e2m1_pair(uint32_t byte) {
+// The two e2m1 codes of byte K (the low nibble first) as f16.
+template <int K> __device__ __forceinline__ uint32_t e2m1_pair(uint32_t w) {
     uint32_t d;
-    asm("{ .reg .b8 c, z0, z1, z2;\n mov.b32 {c, z0, z1, z2}, %1;\n cvt.rn.f16x2.e2m1x2 %0, c; }" : "=r"(d) : "r"(byte));
+    asm("{ .reg .b8 c, z0, z1, z2;\n mov.b32 {c, z0, z1, z2}, %1;\n cvt.rn.f16x2.e2m1x2 %0, c; }" : "=r"(d) : "r"(w >> (8 * K)));
     return d;
 }
 
@@ -122,13 +122,13 @@ __device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfl
 __device__ __forceinline__ void store_f32(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-constexpr int kWarps = 4, kThreads = 32 * kWarps;
+constexpr int kWarps = 6, kThreads = 32 * kWarps;
 constexpr int kStages = 4;               // tiles of a warp's ring: two pairs
 constexpr int kMaxSms = 160;
 constexpr float kFloor = -1e30f;         // the reference of a row that has seen nothing
 
 // Resident CTAs per SM that the registers of a variant allow.
-constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 4 ? 4 : ng * nt <= 5 ? 3 : 2; }
+constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 5 ? 2 : 1; }
 
 struct Segment { int r, h, rt; };
 
@@ -405,13 +405,13 @@ struct Worker {
             for (int k = 0; k < 4; k += PREC ? 2 : 1)
 #pragma unroll
                 for (int i = 0; i < SW; i++) {
-                    if (MX) any = __vmaxu4(any, v[u][k][i]);
+                    if (MX) any |= v[u][k][i];                               // at least the largest; eref ends in ones, so that it is that mostly
                     else if (PREC) any = __vmaxu2(any, v[u][k][i] & 0x7fff7fffu);
                     else any |= v[u][k][i];
                 }
         if (MX) {
-            any = __vmaxu4(any, any >> 16);
-            move = (int)max(any & 0xff, any >> 8 & 0xff) > eref;
+            any |= any >> 16;
+            move = (int)((any | any >> 8) & 0xff) > eref;
         } else if (PREC) {
             move = (int)max(any >> 10 & 31, any >> 26) - 15 > vexp;
         } else {
@@ -444,6 +444,7 @@ struct Worker {
             for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
             float shrink = 1.0f;
             if (MX) {
+                top = min(top | 3, 254);
                 if (top > eref) {
                     shrink = top - eref > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (top - eref)) << 23);
                     eref = top;
@@ -535,8 +536,8 @@ struct Worker {
                     } else {
                         uint32_t d0, d1;
                         if (MX) {
-                            d0 = rel_f16(v[u][0][j / 4], v[u][1][j / 4], j % 4);
-                            d1 = rel_f16(v[u][2][j / 4], v[u][3][j / 4], j % 4);
+                            d0 = rel_f16(v[u][0], v[u][1], j);
+                            d1 = rel_f16(v[u][2], v[u][3], j);
                         } else {
                             d0 = pair_of(v[u][0], v[u][1], j);
                             d1 = pair_of(v[u][2], v[u][3], j);
@@ -557,8 +558,8 @@ struct Worker {
     // A word's 8 codes as four pairs.
     __device__ __forceinline__ static void codes4(uint32_t *f, uint32_t x) {
         if (MX) {
-#pragma unroll
-            for (int k = 0; k < 4; k++) f[k] = e2m1_pair(x >> (8 * k));
+            f[0] = e2m1_pair<0>(x); f[1] = e2m1_pair<1>(x);
+            f[2] = e2m1_pair<2>(x); f[3] = e2m1_pair<3>(x);
         } else {
             if (SUBN) {                                                      // r and y of the low bytes, then of the high ones
                 f[1] = x & 0x00ff00ffu; f[0] = x & 0x000f000fu;
@@ -574,12 +575,11 @@ struct Worker {
     // Block j's 4 codes of two tokens as four pairs of the same dim.
     __device__ __forceinline__ static void value4(uint32_t *f, const uint32_t *a, const uint32_t *b, int j) {
         if (MX) {
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                const uint32_t x = e2m1_pair(a[j / 2] >> (16 * (j % 2) + 8 * k)), y = e2m1_pair(b[j / 2] >> (16 * (j % 2) + 8 * k));
-                f[2 * k] = prmt(x, y, 0x5410);
-                f[2 * k + 1] = prmt(x, y, 0x7632);
-            }
+            const uint32_t wa = a[j / 2], wb = b[j / 2];
+            const uint32_t x0 = j % 2 ? e2m1_pair<2>(wa) : e2m1_pair<0>(wa), y0 = j % 2 ? e2m1_pair<2>(wb) : e2m1_pair<0>(wb);
+            const uint32_t x1 = j % 2 ? e2m1_pair<3>(wa) : e2m1_pair<1>(wa), y1 = j % 2 ? e2m1_pair<3>(wb) : e2m1_pair<1>(wb);
+            f[0] = prmt(x0, y0, 0x5410); f[1] = prmt(x0, y0, 0x7632);
+            f[2] = prmt(x1, y1, 0x5410); f[3] = prmt(x1, y1, 0x7632);
         } else {
             if (SUBN) {                                                      // y = n0 + 16 n1 and 16 n1 of the low bytes, then of the high ones
                 const uint32_t x = pair_of(a, b, j);
@@ -608,9 +608,10 @@ struct Worker {
     }
     // mxfp4 scales relative to eref: 2^(e - eref).
     __device__ __forceinline__ float rel_f32(uint32_t e) const { return __uint_as_float((uint32_t)max((int)e - eref + 127, 0) << 23); }
-    __device__ __forceinline__ uint32_t rel_f16(uint32_t a, uint32_t b, int k) const {
-        const uint32_t x = prmt(a >> (8 * k), b >> (8 * k), 0x5410) & 0x00ff00ffu, base = (uint32_t)(eref - 15) * 0x10001u;
-        return (__vmaxs2(x, base) - base) << 10;
+    __device__ __forceinline__ uint32_t rel_f16(const uint32_t *a, const uint32_t *b, int j) const {
+        const uint32_t x = prmt(a[j / 4], b[j / 4], j % 4 < 2 ? 0x5410 : 0x7632), base = (uint32_t)(eref - 15) * 0x10001u;      // two blocks' bytes of both tokens
+        const uint32_t e = j % 2 ? prmt(x, 0, 0x4341) : x & 0x00ff00ffu;
+        return __vmaxs2(e, base) * 1024u - base * 1024u;
     }
 
     // Cache tiles [a, b) of request r's head h into the rows' sums.
