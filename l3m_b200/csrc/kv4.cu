@@ -23,8 +23,7 @@ int refuse(const char *entry, const char *why) {
     return l3m_error_msg(msg);
 }
 
-int launched(const char *entry) {
-    const cudaError_t e = cudaGetLastError();
+int launched(cudaError_t e, const char *entry) {
     return e == cudaSuccess ? 0 : l3m_error_cuda(e, entry);
 }
 
@@ -87,6 +86,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
     __shared__ int left_s;
     const int tid = threadIdx.x;
     int status = 0;
+    asm volatile("griddepcontrol.wait;" ::: "memory");                      // what ran before on the stream is done and visible
 
     const int free0 = *a.n_free;
     const int old_top = min(max(free0, 0), a.n_pages);
@@ -203,34 +203,47 @@ constexpr int kQkvThreads = 256;
 
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ void from_f32(float *p, float x) { *p = x; }
-__device__ __forceinline__ void from_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-// 8 values at p: one or two 16-byte accesses where every row starts 16-byte aligned (vec), else one by one.
-__device__ __forceinline__ void load8(float *x, const float *p, bool vec) {
-    if (vec) {
-        const float4 a = ((const float4 *)p)[0], b = ((const float4 *)p)[1];
+// 8 values at p as they lie in memory: one or two 16-byte accesses where every row starts 16-byte aligned (vec), else one by one.
+template <typename T> struct Raw8;
+template <> struct Raw8<float> {
+    float4 a, b;
+    __device__ __forceinline__ void load(const float *p, bool vec) {
+        if (vec) {
+            a = ((const float4 *)p)[0];
+            b = ((const float4 *)p)[1];
+        } else {
+            a = make_float4(p[0], p[1], p[2], p[3]);
+            b = make_float4(p[4], p[5], p[6], p[7]);
+        }
+    }
+    __device__ __forceinline__ void zero() { a = b = make_float4(0.0f, 0.0f, 0.0f, 0.0f); }
+    __device__ __forceinline__ void get(float *x) const {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = p[e];
     }
-}
-__device__ __forceinline__ void load8(float *x, const __nv_bfloat16 *p, bool vec) {
-    if (vec) {
-        const uint4 v = *(const uint4 *)p;
-        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+};
+template <> struct Raw8<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vec) {
+        if (vec) {
+            const uint4 v = *(const uint4 *)p;
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+        } else {
+            const uint16_t *h = (const uint16_t *)p;
+#pragma unroll
+            for (int e = 0; e < 4; e++) w[e] = h[2 * e] | (uint32_t)h[2 * e + 1] << 16;
+        }
+    }
+    __device__ __forceinline__ void zero() { w[0] = w[1] = w[2] = w[3] = 0; }
+    __device__ __forceinline__ void get(float *x) const {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             x[2 * e] = __uint_as_float(w[e] << 16);
             x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
         }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = __bfloat162float(p[e]);
     }
-}
+};
 __device__ __forceinline__ void store8(float *p, const float *x, float f, bool vec) {
     if (vec) {
         ((float4 *)p)[0] = make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
@@ -256,7 +269,8 @@ struct QkvArgs {
     l3m_qkv a;
     Kv4Dev c;
     int store, mx, vec;
-    int heads, chunks, per_chunk;         // rows per token; warps per token and the rows each takes
+    int q_groups, k_groups, groups;       // a token's row groups (one warp's rows at a time): queries, keys, all
+    int chunks, per_chunk;                // warps per token and the groups each takes
 };
 
 __device__ __forceinline__ double finite(double x) { return x != x ? 0.0 : fmin(fmax(x, -(double)FLT_MAX), (double)FLT_MAX); }
@@ -331,8 +345,9 @@ __device__ __noinline__ Held exact_row(const T *src, const float *w, const float
     return r;
 }
 
-// A row (a head of a token) is held by LPR lanes, 8 contiguous dims each, so 4 lanes hold a block. A warp
-// takes a run of one token's rows (queries, then keys, then values): position, rotation and slot are read once.
+// A row (a head of a token) is held by LPR lanes, 8 contiguous dims each, so 4 lanes hold a block; a group of 32 / LPR rows
+// of one kind is a warp's work at a time. A warp takes a run of one token's groups (queries, then keys, then
+// values): position, rotation and slot are read once, and the next group's rows are under way while one is worked on.
 //
 // Codes and scales have to be those of exact arithmetic, but a value next to a border between two codes may land
 // on either side of it in 32 bits. So u (the normed, rotated value before the row's factor, which
@@ -340,91 +355,87 @@ __device__ __noinline__ Held exact_row(const T *src, const float *w, const float
 // distance from the border, and where the distance is within the bound the row is redone in 64 bits (about 1% of the rows).
 // q4_0's test is exact for exact u: code >= b iff (b - 8.5) / 8 * |top| + u * sign(top) <= 0, one fma whose sign cannot
 // be rounded away; so values, which are neither normed nor rotated, never need 64 bits for it.
+enum { kQuery, kKey, kValue };
+
 template <typename T, int LPR, int ROPE>
-__global__ void __launch_bounds__(kQkvThreads) qkv_kernel(const QkvArgs p) {
-    const l3m_qkv &a = p.a;
-    __shared__ float mate_buf[ROPE == 2 ? kQkvThreads * 8 : 1];
-    constexpr int RPW = 32 / LPR;
-    const int wl = threadIdx.x & 31, lane = wl & (LPR - 1), sub = wl / LPR;
-    const int D = a.head_dim, d0 = lane * 8, half = ROPE ? a.rot_dim / 2 : 0;
-    const bool in = d0 < D;
-    float qw[8], kw[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        qw[e] = a.q_norm && in ? a.q_norm[d0 + e] : 1.0f;
-        kw[e] = a.k_norm && in ? a.k_norm[d0 + e] : 1.0f;
+struct RowWorker {
+    static constexpr int RPW = 32 / LPR;
+    const QkvArgs &p;
+    float *mate_buf;
+    int wl, lane, sub, d0, half, tok, tr;
+    bool in, partial;
+    int shift, mate_lane;
+    float cs[8], sn[8];                   // cos and sin of this lane's dims, sin with the sign of the mate's term
+    const float *turn;
+    uint8_t *tile;
+
+    __device__ __forceinline__ RowWorker(const QkvArgs &args, float *buf) : p(args), mate_buf(buf) {
+        wl = threadIdx.x & 31;
+        lane = wl & (LPR - 1);
+        sub = wl / LPR;
+        d0 = lane * 8;
+        half = ROPE ? p.a.rot_dim / 2 : 0;
+        in = d0 < p.a.head_dim;
+        partial = ROPE && p.a.rot_dim < p.a.head_dim;
+        shift = ROPE == 2 && (half & 7) == 0 ? half >> 3 : 0;                 // halves: the mate's lane is this far away; 0: through shared memory
+        mate_lane = (wl & ~(LPR - 1)) + (d0 < half ? lane + shift : d0 < 2 * half ? lane - shift : lane);
     }
-    const bool partial = ROPE && a.rot_dim < D;
-    const int shift = ROPE == 2 && (half & 7) == 0 ? half >> 3 : 0;           // halves: the mate's lane is this far away; 0: through shared memory
-    const int mate_lane = (wl & ~(LPR - 1)) + (d0 < half ? lane + shift : d0 < 2 * half ? lane - shift : lane);
-    const long long items = (long long)a.n_tokens * p.chunks;
-    for (long long item = blockIdx.x * (kQkvThreads / 32) + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * (kQkvThreads / 32)) {
-        const int tok = (int)(item / p.chunks), first = (int)(item - (long long)tok * p.chunks) * p.per_chunk, end = min(first + p.per_chunk, p.heads);
-        const int pos = a.pos[tok];
-        if (pos < 0) continue;
-        if (ROPE && pos >= a.n_pos) {
-            if (a.status && wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_POS);
-            continue;
-        }
-        uint8_t *tile = nullptr;
-        int tr = 0;
-        if (p.store) {
-            const int slot = a.slot[tok];
-            if (slot >= p.c.n_pages * p.c.page) {
-                if (a.status && wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
-            } else if (slot >= 0) {
-                const int page = slot / p.c.page, off = slot - page * p.c.page;
-                tile = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
-                tr = off % kKvTile;
-            }
-        }
-        // cos and sin of this lane's dims; halves carry the sign of the mate's term in sin
-        float cs[8], sn[8];
-        const float *turn = ROPE ? a.rope_table + (size_t)pos * half * 2 : nullptr;
+    __device__ __forceinline__ void rotation(int pos) {
+        turn = ROPE ? p.a.rope_table + (size_t)pos * half * 2 : nullptr;
         if (ROPE) {
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const int d = d0 + e;
+                cs[e] = 1.0f;
+                sn[e] = 0.0f;
                 if (d < 2 * half) {
                     const int i = ROPE == 1 ? d >> 1 : d < half ? d : d - half;
                     const float2 t = *(const float2 *)(turn + 2 * i);
                     cs[e] = t.x;
                     sn[e] = (ROPE == 1 ? e & 1 : d >= half) ? t.y : -t.y;
-                } else {
-                    cs[e] = 1.0f;
-                    sn[e] = 0.0f;
                 }
             }
         }
-        for (int hb = first; hb < end; hb += RPW) {
-            const int h = hb + sub;
-            const bool live = h < end;
-            const int kind = !live || h < a.n_heads ? 0 : h < p.heads - (p.store ? a.n_kv_heads : 0) ? 1 : 2;
-            const int hh = kind == 0 ? h : kind == 1 ? h - a.n_heads : h - (p.heads - a.n_kv_heads);
-            const T *src = (const T *)(kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (size_t)tok * (kind == 0 ? a.q_ld : kind == 1 ? a.k_ld : a.v_ld) + (size_t)hh * D;
-            float u[8];
-            if (live && in) {
-                load8(u, src + d0, p.vec);
-            } else {
+    }
+
+    // Groups [g0, g1) of a kind.
+    template <int KIND> __device__ __forceinline__ void rows(int g0, int g1) {
+        const l3m_qkv &a = p.a;
+        const int heads = KIND == kQuery ? a.n_heads : a.n_kv_heads;
+        const T *src = (const T *)(KIND == kQuery ? a.q : KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kQuery ? a.q_ld : KIND == kKey ? a.k_ld : a.v_ld) + d0;
+        const float *w = KIND == kQuery ? a.q_norm : KIND == kKey ? a.k_norm : nullptr;
+        float wt[8];
+        if (KIND != kValue && w && in) {
 #pragma unroll
-                for (int e = 0; e < 8; e++) u[e] = 0.0f;
-            }
-            const float *w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+            for (int e = 0; e < 8; e++) wt[e] = w[d0 + e];
+        }
+        const int D = a.head_dim;
+        const float inv_d = 1.0f / (float)D;
+        Raw8<T> next;
+        auto fetch = [&](int g) {
+            const int h = g * RPW + sub;
+            if (g < g1 && h < heads && in) next.load(src + (size_t)h * D, p.vec);
+            else next.zero();
+        };
+        fetch(g0);
+        for (int g = g0; g < g1; g++) {
+            const int h = g * RPW + sub;
+            const bool live = h < heads;
+            float u[8];
+            next.get(u);
+            fetch(g + 1);
             float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value
-            if (a.q_norm || a.k_norm) {
+            if (KIND != kValue && w) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) ss = fmaf(u[e], u[e], ss);
 #pragma unroll
                 for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                if (w) {
-                    const float m = __fdiv_rn(ss, (float)D) + a.eps;
-                    f = __frcp_rn(__fsqrt_rn(m));
+                f = rsqrtf(fmaf(ss, inv_d, a.eps));
 #pragma unroll
-                    for (int e = 0; e < 8; e++) u[e] *= kind ? kw[e] : qw[e];
-                }
+                for (int e = 0; e < 8; e++) u[e] = in ? u[e] * wt[e] : 0.0f;
             }
-            if (ROPE) {
+            if (KIND != kValue && ROPE) {
                 float m[8];
                 if (ROPE == 1) {
 #pragma unroll
@@ -444,100 +455,152 @@ __global__ void __launch_bounds__(kQkvThreads) qkv_kernel(const QkvArgs p) {
                         m[e] = d < half ? row[d + half] : d < 2 * half ? row[d - half] : 0.0f;
                     }
                 }
-                if (kind < 2) {
 #pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        size = fmaxf(size, fabsf(u[e]) + fabsf(m[e]));
-                        const float r = fmaf(m[e], sn[e], u[e] * cs[e]);
-                        u[e] = partial && d0 + e >= a.rot_dim ? u[e] : r;
-                    }
+                for (int e = 0; e < 8; e++) {
+                    if (KIND == kKey) size = fmaxf(size, fabsf(u[e]) + fabsf(m[e]));
+                    const float r = fmaf(m[e], sn[e], u[e] * cs[e]);
+                    u[e] = partial && d0 + e >= a.rot_dim ? u[e] : r;
                 }
             }
             Held held = {0, 0};
-            const bool keep = live && kind && tile;
-            if (__any_sync(0xffffffffu, keep)) {
-                // The block's extremes; zero keeps a sum of zeros, anything not finite spoils it.
-                float hi = u[0], lo = u[0], zero = 0.0f;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    hi = fmaxf(hi, u[e]);
-                    lo = fminf(lo, u[e]);
-                    zero = fmaf(u[e], 0.0f, zero);
-                }
-#pragma unroll
-                for (int o = 1; o < 4; o <<= 1) {
-                    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-                    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-                    size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
-                }
-                const float mag = fmaxf(hi, -lo);
-                // An upper bound on the error of u: three roundings of |a| + |b| at 2^-24 (the rotation), one of u (the weight).
-                const bool exact = kind == 2 || (!w && !(ROPE && a.rot_dim));
-                const float err = exact ? 0.0f : ROPE && a.rot_dim ? size * 0x1p-22f : mag * 0x1p-23f;
-                bool again = !(zero == 0.0f) || (mag < 0x1p-100f && (mag > 0.0f || err > 0.0f)) || mag > 0x1p120f;
-                if (!p.mx) {
-                    // opposite signs of one size: the sign of the first decides
-                    again |= mag > 0.0f && fabsf(hi + lo) <= 2.0f * err;
-                    const float top = hi >= -lo ? hi : lo, inv = __fdividef(-8.0f, top), sgn = hi >= -lo ? 1.0f : -1.0f;
-                    const float tol = exact ? -1.0f : 3.0f * err + mag * 0x1p-22f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float b = rintf(fmaf(u[e], inv, 8.5f));
-                        const float r = fmaf(fmaf(b, 0.125f, -1.0625f), mag, u[e] * sgn);
-                        again |= fabsf(r) <= tol;
-                        const int code = (int)b - (r <= 0.0f ? 0 : 1);
-                        held.codes |= (unsigned)min(max(code, 0), 15) << (4 * e);
-                    }
-                    const float s = top * -0.125f * f, rel = 0x1p-20f + __fdividef(2.0f * err, mag);
-                    const unsigned short s0 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f - rel), -65504.0f), 65504.0f)));
-                    const unsigned short s1 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f + rel), -65504.0f), 65504.0f)));
-                    if (exact) held.scale = __half_as_ushort(__float2half_rn(fminf(fmaxf(s, -65504.0f), 65504.0f)));
-                    else held.scale = s0;
-                    again |= !exact && s0 != s1;
-                    if (mag == 0.0f) held = {0x88888888u, 0};
-                } else {
-                    const float m = mag * f, rel = exact ? 0.0f : 0x1p-20f + __fdividef(2.0f * err, mag);
-                    const unsigned e0 = __float_as_uint(m * (1.0f - rel)) >> 23, e1 = __float_as_uint(m * (1.0f + rel)) >> 23;
-                    again |= mag > 0.0f && (e0 != e1 || e0 < 20u || e0 > 250u || f > 0x1p17f);   // far from either end, fi below is a normal number
-                    const float inv = mag > 0.0f ? __uint_as_float((256u - e0) << 23) : 0.0f;   // 2^(127 - e8), e8 = e0 - 2
-                    const float fi = f * inv, tol = exact ? -1.0f : (3.0f * err + mag * 0x1p-20f) * fi * 2.0f;
-#pragma unroll
-                    for (int e = 0; e < 8; e++) {
-                        const float v = fabsf(u[e]) * fi;                     // in [0, 8): the steps are 1/2 below 2, 1 below 4, 2 above
-                        const float r = fmaf(v, v < 2.0f ? 2.0f : v < 4.0f ? 1.0f : 0.5f, -0.5f), c = ceilf(r);
-                        again |= fabsf(r - rintf(r)) <= tol;
-                        const int code = min((int)c + (v < 2.0f ? 0 : v < 4.0f ? 2 : 4), 7);
-                        held.codes |= (unsigned)(code | (u[e] < 0.0f && code ? 8 : 0)) << (4 * e);
-                    }
-                    held.scale = mag > 0.0f ? e0 - 2 : 0;
-                }
-                again &= keep;
-                if (__any_sync(0xffffffffu, again)) {
-                    const Held h64 = exact_row<T, LPR, ROPE>(live ? src : nullptr, w, kind == 2 ? nullptr : turn, D, kind == 2 ? 0 : a.rot_dim, a.eps, p.mx);
-                    const unsigned blockmask = 0xfu << (wl & ~3);
-                    if (__ballot_sync(0xffffffffu, again) & blockmask) held = h64;
+            if (KIND != kQuery && tile) held = KIND == kKey ? quantise<KIND>(u, size, f, w, src + (size_t)h * D - d0, live) : quantise<KIND>(u, 0.0f, 1.0f, nullptr, src + (size_t)h * D - d0, live);
+            if (KIND != kValue) {
+                T *out = (T *)(KIND == kQuery ? a.q_out : a.k_out);
+                if (out) {
+                    __syncwarp();                                            // in place: every lane has read its row
+                    if (live && in) store8(out + (size_t)tok * (KIND == kQuery ? a.q_out_ld : a.k_out_ld) + (size_t)h * D + d0, u, f, p.vec);
                 }
             }
-            __syncwarp();                                                    // in place: every lane has read its row
-            if (live && in && kind == 0) store8((T *)a.q_out + (size_t)tok * a.q_out_ld + (size_t)hh * D + d0, u, f, p.vec);
-            if (live && in && kind == 1 && a.k_out) store8((T *)a.k_out + (size_t)tok * a.k_out_ld + (size_t)hh * D + d0, u, f, p.vec);
-            if (keep && lane < 4 * p.c.ng) {
-                const int j = lane >> 2, t = lane & 3, ng = p.c.ng;
-                uint8_t *at = tile + (size_t)hh * p.c.tiles * p.c.tile_bytes;
-                if (kind == 1) {
-                    *(uint32_t *)(at + tr * 16 * ng + (t * ng + j) * 4) = held.codes;
-                } else {
-                    uint16_t *v = (uint16_t *)(at + 256 * ng + tr * 16 * ng);
-                    v[2 * t * ng + j] = (uint16_t)held.codes;
-                    v[(2 * t + 1) * ng + j] = (uint16_t)(held.codes >> 16);
-                }
-                if (t == 0) {
-                    uint8_t *s = at + (kind == 1 ? p.c.k_scales() : p.c.v_scales()) + (tr * ng + j) * p.c.sb;
-                    if (p.mx) *s = (uint8_t)held.scale;
-                    else *(uint16_t *)s = (uint16_t)held.scale;
-                }
+            if (KIND != kQuery && tile && live && lane < 4 * p.c.ng) put<KIND>(h, held);
+        }
+    }
+
+    template <int KIND> __device__ __forceinline__ Held quantise(const float *u, float size, float f, const float *w, const T *src, bool live) const {
+        // The block's extremes; zero keeps a sum of zeros, anything not finite spoils it.
+        float hi = u[0], lo = u[0], zero = 0.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            hi = fmaxf(hi, u[e]);
+            lo = fminf(lo, u[e]);
+            zero = fmaf(u[e], 0.0f, zero);
+        }
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+            hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+            lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+            if (KIND == kKey && ROPE) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
+        }
+        const float mag = fmaxf(hi, -lo);
+        // An upper bound on the error of u: three roundings of |a| + |b| at 2^-24 (the rotation), one of u (the weight).
+        const bool exact = KIND == kValue || (!w && !ROPE);
+        const float err = exact ? 0.0f : ROPE ? size * 0x1p-22f : mag * 0x1p-23f;
+        bool again = !(zero == 0.0f) || (mag < 0x1p-100f && (mag > 0.0f || err > 0.0f)) || mag > 0x1p120f;
+        Held held = {0, 0};
+        if (!p.mx) {
+            // opposite signs of one size: the sign of the first decides
+            again |= mag > 0.0f && fabsf(hi + lo) <= 2.0f * err;
+            const float top = hi >= -lo ? hi : lo, inv = __fdividef(-8.0f, top), sgn = hi >= -lo ? 1.0f : -1.0f;
+            const float tol = exact ? -1.0f : 3.0f * err + mag * 0x1p-22f;
+            float near = FLT_MAX;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                // The candidate border next to t = u / d + 8.5, as an integer in the low bits of b; r: on which side u lies, and how far
+                const float b = fmaf(u[e], inv, 8.5f) + 12582912.0f, k = b - 12582912.0f;
+                const float r = fmaf(fmaf(k, 0.125f, -1.0625f), mag, u[e] * sgn);
+                near = fminf(near, fabsf(r));
+                int code = (int)__float_as_uint(b) - 0x4b400000 - (r <= 0.0f ? 0 : 1);
+                code = min(max(code, 0), 15);
+                held.codes |= (unsigned)code << (4 * e);
+            }
+            again |= near <= tol;
+            const float s = top * -0.125f * f;
+            if (exact) {
+                held.scale = __half_as_ushort(__float2half_rn(fminf(fmaxf(s, -65504.0f), 65504.0f)));
+            } else {
+                const float rel = 0x1p-20f + __fdividef(2.0f * err, mag);
+                const unsigned short s0 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f - rel), -65504.0f), 65504.0f)));
+                const unsigned short s1 = __half_as_ushort(__float2half_rn(fminf(fmaxf(s * (1.0f + rel), -65504.0f), 65504.0f)));
+                held.scale = s0;
+                again |= s0 != s1;
+            }
+            if (mag == 0.0f) held = {0x88888888u, 0};
+        } else {
+            const float m = mag * f, rel = exact ? 0.0f : 0x1p-20f + __fdividef(2.0f * err, mag);
+            const unsigned e0 = __float_as_uint(m * (1.0f - rel)) >> 23, e1 = __float_as_uint(m * (1.0f + rel)) >> 23;
+            again |= mag > 0.0f && (e0 != e1 || e0 < 20u || e0 > 250u || f > 0x1p17f);   // far from either end, fi below is a normal number
+            const float inv = mag > 0.0f ? __uint_as_float((256u - e0) << 23) : 0.0f;   // 2^(127 - e8), e8 = e0 - 2
+            const float fi = f * inv, tol = exact ? -1.0f : (3.0f * err + mag * 0x1p-20f) * fi * 2.0f;
+            float near = FLT_MAX;
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = fabsf(u[e]) * fi;                             // in [0, 8): the steps are 1/2 below 2, 1 below 4, 2 above
+                const float r = fmaf(v, v < 2.0f ? 2.0f : v < 4.0f ? 1.0f : 0.5f, -0.5f), c = ceilf(r);
+                near = fminf(near, fabsf(r - rintf(r)));
+                const int code = min((int)c + (v < 2.0f ? 0 : v < 4.0f ? 2 : 4), 7);
+                held.codes |= (unsigned)(code | (u[e] < 0.0f && code ? 8 : 0)) << (4 * e);
+            }
+            again |= near <= tol;
+            held.scale = mag > 0.0f ? e0 - 2 : 0;
+        }
+        again &= live;
+        if (__any_sync(0xffffffffu, again)) {
+            const Held h64 = exact_row<T, LPR, ROPE>(live ? src : nullptr, w, KIND == kValue ? nullptr : turn, p.a.head_dim, KIND == kValue ? 0 : p.a.rot_dim, p.a.eps, p.mx);
+            const unsigned block = 0xfu << (wl & ~3);
+            if (__ballot_sync(0xffffffffu, again) & block) held = h64;
+        }
+        return held;
+    }
+
+    template <int KIND> __device__ __forceinline__ void put(int h, const Held &held) const {
+        const int j = lane >> 2, t = lane & 3, ng = p.c.ng;
+        uint8_t *at = tile + (size_t)h * p.c.tiles * p.c.tile_bytes;
+        if (KIND == kKey) {
+            *(uint32_t *)(at + tr * 16 * ng + (t * ng + j) * 4) = held.codes;
+        } else {
+            uint16_t *v = (uint16_t *)(at + 256 * ng + tr * 16 * ng);
+            v[2 * t * ng + j] = (uint16_t)held.codes;
+            v[(2 * t + 1) * ng + j] = (uint16_t)(held.codes >> 16);
+        }
+        if (t == 0) {
+            uint8_t *s = at + (KIND == kKey ? p.c.k_scales() : p.c.v_scales()) + (tr * ng + j) * p.c.sb;
+            if (p.mx) *s = (uint8_t)held.scale;
+            else *(uint16_t *)s = (uint16_t)held.scale;
+        }
+    }
+};
+
+template <typename T, int LPR, int ROPE>
+__global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const QkvArgs p) {
+    const l3m_qkv &a = p.a;
+    __shared__ float mate_buf[ROPE == 2 ? kQkvThreads * 8 : 1];
+    RowWorker<T, LPR, ROPE> w(p, mate_buf);
+    asm volatile("griddepcontrol.wait;" ::: "memory");                      // what ran before on the stream is done and visible
+    const long long items = (long long)a.n_tokens * p.chunks;
+    for (long long item = blockIdx.x * (kQkvThreads / 32) + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * (kQkvThreads / 32)) {
+        const int tok = (int)(item / p.chunks), g0 = (int)(item - (long long)tok * p.chunks) * p.per_chunk, g1 = min(g0 + p.per_chunk, p.groups);
+        const int pos = a.pos[tok];
+        if (pos < 0) continue;
+        if (ROPE && pos >= a.n_pos) {
+            if (a.status && w.wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_POS);
+            continue;
+        }
+        w.tok = tok;
+        w.tile = nullptr;
+        if (p.store) {
+            const int slot = a.slot[tok];
+            if (slot >= p.c.n_pages * p.c.page) {
+                if (a.status && w.wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
+            } else if (slot >= 0) {
+                const int page = slot / p.c.page, off = slot - page * p.c.page;
+                w.tile = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
+                w.tr = off % kKvTile;
             }
         }
+        if (g0 < p.q_groups + p.k_groups) w.rotation(pos);
+        if (g0 < p.q_groups) w.template rows<kQuery>(g0, min(g1, p.q_groups));
+        const int k0 = p.q_groups, v0 = p.q_groups + p.k_groups;
+        if (g0 < v0 && g1 > k0) w.template rows<kKey>(max(g0 - k0, 0), min(g1, v0) - k0);
+        if (g1 > v0 && w.tile) w.template rows<kValue>(max(g0 - v0, 0), g1 - v0);
     }
 }
 
@@ -545,7 +608,8 @@ __global__ void __launch_bounds__(kQkvThreads) qkv_kernel(const QkvArgs p) {
 
 struct LoadArgs {
     Kv4Dev c;
-    int mx, n;
+    int mx, n, parts, vec;
+    unsigned per_part;                    // 2^32 / parts, rounded up: i / parts = i * per_part >> 32 for the small i here
     void *k, *v;
     const int32_t *slots;
 };
@@ -559,30 +623,48 @@ __device__ __forceinline__ float scale_value(const uint8_t *p, int mx) {
     return mx ? (*p ? __uint_as_float((uint32_t)*p << 23) : __uint_as_float(0x00400000u)) : __half2float(*(const __half *)p);
 }
 
-// One thread per 8 values of one row.
+// One warp per row: the lanes go over its keys' and values' pieces of 8.
 template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const LoadArgs p) {
-    const int parts = p.c.dim / 8;
-    const long long items = (long long)p.n * p.c.n_kv * parts * 2;
-    for (long long i = blockIdx.x * 256LL + threadIdx.x; i < items; i += gridDim.x * 256LL) {
-        const int c = (int)(i % parts);
-        long long r = i / parts;
-        const int head = (int)(r % p.c.n_kv);
-        r /= p.c.n_kv;
-        const int row = (int)(r % p.n), is_v = (int)(r / p.n);
-        T *out = (T *)(is_v ? p.v : p.k);
+    const int lane = threadIdx.x & 31, per = p.c.n_kv * p.parts, ng = p.c.ng;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    for (long long row = blockIdx.x * 8LL + (threadIdx.x >> 5); row < p.n; row += gridDim.x * 8LL) {
         const int slot = p.slots[row];
-        if (!out || slot < 0 || slot >= p.c.n_pages * p.c.page) continue;
-        const int page = slot / p.c.page, off = slot - page * p.c.page, tr = off % kKvTile, j = c >> 2, t = c & 3, ng = p.c.ng;
-        const uint8_t *tile = p.c.data + p.c.tile_at(page, head, off / kKvTile);
-        const uint8_t *codes = tile + (is_v ? 256 * ng : 0) + tr * 16 * ng;
-        uint32_t w;
-        if (is_v) w = ((const uint16_t *)codes)[2 * t * ng + j] | (uint32_t)((const uint16_t *)codes)[(2 * t + 1) * ng + j] << 16;
-        else w = ((const uint32_t *)codes)[t * ng + j];
-        const float s = scale_value(tile + (is_v ? p.c.v_scales() : p.c.k_scales()) + (tr * ng + j) * p.c.sb, p.mx);
-        T *dst = out + ((size_t)row * p.c.n_kv + head) * p.c.dim + c * 8;
-        for (int e = 0; e < 8; e++) from_f32(dst + e, code_value(w >> (4 * e) & 15, p.mx) * s);
+        if (slot < 0 || slot >= p.c.n_pages * p.c.page) continue;
+        const int page = slot / p.c.page, off = slot - page * p.c.page, tr = off % kKvTile;
+        const uint8_t *tile0 = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
+        for (int i = lane; i < 2 * per; i += 32) {
+            const int is_v = i >= per, x = is_v ? i - per : i, head = p.parts == 1 ? x : (int)__umulhi((unsigned)x, p.per_part), c = x - head * p.parts, j = c >> 2, t = c & 3;
+            T *out = (T *)(is_v ? p.v : p.k);
+            if (!out) continue;
+            const uint8_t *tile = tile0 + (size_t)head * p.c.tiles * p.c.tile_bytes;
+            const uint8_t *codes = tile + (is_v ? 256 * ng : 0) + tr * 16 * ng;
+            uint32_t w;
+            if (is_v) w = ((const uint16_t *)codes)[2 * t * ng + j] | (uint32_t)((const uint16_t *)codes)[(2 * t + 1) * ng + j] << 16;
+            else w = ((const uint32_t *)codes)[t * ng + j];
+            const float s = scale_value(tile + (is_v ? p.c.v_scales() : p.c.k_scales()) + (tr * ng + j) * p.c.sb, p.mx);
+            float x8[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) x8[e] = code_value(w >> (4 * e) & 15, p.mx);
+            store8(out + ((size_t)row * p.c.n_kv + head) * p.c.dim + c * 8, x8, s, p.vec);
+        }
     }
+}
+
+// Launches with the grid allowed up while what precedes it on the stream drains: the kernels here wait for it themselves.
+template <typename... P, typename... A>
+cudaError_t launch_early(void (*kernel)(P...), int grid, int block, size_t smem, cudaStream_t s, const A &...args) {
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 int sm_count() {
@@ -622,8 +704,7 @@ L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream) {
     const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return l3m_error_cuda(e, me);
     const int grid = std::max(1, std::min(sm_count(), (a->max_tokens + kPlanThreads - 1) / kPlanThreads));
-    plan_kernel<<<grid, kPlanThreads, smem, (cudaStream_t)stream>>>(p);
-    return launched(me);
+    return launched(launch_early(plan_kernel, grid, kPlanThreads, smem, (cudaStream_t)stream, p), me);
 }
 
 L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *stream) {
@@ -653,10 +734,9 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
     if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->k_out) & mask) ||
         (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm | (uintptr_t)a->rope_table | (uintptr_t)a->pos | (uintptr_t)a->slot) & 3))
         return refuse(me, "a pointer is not aligned to its type");
-    const int kv_rows = (with_k ? a->n_kv_heads : 0) + (with_v ? a->n_kv_heads : 0), heads = a->n_heads + kv_rows;
-    if (!heads) return 0;
+    if (!a->n_heads && !with_k && !with_v) return 0;
     if (a->rope && ((uintptr_t)a->rope_table & 7)) return refuse(me, "rope_table must be 8-byte aligned");
-    QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, heads, 1, heads};
+    QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, 0, 0, 0, 1, 1};
     if (cache) p.c = kv4_dev(cache);
     // 16-byte accesses where every row of every tensor starts on 16 bytes.
     const int per16 = a->dtype == L3M_DT_F32 ? 4 : 8;
@@ -669,31 +749,33 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
     p.vec = !(at & 15) && ld % per16 == 0;
     const int rope = a->rope && a->rot_dim ? a->rope : 0;
     const int ng = (a->head_dim + kKvBlock - 1) / kKvBlock, lpr = ng == 1 ? 4 : ng == 2 ? 8 : ng <= 4 ? 16 : 32;
+    const int rpw = 32 / lpr;
+    p.q_groups = (a->n_heads + rpw - 1) / rpw;
+    p.k_groups = with_k ? (a->n_kv_heads + rpw - 1) / rpw : 0;
+    p.groups = p.q_groups + p.k_groups + (with_v ? (a->n_kv_heads + rpw - 1) / rpw : 0);
     // One warp per token takes all its rows when there are tokens enough to fill the GPU; else its rows are shared out.
-    const int sms = sm_count(), groups = (heads * lpr + 31) / 32;
-    const long long want = (32LL * sms + a->n_tokens - 1) / a->n_tokens;
-    p.chunks = (int)std::min<long long>(std::max(1LL, want), groups);
-    p.per_chunk = (groups + p.chunks - 1) / p.chunks * (32 / lpr);
-    p.chunks = (heads + p.per_chunk - 1) / p.per_chunk;
+    const int sms = sm_count();
+    const long long want = (24LL * sms + a->n_tokens - 1) / a->n_tokens;
+    p.chunks = (int)std::min<long long>(std::max(1LL, want), p.groups);
+    p.per_chunk = (p.groups + p.chunks - 1) / p.chunks;
+    p.chunks = (p.groups + p.per_chunk - 1) / p.per_chunk;
     const long long warps = (long long)a->n_tokens * p.chunks;
-    const int grid = (int)std::min<long long>(8LL * sms, (warps + kQkvThreads / 32 - 1) / (kQkvThreads / 32));
+    const int grid = (int)std::min<long long>(1 << 20, (warps + kQkvThreads / 32 - 1) / (kQkvThreads / 32));
     const cudaStream_t s = (cudaStream_t)stream;
     auto go = [&](auto t, auto r) {
         typedef decltype(t) T;
         constexpr int R = decltype(r)::value;
-        if (lpr == 4) qkv_kernel<T, 4, R><<<grid, kQkvThreads, 0, s>>>(p);
-        else if (lpr == 8) qkv_kernel<T, 8, R><<<grid, kQkvThreads, 0, s>>>(p);
-        else if (lpr == 16) qkv_kernel<T, 16, R><<<grid, kQkvThreads, 0, s>>>(p);
-        else qkv_kernel<T, 32, R><<<grid, kQkvThreads, 0, s>>>(p);
+        if (lpr == 4) return launch_early(qkv_kernel<T, 4, R>, grid, kQkvThreads, 0, s, p);
+        if (lpr == 8) return launch_early(qkv_kernel<T, 8, R>, grid, kQkvThreads, 0, s, p);
+        if (lpr == 16) return launch_early(qkv_kernel<T, 16, R>, grid, kQkvThreads, 0, s, p);
+        return launch_early(qkv_kernel<T, 32, R>, grid, kQkvThreads, 0, s, p);
     };
     auto by_rope = [&](auto t) {
-        if (rope == 0) go(t, std::integral_constant<int, 0>{});
-        else if (rope == 1) go(t, std::integral_constant<int, 1>{});
-        else go(t, std::integral_constant<int, 2>{});
+        if (rope == 0) return go(t, std::integral_constant<int, 0>{});
+        if (rope == 1) return go(t, std::integral_constant<int, 1>{});
+        return go(t, std::integral_constant<int, 2>{});
     };
-    if (a->dtype == L3M_DT_F32) by_rope(float{});
-    else by_rope(__nv_bfloat16{});
-    return launched(me);
+    return launched(a->dtype == L3M_DT_F32 ? by_rope(float{}) : by_rope(__nv_bfloat16{}), me);
 }
 
 L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, const int32_t *slots, int n, void *stream) {
@@ -704,12 +786,11 @@ L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, 
     if (n == 0 || (!k && !v)) return 0;
     if (!slots) return refuse(me, "slots are required");
     if (((uintptr_t)k | (uintptr_t)v) & (dtype == L3M_DT_F32 ? 3 : 1) || (uintptr_t)slots & 3) return refuse(me, "a pointer is not aligned to its type");
-    const LoadArgs p = {kv4_dev(cache), cache->dtype == L3M_DT_MXFP4, n, k, v, slots};
-    const long long items = (long long)n * cache->n_kv_heads * (cache->head_dim / 8) * 2;
-    const int grid = (int)std::min<long long>(16LL * sm_count(), (items + 255) / 256);
-    if (dtype == L3M_DT_F32) load_kernel<float><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    else load_kernel<__nv_bfloat16><<<grid, 256, 0, (cudaStream_t)stream>>>(p);
-    return launched(me);
+    const int parts = cache->head_dim / 8;
+    const LoadArgs p = {kv4_dev(cache), cache->dtype == L3M_DT_MXFP4, n, parts, !(((uintptr_t)k | (uintptr_t)v) & 15), (unsigned)(0xffffffffu / parts + 1), k, v, slots};
+    const int grid = (n + 7) / 8;
+    const cudaStream_t s = (cudaStream_t)stream;
+    return launched(dtype == L3M_DT_F32 ? launch_early(load_kernel<float>, grid, 256, 0, s, p) : launch_early(load_kernel<__nv_bfloat16>, grid, 256, 0, s, p), me);
 }
 
 }  // extern "C"
