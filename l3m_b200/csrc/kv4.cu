@@ -36,28 +36,28 @@ struct PlanArgs {
     l3m_kv4_plan a;
 };
 
-// Inclusive sum over the block; `total` gets the block's sum. ws: one value per warp, reused.
-__device__ long long block_scan(long long v, long long *ws, long long *total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+struct Sums { long long gone, rows, pages; };          // pages returned, rows of q, pages wanted
+
+__device__ __forceinline__ Sums add(const Sums &a, const Sums &b) { return {a.gone + b.gone, a.rows + b.rows, a.pages + b.pages}; }
+
+// Inclusive sums over the block; `total` gets the block's. ws: one entry per warp, free again when this returns.
+__device__ Sums block_scan(Sums v, Sums *ws, Sums *total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+#pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long u = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += u;
+        const Sums u = {__shfl_up_sync(0xffffffffu, v.gone, o), __shfl_up_sync(0xffffffffu, v.rows, o), __shfl_up_sync(0xffffffffu, v.pages, o)};
+        if (lane >= o) v = add(v, u);
     }
     if (lane == 31) ws[warp] = v;
     __syncthreads();
-    if (warp == 0) {
-        long long s = ws[lane];
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long u = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += u;
-        }
-        ws[lane] = s;
+    Sums all = {0, 0, 0}, before = {0, 0, 0};
+    for (int k = 0; k < warps; k++) {
+        if (k == warp) before = all;
+        all = add(all, ws[k]);
     }
+    *total = all;
     __syncthreads();
-    if (warp) v += ws[warp - 1];
-    *total = ws[31];
-    __syncthreads();
-    return v;
+    return add(v, before);
 }
 
 // The last index i of sorted a[0..n) with a[i] <= x (a[0] <= x is the caller's promise).
@@ -71,18 +71,22 @@ __device__ int last_not_above(const int *a, int n, int x) {
     return lo;
 }
 
+__device__ __forceinline__ bool bad_lengths(const l3m_kv4_plan &a, long long kv, long long count) {
+    return kv < 0 || (kv + count + a.page - 1) / a.page > a.max_blocks || kv + count > 0x7fffffff;
+}
+
 // Every CTA sums the requests' lengths for itself (a few microseconds at most: they fit one SM's
 // shared memory), so the CTAs need nothing from each other; then they share out the rows of slot and
 // pos, the new table entries and the returned pages. A page that comes off the stack above its old
 // top is one that an ended request returns in this call: it is read from that request's table row,
 // which nobody writes, not from the stack, which another CTA may still be writing.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
+__global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constant__ PlanArgs p) {
     const l3m_kv4_plan &a = p.a;
     extern __shared__ int sh[];
     const int n = a.n_req;
     int *gone = sh, *used = sh + (n + 1), *start = sh + 2 * (n + 1);      // exclusive sums: pages returned, pages taken, rows
     uint8_t *ok = (uint8_t *)(sh + 3 * (n + 1));
-    __shared__ long long ws[32];
+    __shared__ Sums ws[32];
     __shared__ int left_s;
     const int tid = threadIdx.x;
     int status = 0;
@@ -92,70 +96,55 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
     const int old_top = min(max(free0, 0), a.n_pages);
     if (free0 != old_top) status |= L3M_KV4_BAD_LENGTH;
 
-    // Pass 1: what ended requests return.
-    long long base = 0;
-    for (int c = 0; c < n; c += kPlanThreads) {
+    // Running sums over the requests of what ended ones return and of what the others bring and want.
+    Sums base = {0, 0, 0};
+    for (int c = 0; c < n; c += blockDim.x) {
         const int r = c + tid;
-        long long give = 0;
+        Sums v = {0, 0, 0}, sum;
         if (r < n) {
-            const long long kv = a.kv_len[r];
-            const long long held = (kv + a.page - 1) / a.page;
-            if (a.new_len[r] < 0 && kv >= 0 && held <= a.max_blocks) give = held;
+            const long long kv = a.kv_len[r], fresh = a.new_len[r], count = fresh > 0 ? fresh : 0;
+            const long long held = (kv + a.page - 1) / a.page, after = (kv + count + a.page - 1) / a.page;
+            if (fresh < 0 && kv >= 0 && held <= a.max_blocks) v.gone = held;
+            v.rows = count;
+            if (!bad_lengths(a, kv, count)) v.pages = after - held;
         }
-        long long sum;
-        const long long upto = block_scan(give, ws, &sum);
-        if (r < n) gone[r] = (int)min(base + upto - give, (long long)a.n_pages);
-        base += sum;
+        const Sums upto = add(base, block_scan(v, ws, &sum));
+        if (r < n) {
+            gone[r] = (int)min(upto.gone - v.gone, (long long)a.n_pages);
+            start[r] = (int)min(upto.rows - v.rows, 0x7fffffffLL);
+            used[r] = (int)min(upto.pages - v.pages, 0x7fffffffLL);
+        }
+        base = add(base, sum);
     }
-    if (base > a.n_pages - old_top) {                                     // more pages than the pool has: the excess is dropped
+    if (base.gone > a.n_pages - old_top) {                                // more pages than the pool has: the excess is dropped
         status |= L3M_KV4_BAD_LENGTH;
-        base = a.n_pages - old_top;
+        base.gone = a.n_pages - old_top;
     }
-    const int n_gone = (int)base, top = old_top + n_gone;
+    const int n_gone = (int)base.gone, top = old_top + n_gone;
     if (tid == 0) {
         gone[n] = n_gone;
+        start[n] = (int)min(base.rows, 0x7fffffffLL);
+        used[n] = (int)min(base.pages, 0x7fffffffLL);
         left_s = top;
-    }
-
-    // Pass 2: what the others take.
-    long long rows = 0, pages = 0;
-    for (int c = 0; c < n; c += kPlanThreads) {
-        const int r = c + tid;
-        long long count = 0, need = 0, kv = 0;
-        int bad = 0, ended = 0;
-        if (r < n) {
-            kv = a.kv_len[r];
-            ended = a.new_len[r] < 0;
-            count = max(a.new_len[r], 0);
-            const long long held = (kv + a.page - 1) / a.page, after = (kv + count + a.page - 1) / a.page;
-            bad = kv < 0 || after > a.max_blocks || kv + count > 0x7fffffff;
-            if (!bad) need = after - held;
-        }
-        long long sum;
-        const long long rows_upto = block_scan(count, ws, &sum) + rows;
-        rows += sum;
-        const long long pages_upto = block_scan(need, ws, &sum) + pages;
-        pages += sum;
-        if (r < n) {
-            const bool pages_ok = need == 0 || pages_upto <= top, rows_ok = rows_upto <= a.max_tokens;
-            const bool served = !bad && !ended && pages_ok && rows_ok;
-            if (bad) status |= L3M_KV4_BAD_LENGTH;
-            if (!pages_ok) status |= L3M_KV4_NO_PAGES;
-            if (count && !rows_ok) status |= L3M_KV4_NO_ROOM;
-            used[r] = (int)min(pages_upto - need, 0x7fffffffLL);
-            start[r] = (int)min(rows_upto - count, 0x7fffffffLL);
-            ok[r] = served;
-            if (blockIdx.x == 0) {
-                a.q_start[r + 1] = (int)min(rows_upto, 0x7fffffffLL);
-                a.kv_total[r] = served ? (int)(kv + count) : 0;
-            }
-            if (served && need) atomicMin(&left_s, (int)(top - pages_upto));
-        }
-    }
-    if (tid == 0) {
-        used[n] = (int)min(pages, 0x7fffffffLL);
-        start[n] = (int)min(rows, 0x7fffffffLL);
         if (blockIdx.x == 0) a.q_start[0] = 0;
+    }
+    __syncthreads();
+    for (int r = tid; r < n; r += blockDim.x) {
+        const long long kv = a.kv_len[r], fresh = a.new_len[r], count = fresh > 0 ? fresh : 0;
+        const bool bad = bad_lengths(a, kv, count);
+        const int pages_upto = used[r + 1], rows_upto = start[r + 1];
+        const long long need = bad ? 0 : (kv + count + a.page - 1) / a.page - (kv + a.page - 1) / a.page;
+        const bool pages_ok = need == 0 || pages_upto <= top, rows_ok = rows_upto <= a.max_tokens;
+        const bool served = !bad && fresh >= 0 && pages_ok && rows_ok;
+        if (bad) status |= L3M_KV4_BAD_LENGTH;
+        if (!pages_ok) status |= L3M_KV4_NO_PAGES;
+        if (count && !rows_ok) status |= L3M_KV4_NO_ROOM;
+        ok[r] = served;
+        if (blockIdx.x == 0) {
+            a.q_start[r + 1] = rows_upto;
+            a.kv_total[r] = served ? (int)(kv + count) : 0;
+        }
+        if (served && need) atomicMin(&left_s, top - pages_upto);
     }
     __syncthreads();
     if (blockIdx.x == 0) {
@@ -163,7 +152,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const PlanArgs p) {
         if (status && a.status) atomicOr((int *)a.status, status);
     }
     const int taken = top - left_s;
-    const int step = gridDim.x * kPlanThreads, first = blockIdx.x * kPlanThreads + tid;
+    const int step = gridDim.x * blockDim.x, first = blockIdx.x * blockDim.x + tid;
     auto returned = [&](int i) {                                          // the i-th returned page
         const int r = last_not_above(gone, n, i);
         return a.tables[(size_t)r * a.max_blocks + (i - gone[r])];
@@ -204,12 +193,12 @@ constexpr int kQkvThreads = 256;
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// 8 values at p as they lie in memory: one or two 16-byte accesses where every row starts 16-byte aligned (vec), else one by one.
+// 8 values at p as they lie in memory: one or two 16-byte accesses where every row starts 16-byte aligned (VEC), else one by one.
 template <typename T> struct Raw8;
 template <> struct Raw8<float> {
     float4 a, b;
-    __device__ __forceinline__ void load(const float *p, bool vec) {
-        if (vec) {
+    template <bool VEC> __device__ __forceinline__ void load(const float *p) {
+        if (VEC) {
             a = ((const float4 *)p)[0];
             b = ((const float4 *)p)[1];
         } else {
@@ -225,8 +214,8 @@ template <> struct Raw8<float> {
 };
 template <> struct Raw8<__nv_bfloat16> {
     uint32_t w[4];
-    __device__ __forceinline__ void load(const __nv_bfloat16 *p, bool vec) {
-        if (vec) {
+    template <bool VEC> __device__ __forceinline__ void load(const __nv_bfloat16 *p) {
+        if (VEC) {
             const uint4 v = *(const uint4 *)p;
             w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
         } else {
@@ -244,8 +233,8 @@ template <> struct Raw8<__nv_bfloat16> {
         }
     }
 };
-__device__ __forceinline__ void store8(float *p, const float *x, float f, bool vec) {
-    if (vec) {
+template <bool VEC> __device__ __forceinline__ void store8(float *p, const float *x, float f) {
+    if (VEC) {
         ((float4 *)p)[0] = make_float4(x[0] * f, x[1] * f, x[2] * f, x[3] * f);
         ((float4 *)p)[1] = make_float4(x[4] * f, x[5] * f, x[6] * f, x[7] * f);
     } else {
@@ -253,8 +242,8 @@ __device__ __forceinline__ void store8(float *p, const float *x, float f, bool v
         for (int e = 0; e < 8; e++) p[e] = x[e] * f;
     }
 }
-__device__ __forceinline__ void store8(__nv_bfloat16 *p, const float *x, float f, bool vec) {
-    if (vec) {
+template <bool VEC> __device__ __forceinline__ void store8(__nv_bfloat16 *p, const float *x, float f) {
+    if (VEC) {
         __nv_bfloat162 h[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) h[e] = __floats2bfloat162_rn(x[2 * e] * f, x[2 * e + 1] * f);
@@ -268,7 +257,7 @@ __device__ __forceinline__ void store8(__nv_bfloat16 *p, const float *x, float f
 struct QkvArgs {
     l3m_qkv a;
     Kv4Dev c;
-    int store, mx, vec;
+    int store, mx;
     int q_groups, k_groups, groups;       // a token's row groups (one warp's rows at a time): queries, keys, all
     int chunks, per_chunk;                // warps per token and the groups each takes
 };
@@ -278,71 +267,16 @@ __device__ __forceinline__ double finite(double x) { return x != x ? 0.0 : fmin(
 // What a lane stores of its row: the codes of its 8 values and its block's scale bits.
 struct Held { unsigned codes, scale; };
 
-// The definition, in 64 bits, read again from memory: for the rows whose 32-bit values lie too near a border.
-// Every lane of the warp takes part (lanes without a row with src null).
-template <typename T, int LPR, int ROPE>
-__device__ __noinline__ Held exact_row(const T *src, const float *w, const float *turn, int D, int rot, float eps, int mx) {
-    const int lane = threadIdx.x & (LPR - 1), d0 = lane * 8, half = rot / 2;
-    const bool mine = src && d0 < D;
-    double u[8], ss = 0.0, f = 1.0;
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const int d = d0 + e;
-        double x = mine ? (double)to_f32(src[d]) : 0.0;
-        if (w) ss += x * x;
-        if (mine && w) x *= (double)w[d];
-        u[e] = x;
-        if (ROPE && mine && turn && d < rot) {
-            const int md = ROPE == 1 ? d ^ 1 : d < half ? d + half : d - half, i = ROPE == 1 ? d >> 1 : d < half ? d : d - half;
-            const bool second = ROPE == 1 ? (d & 1) != 0 : d >= half;
-            double m = (double)to_f32(src[md]);
-            if (w) m *= (double)w[md];
-            const double c = (double)turn[2 * i], s = (double)turn[2 * i + 1];
-            u[e] = second ? m * s + x * c : x * c - m * s;
-        }
-        u[e] = finite(u[e]);
-    }
-    for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (w) f = finite(1.0 / sqrt(ss / D + (double)eps));
-    double top = 0.0;
-    int at = 0;
-#pragma unroll
-    for (int e = 0; e < 8; e++)
-        if (fabs(u[e]) > fabs(top)) {
-            top = u[e];
-            at = e;
-        }
-    at += (lane & 3) * 8;
-    for (int o = 1; o < 4; o <<= 1) {                                       // the first of equals over the block's 4 lanes
-        const double ot = __shfl_xor_sync(0xffffffffu, top, o);
-        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
-        if (fabs(ot) > fabs(top) || (fabs(ot) == fabs(top) && oa < at)) {
-            top = ot;
-            at = oa;
-        }
-    }
-    Held r = {0, 0};
-    if (!mx) {
-        const double d = top / -8.0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const double q = d != 0.0 ? floor(u[e] / d + 8.5) : 8.0;
-            r.codes |= (unsigned)(int)fmin(fmax(q, 0.0), 15.0) << (4 * e);
-        }
-        r.scale = top != 0.0 ? __half_as_ushort(__float2half_rn(fminf(fmaxf((float)(d * f), -65504.0f), 65504.0f))) : 0;
-    } else {
-        const double m = fabs(top * f);
-        const int e8 = m > 0.0 ? min(max(ilogb(m) + 125, 0), 254) : 0;
-        const double inv = ldexp(1.0, 127 - e8);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const double y = u[e] * f, v = fabs(y) * inv;
-            const unsigned mag = (v > 0.25) + (v > 0.75) + (v > 1.25) + (v > 1.75) + (v > 2.5) + (v > 3.5) + (v > 5.0);
-            r.codes |= (mag | (y < 0.0 && mag ? 8u : 0u)) << (4 * e);
-        }
-        r.scale = (unsigned)e8;
-    }
-    return r;
+// Two values as e2m1, rounded to nearest (ties to even), at most 6: the first in the low nibble.
+__device__ __forceinline__ unsigned e2m1_codes(float lo, float hi) {
+    uint32_t d;
+    asm("{ .reg .b8 c, z;\n .reg .b16 w;\n mov.b16 w, 0;\n mov.b16 {z, z}, w;\n cvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n mov.b32 %0, {c, z, z, z}; }" : "=r"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+// Codes of -0 made 0.
+__device__ __forceinline__ unsigned no_minus_zero(unsigned w) {
+    const unsigned m = w & 0x77777777u, some = (m | m >> 1 | m >> 2) & 0x11111111u;
+    return m | (w & some << 3);
 }
 
 // A row (a head of a token) is held by LPR lanes, 8 contiguous dims each, so 4 lanes hold a block; a group of 32 / LPR rows
@@ -353,21 +287,128 @@ __device__ __noinline__ Held exact_row(const T *src, const float *w, const float
 // on either side of it in 32 bits. So u (the normed, rotated value before the row's factor, which
 // q4_0's codes do not depend on) is computed in 32 bits with a bound on its error, each decision with its
 // distance from the border, and where the distance is within the bound the row is redone in 64 bits (about 1% of the rows).
-// q4_0's test is exact for exact u: code >= b iff (b - 8.5) / 8 * |top| + u * sign(top) <= 0, one fma whose sign cannot
-// be rounded away; so values, which are neither normed nor rotated, never need 64 bits for it.
 enum { kQuery, kKey, kValue };
 
-template <typename T, int LPR, int ROPE>
+// Where a token's rows go: its tile of head 0 (null: nowhere) and its row there.
+struct Place {
+    uint8_t *tile;
+    int tr;
+};
+
+// One lane's share of a row of head h: t of block j.
+template <int KIND> __device__ __forceinline__ void put_row(const QkvArgs &p, const Place &to, int h, int lane, const Held &held) {
+    const int j = lane >> 2, t = lane & 3, ng = p.c.ng;
+    uint8_t *at = to.tile + (size_t)h * p.c.tiles * p.c.tile_bytes;
+    if (KIND == kKey) {
+        *(uint32_t *)(at + to.tr * 16 * ng + (t * ng + j) * 4) = held.codes;
+    } else {
+        uint16_t *v = (uint16_t *)(at + 256 * ng + to.tr * 16 * ng);
+        v[2 * t * ng + j] = (uint16_t)held.codes;
+        v[(2 * t + 1) * ng + j] = (uint16_t)(held.codes >> 16);
+    }
+    if (t == 0) {
+        uint8_t *s = at + (KIND == kKey ? p.c.k_scales() : p.c.v_scales()) + (to.tr * ng + j) * p.c.sb;
+        if (p.mx) *s = (uint8_t)held.scale;
+        else *(uint16_t *)s = (uint16_t)held.scale;
+    }
+}
+
+// Group g by the definition, in 64 bits: for rows whose 32-bit values lie too near a border.
+template <typename T, int LPR, int ROPE, int KIND>
+__device__ __noinline__ void exact_rows(const QkvArgs &p, int tok, Place to, const float *turn, int g) {
+    const l3m_qkv &a = p.a;
+    const int wl = threadIdx.x & 31, lane = wl & (LPR - 1), d0 = lane * 8, h = g * (32 / LPR) + wl / LPR, D = a.head_dim;
+    const int rot = KIND == kKey && ROPE ? a.rot_dim : 0, half = rot / 2;
+    const bool live = h < a.n_kv_heads, mine = live && d0 < D;
+    const T *src = (const T *)(KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kKey ? a.k_ld : a.v_ld) + (size_t)h * D;
+    const float *w = KIND == kKey ? a.k_norm : nullptr;
+    double u[8], ss = 0.0, f = 1.0;
+#pragma unroll 1
+    for (int e = 0; e < 8; e++) {
+        const int d = d0 + e;
+        double x = mine ? (double)to_f32(src[d]) : 0.0;
+        if (w) ss += x * x;
+        if (mine && w) x *= (double)w[d];
+        if (mine && d < rot) {
+            const int md = ROPE == 1 ? d ^ 1 : d < half ? d + half : d - half, i = ROPE == 1 ? d >> 1 : d < half ? d : d - half;
+            const bool second = ROPE == 1 ? (d & 1) != 0 : d >= half;
+            double m = (double)to_f32(src[md]);
+            if (w) m *= (double)w[md];
+            const double c = (double)turn[2 * i], s = (double)turn[2 * i + 1];
+            x = second ? m * s + x * c : x * c - m * s;
+        }
+        u[e] = x;
+    }
+    for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+    if (w) f = 1.0 / sqrt(ss / D + (double)a.eps);
+    __syncwarp();                                                        // in place: every lane has read its row
+    if (KIND == kKey && a.k_out && mine) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = (float)(u[e] * f);
+        store8<false>((T *)a.k_out + (size_t)tok * a.k_out_ld + (size_t)h * D + d0, x, 1.0f);
+    }
+    f = finite(f);
+    double top = 0.0;
+    int at = 0;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        u[e] = finite(u[e]);
+        if (fabs(u[e]) > fabs(top)) {
+            top = u[e];
+            at = e;
+        }
+    }
+    at += (lane & 3) * 8;
+    for (int o = 1; o < 4; o <<= 1) {                                   // the first of equals over the block's 4 lanes
+        const double ot = __shfl_xor_sync(0xffffffffu, top, o);
+        const int oa = __shfl_xor_sync(0xffffffffu, at, o);
+        if (fabs(ot) > fabs(top) || (fabs(ot) == fabs(top) && oa < at)) {
+            top = ot;
+            at = oa;
+        }
+    }
+    Held held = {0, 0};
+    const double mag = fabs(top);
+    if (!p.mx) {
+        // As in quantise(), a candidate and the sign of its fma; within the rounding of the definition's own quotient, that quotient
+        const double d = top / -8.0, inv = mag > 0.0 ? 1.0 / d : 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double b = rint(fma(u[e], inv, 8.5)), r = fma(fma(b, 0.125, -1.0625), mag, top < 0.0 ? -u[e] : u[e]);
+            int code = (int)b - (r <= 0.0 ? 0 : 1);
+            if (fabs(r) <= 1e-14 * mag) code = (int)floor(u[e] / d + 8.5);
+            held.codes |= (unsigned)min(max(code, 0), 15) << (4 * e);
+        }
+        held.scale = __half_as_ushort(__float2half_rn(fminf(fmaxf((float)(d * f), -65504.0f), 65504.0f)));
+        if (mag == 0.0) held = {0x88888888u, 0};
+    } else {
+        const double m = mag * f;
+        const int e8 = m > 0.0 ? min(max(ilogb(m) + 125, 0), 254) : 0;
+        const double inv = ldexp(1.0, 127 - e8);
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const double y = u[e] * f, v = fabs(y) * inv;
+            const unsigned code = (v > 0.25) + (v > 0.75) + (v > 1.25) + (v > 1.75) + (v > 2.5) + (v > 3.5) + (v > 5.0);
+            held.codes |= (code | (y < 0.0 && code ? 8u : 0u)) << (4 * e);
+        }
+        held.scale = (unsigned)e8;
+    }
+    if (live && lane < 4 * p.c.ng) put_row<KIND>(p, to, h, lane, held);
+}
+
+template <typename T, int LPR, int ROPE, bool VEC>
 struct RowWorker {
     static constexpr int RPW = 32 / LPR;
+    static constexpr bool FEW = sizeof(T) == 2;                              // 8 significant bits a value
     const QkvArgs &p;
     float *mate_buf;
-    int wl, lane, sub, d0, half, tok, tr;
+    int wl, lane, sub, d0, half, tok;
     bool in, partial;
     int shift, mate_lane;
     float cs[8], sn[8];                   // cos and sin of this lane's dims, sin with the sign of the mate's term
     const float *turn;
-    uint8_t *tile;
+    Place to;
 
     __device__ __forceinline__ RowWorker(const QkvArgs &args, float *buf) : p(args), mate_buf(buf) {
         wl = threadIdx.x & 31;
@@ -398,32 +439,31 @@ struct RowWorker {
         }
     }
 
-    // Groups [g0, g1) of a kind.
-    template <int KIND> __device__ __forceinline__ void rows(int g0, int g1) {
+    // Groups [g0, g1) of a kind, 64 at most. Returns which of them are left for exact_rows(): nothing of those is written.
+    template <int KIND> __device__ __forceinline__ unsigned long long rows(int g0, int g1) {
         const l3m_qkv &a = p.a;
-        const int heads = KIND == kQuery ? a.n_heads : a.n_kv_heads;
-        const T *src = (const T *)(KIND == kQuery ? a.q : KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kQuery ? a.q_ld : KIND == kKey ? a.k_ld : a.v_ld) + d0;
+        const int heads = KIND == kQuery ? a.n_heads : a.n_kv_heads, D = a.head_dim, step = RPW * D;
+        int h = g0 * RPW + sub;
+        const T *src = (const T *)(KIND == kQuery ? a.q : KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kQuery ? a.q_ld : KIND == kKey ? a.k_ld : a.v_ld) + (size_t)h * D + d0;
+        T *out = KIND == kValue ? nullptr : (T *)(KIND == kQuery ? a.q_out : a.k_out);
+        if (out) out += (size_t)tok * (KIND == kQuery ? a.q_out_ld : a.k_out_ld) + (size_t)h * D + d0;
         const float *w = KIND == kQuery ? a.q_norm : KIND == kKey ? a.k_norm : nullptr;
         float wt[8];
-        if (KIND != kValue && w && in) {
+        if (KIND != kValue && w) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) wt[e] = w[d0 + e];
+            for (int e = 0; e < 8; e++) wt[e] = in ? w[d0 + e] : 0.0f;
         }
-        const int D = a.head_dim;
-        const float inv_d = 1.0f / (float)D;
+        const float inv_d = __fdividef(1.0f, (float)D);
+        unsigned long long left = 0;
         Raw8<T> next;
-        auto fetch = [&](int g) {
-            const int h = g * RPW + sub;
-            if (g < g1 && h < heads && in) next.load(src + (size_t)h * D, p.vec);
-            else next.zero();
-        };
-        fetch(g0);
-        for (int g = g0; g < g1; g++) {
-            const int h = g * RPW + sub;
+        next.zero();
+        if (h < heads && in) next.template load<VEC>(src);
+        for (int g = g0; g < g1; g++, h += RPW) {
             const bool live = h < heads;
             float u[8];
             next.get(u);
-            fetch(g + 1);
+            src += step;
+            if (g + 1 < g1 && h + RPW < heads && in) next.template load<VEC>(src);
             float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value
             if (KIND != kValue && w) {
                 float ss = 0.0f;
@@ -433,7 +473,7 @@ struct RowWorker {
                 for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 f = rsqrtf(fmaf(ss, inv_d, a.eps));
 #pragma unroll
-                for (int e = 0; e < 8; e++) u[e] = in ? u[e] * wt[e] : 0.0f;
+                for (int e = 0; e < 8; e++) u[e] *= wt[e];
             }
             if (KIND != kValue && ROPE) {
                 float m[8];
@@ -455,27 +495,40 @@ struct RowWorker {
                         m[e] = d < half ? row[d + half] : d < 2 * half ? row[d - half] : 0.0f;
                     }
                 }
+                if (partial) {                                               // dims behind rot_dim: no mate, whatever it holds
+#pragma unroll
+                    for (int e = 0; e < 8; e++) m[e] = d0 + e < a.rot_dim ? m[e] : 0.0f;
+                }
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
                     if (KIND == kKey) size = fmaxf(size, fabsf(u[e]) + fabsf(m[e]));
-                    const float r = fmaf(m[e], sn[e], u[e] * cs[e]);
-                    u[e] = partial && d0 + e >= a.rot_dim ? u[e] : r;
+                    u[e] = fmaf(m[e], sn[e], u[e] * cs[e]);
                 }
             }
             Held held = {0, 0};
-            if (KIND != kQuery && tile) held = KIND == kKey ? quantise<KIND>(u, size, f, w, src + (size_t)h * D - d0, live) : quantise<KIND>(u, 0.0f, 1.0f, nullptr, src + (size_t)h * D - d0, live);
-            if (KIND != kValue) {
-                T *out = (T *)(KIND == kQuery ? a.q_out : a.k_out);
-                if (out) {
-                    __syncwarp();                                            // in place: every lane has read its row
-                    if (live && in) store8(out + (size_t)tok * (KIND == kQuery ? a.q_out_ld : a.k_out_ld) + (size_t)h * D + d0, u, f, p.vec);
+            if (KIND != kQuery && to.tile) {
+                bool near;
+                held = quantise<KIND>(u, size, f, w, &near);
+                if (__any_sync(0xffffffffu, near && live)) {
+                    left |= 1ull << (g - g0);
+                    if (KIND == kKey && out) out += step;
+                    continue;
                 }
             }
-            if (KIND != kQuery && tile && live && lane < 4 * p.c.ng) put<KIND>(h, held);
+            if (KIND != kValue && out) {
+                __syncwarp();                                                // in place: every lane has read its row
+                if (live && in) store8<VEC>(out, u, f);
+                out += step;
+            }
+            if (KIND != kQuery && to.tile && live && lane < 4 * p.c.ng) put_row<KIND>(p, to, h, lane, held);
         }
+        return left;
     }
 
-    template <int KIND> __device__ __forceinline__ Held quantise(const float *u, float size, float f, const float *w, const T *src, bool live) const {
+    // A row's codes and scales; *close: some decision lies within the error's bound of its border. Each code is that of the value moved down
+    // by the bound and that of the value moved up: where they agree they are right. Values of 8 bits that no
+    // arithmetic has touched lie on a border or 2^-9 from it: a smaller move makes ties go as they should.
+    template <int KIND> __device__ __forceinline__ Held quantise(const float *u, float size, float f, const float *w, bool *close) const {
         // The block's extremes; zero keeps a sum of zeros, anything not finite spoils it.
         float hi = u[0], lo = u[0], zero = 0.0f;
 #pragma unroll
@@ -497,22 +550,30 @@ struct RowWorker {
         bool again = !(zero == 0.0f) || (mag < 0x1p-100f && (mag > 0.0f || err > 0.0f)) || mag > 0x1p120f;
         Held held = {0, 0};
         if (!p.mx) {
-            // opposite signs of one size: the sign of the first decides
-            again |= mag > 0.0f && fabsf(hi + lo) <= 2.0f * err;
-            const float top = hi >= -lo ? hi : lo, inv = __fdividef(-8.0f, top), sgn = hi >= -lo ? 1.0f : -1.0f;
-            const float tol = exact ? -1.0f : 3.0f * err + mag * 0x1p-22f;
-            float near = FLT_MAX;
+            float top = hi >= -lo ? hi : lo;
+            bool even = mag > 0.0f && fabsf(hi + lo) <= 2.0f * err;          // opposite signs of one size: the sign of the first decides
+            if (exact && __any_sync(0xffffffffu, even)) {
+                int first = 1 << 20;
+#pragma unroll
+                for (int e = 7; e >= 0; e--) first = fabsf(u[e]) == mag ? (lane & 3) * 16 + 2 * e + (u[e] < 0.0f) : first;
+                first = min(first, __shfl_xor_sync(0xffffffffu, first, 1));
+                first = min(first, __shfl_xor_sync(0xffffffffu, first, 2));
+                top = even ? (first & 1 ? -mag : mag) : top;
+                even = false;
+            }
+            again |= even;
+            // code = the integer part of t = u / d + 8.5, 15 at most; rounded down into the low bits of t + 3 * 2^22
+            const float inv = __fdividef(-8.0f, top), per = __fdividef(16.5f * err, mag), tau = exact && FEW ? 0x1p-12f : per + 0x1p-18f;
+            unsigned down = 0, up = 0;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                // The candidate border next to t = u / d + 8.5, as an integer in the low bits of b; r: on which side u lies, and how far
-                const float b = fmaf(u[e], inv, 8.5f) + 12582912.0f, k = b - 12582912.0f;
-                const float r = fmaf(fmaf(k, 0.125f, -1.0625f), mag, u[e] * sgn);
-                near = fminf(near, fabsf(r));
-                int code = (int)__float_as_uint(b) - 0x4b400000 - (r <= 0.0f ? 0 : 1);
-                code = min(max(code, 0), 15);
-                held.codes |= (unsigned)code << (4 * e);
+                const float t = fmaf(u[e], inv, 8.5f);
+                up += __float_as_uint(__fadd_rd(fminf(t + tau, 15.5f), 12582912.0f)) << (4 * e);
+                if (!(exact && FEW)) down += __float_as_uint(__fadd_rd(fminf(t - tau, 15.5f), 12582912.0f)) << (4 * e);
             }
-            again |= near <= tol;
+            constexpr unsigned kBase = 0x4b400000u * 0x11111111u;            // the sum of the numbers' other bits
+            held.codes = up - kBase;
+            if (!(exact && FEW)) again |= up != down;
             const float s = top * -0.125f * f;
             if (exact) {
                 held.scale = __half_as_ushort(__float2half_rn(fminf(fmaxf(s, -65504.0f), 65504.0f)));
@@ -523,57 +584,41 @@ struct RowWorker {
                 held.scale = s0;
                 again |= s0 != s1;
             }
-            if (mag == 0.0f) held = {0x88888888u, 0};
+            if (mag == 0.0f) {
+                held = {0x88888888u, 0};
+                again = !(zero == 0.0f) || err > 0.0f;
+            }
         } else {
             const float m = mag * f, rel = exact ? 0.0f : 0x1p-20f + __fdividef(2.0f * err, mag);
             const unsigned e0 = __float_as_uint(m * (1.0f - rel)) >> 23, e1 = __float_as_uint(m * (1.0f + rel)) >> 23;
             again |= mag > 0.0f && (e0 != e1 || e0 < 20u || e0 > 250u || f > 0x1p17f);   // far from either end, fi below is a normal number
             const float inv = mag > 0.0f ? __uint_as_float((256u - e0) << 23) : 0.0f;   // 2^(127 - e8), e8 = e0 - 2
-            const float fi = f * inv, tol = exact ? -1.0f : (3.0f * err + mag * 0x1p-20f) * fi * 2.0f;
-            float near = FLT_MAX;
+            const float fi = f * inv, tau = exact ? 0.0f : (3.0f * err + mag * 0x1p-20f) * fi;
+            // Rounded to nearest; ties go down because the number has been moved towards zero.
+            unsigned down = 0, up = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = fabsf(u[e]) * fi;                             // in [0, 8): the steps are 1/2 below 2, 1 below 4, 2 above
-                const float r = fmaf(v, v < 2.0f ? 2.0f : v < 4.0f ? 1.0f : 0.5f, -0.5f), c = ceilf(r);
-                near = fminf(near, fabsf(r - rintf(r)));
-                const int code = min((int)c + (v < 2.0f ? 0 : v < 4.0f ? 2 : 4), 7);
-                held.codes |= (unsigned)(code | (u[e] < 0.0f && code ? 8 : 0)) << (4 * e);
+            for (int e = 0; e < 8; e += 2) {
+                const float a = u[e] * fi, b = u[e + 1] * fi;
+                const float ta = exact ? fabsf(a) * 0x1p-18f : tau, tb = exact ? fabsf(b) * 0x1p-18f : tau;
+                const float da = a < 0.0f ? a + ta : a - ta, db = b < 0.0f ? b + tb : b - tb;
+                down |= e2m1_codes(da, db) << (4 * e);
+                if (!(exact && FEW)) up |= e2m1_codes(a < 0.0f ? a - tau : a + tau, b < 0.0f ? b - tau : b + tau) << (4 * e);
             }
-            again |= near <= tol;
+            held.codes = no_minus_zero(down);
+            if (!(exact && FEW)) again |= held.codes != no_minus_zero(up);
             held.scale = mag > 0.0f ? e0 - 2 : 0;
+            if (mag == 0.0f) again = !(zero == 0.0f) || err > 0.0f;
         }
-        again &= live;
-        if (__any_sync(0xffffffffu, again)) {
-            const Held h64 = exact_row<T, LPR, ROPE>(live ? src : nullptr, w, KIND == kValue ? nullptr : turn, p.a.head_dim, KIND == kValue ? 0 : p.a.rot_dim, p.a.eps, p.mx);
-            const unsigned block = 0xfu << (wl & ~3);
-            if (__ballot_sync(0xffffffffu, again) & block) held = h64;
-        }
+        *close = again;
         return held;
-    }
-
-    template <int KIND> __device__ __forceinline__ void put(int h, const Held &held) const {
-        const int j = lane >> 2, t = lane & 3, ng = p.c.ng;
-        uint8_t *at = tile + (size_t)h * p.c.tiles * p.c.tile_bytes;
-        if (KIND == kKey) {
-            *(uint32_t *)(at + tr * 16 * ng + (t * ng + j) * 4) = held.codes;
-        } else {
-            uint16_t *v = (uint16_t *)(at + 256 * ng + tr * 16 * ng);
-            v[2 * t * ng + j] = (uint16_t)held.codes;
-            v[(2 * t + 1) * ng + j] = (uint16_t)(held.codes >> 16);
-        }
-        if (t == 0) {
-            uint8_t *s = at + (KIND == kKey ? p.c.k_scales() : p.c.v_scales()) + (tr * ng + j) * p.c.sb;
-            if (p.mx) *s = (uint8_t)held.scale;
-            else *(uint16_t *)s = (uint16_t)held.scale;
-        }
     }
 };
 
-template <typename T, int LPR, int ROPE>
-__global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const QkvArgs p) {
+template <typename T, int LPR, int ROPE, bool VEC>
+__global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const __grid_constant__ QkvArgs p) {
     const l3m_qkv &a = p.a;
     __shared__ float mate_buf[ROPE == 2 ? kQkvThreads * 8 : 1];
-    RowWorker<T, LPR, ROPE> w(p, mate_buf);
+    RowWorker<T, LPR, ROPE, VEC> w(p, mate_buf);
     asm volatile("griddepcontrol.wait;" ::: "memory");                      // what ran before on the stream is done and visible
     const long long items = (long long)a.n_tokens * p.chunks;
     for (long long item = blockIdx.x * (kQkvThreads / 32) + (threadIdx.x >> 5); item < items; item += (long long)gridDim.x * (kQkvThreads / 32)) {
@@ -585,22 +630,25 @@ __global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const QkvArgs p) {
             continue;
         }
         w.tok = tok;
-        w.tile = nullptr;
+        w.to.tile = nullptr;
+        w.to.tr = 0;
         if (p.store) {
             const int slot = a.slot[tok];
             if (slot >= p.c.n_pages * p.c.page) {
                 if (a.status && w.wl == 0) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
             } else if (slot >= 0) {
                 const int page = slot / p.c.page, off = slot - page * p.c.page;
-                w.tile = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
-                w.tr = off % kKvTile;
+                w.to.tile = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
+                w.to.tr = off % kKvTile;
             }
         }
         if (g0 < p.q_groups + p.k_groups) w.rotation(pos);
         if (g0 < p.q_groups) w.template rows<kQuery>(g0, min(g1, p.q_groups));
         const int k0 = p.q_groups, v0 = p.q_groups + p.k_groups;
-        if (g0 < v0 && g1 > k0) w.template rows<kKey>(max(g0 - k0, 0), min(g1, v0) - k0);
-        if (g1 > v0 && w.tile) w.template rows<kValue>(max(g0 - v0, 0), g1 - v0);
+        for (int g = max(g0 - k0, 0); g < min(g1, v0) - k0; g += 64)
+            for (unsigned long long left = w.template rows<kKey>(g, min(g + 64, min(g1, v0) - k0)); left; left &= left - 1) exact_rows<T, LPR, ROPE, kKey>(p, tok, w.to, w.turn, g + __ffsll(left) - 1);
+        for (int g = max(g0 - v0, 0); g < g1 - v0 && w.to.tile; g += 64)
+            for (unsigned long long left = w.template rows<kValue>(g, min(g + 64, g1 - v0)); left; left &= left - 1) exact_rows<T, LPR, ROPE, kValue>(p, tok, w.to, nullptr, g + __ffsll(left) - 1);
     }
 }
 
@@ -608,7 +656,7 @@ __global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const QkvArgs p) {
 
 struct LoadArgs {
     Kv4Dev c;
-    int mx, n, parts, vec;
+    int mx, n, parts, vec, warps;         // warps per row
     unsigned per_part;                    // 2^32 / parts, rounded up: i / parts = i * per_part >> 32 for the small i here
     void *k, *v;
     const int32_t *slots;
@@ -623,17 +671,18 @@ __device__ __forceinline__ float scale_value(const uint8_t *p, int mx) {
     return mx ? (*p ? __uint_as_float((uint32_t)*p << 23) : __uint_as_float(0x00400000u)) : __half2float(*(const __half *)p);
 }
 
-// One warp per row: the lanes go over its keys' and values' pieces of 8.
+// One warp, or several, per row: the lanes go over its keys' and values' pieces of 8.
 template <typename T>
-__global__ void __launch_bounds__(256) load_kernel(const LoadArgs p) {
+__global__ void __launch_bounds__(256) load_kernel(const __grid_constant__ LoadArgs p) {
     const int lane = threadIdx.x & 31, per = p.c.n_kv * p.parts, ng = p.c.ng;
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    for (long long row = blockIdx.x * 8LL + (threadIdx.x >> 5); row < p.n; row += gridDim.x * 8LL) {
+    const long long w0 = blockIdx.x * 8LL + (threadIdx.x >> 5), row = w0 / p.warps;
+    if (row < p.n) {
         const int slot = p.slots[row];
-        if (slot < 0 || slot >= p.c.n_pages * p.c.page) continue;
+        if (slot < 0 || slot >= p.c.n_pages * p.c.page) return;
         const int page = slot / p.c.page, off = slot - page * p.c.page, tr = off % kKvTile;
         const uint8_t *tile0 = p.c.data + p.c.tile_at(page, 0, off / kKvTile);
-        for (int i = lane; i < 2 * per; i += 32) {
+        for (int i = (int)(w0 - row * p.warps) * 32 + lane; i < 2 * per; i += 32 * p.warps) {
             const int is_v = i >= per, x = is_v ? i - per : i, head = p.parts == 1 ? x : (int)__umulhi((unsigned)x, p.per_part), c = x - head * p.parts, j = c >> 2, t = c & 3;
             T *out = (T *)(is_v ? p.v : p.k);
             if (!out) continue;
@@ -646,7 +695,9 @@ __global__ void __launch_bounds__(256) load_kernel(const LoadArgs p) {
             float x8[8];
 #pragma unroll
             for (int e = 0; e < 8; e++) x8[e] = code_value(w >> (4 * e) & 15, p.mx);
-            store8(out + ((size_t)row * p.c.n_kv + head) * p.c.dim + c * 8, x8, s, p.vec);
+            T *to = out + ((size_t)row * p.c.n_kv + head) * p.c.dim + c * 8;
+            if (p.vec) store8<true>(to, x8, s);
+            else store8<false>(to, x8, s);
         }
     }
 }
@@ -703,8 +754,9 @@ L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream) {
     const size_t smem = (size_t)3 * (a->n_req + 1) * 4 + a->n_req;
     const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
     if (e != cudaSuccess) return l3m_error_cuda(e, me);
-    const int grid = std::max(1, std::min(sm_count(), (a->max_tokens + kPlanThreads - 1) / kPlanThreads));
-    return launched(launch_early(plan_kernel, grid, kPlanThreads, smem, (cudaStream_t)stream, p), me);
+    const int threads = a->n_req <= 128 && a->max_tokens <= 2048 ? 128 : kPlanThreads;
+    const int grid = std::max(1, std::min(sm_count(), (a->max_tokens + threads - 1) / threads));
+    return launched(launch_early(plan_kernel, grid, threads, smem, (cudaStream_t)stream, p), me);
 }
 
 L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *stream) {
@@ -736,7 +788,7 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
         return refuse(me, "a pointer is not aligned to its type");
     if (!a->n_heads && !with_k && !with_v) return 0;
     if (a->rope && ((uintptr_t)a->rope_table & 7)) return refuse(me, "rope_table must be 8-byte aligned");
-    QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, 0, 0, 0, 1, 1};
+    QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, 0, 0, 1, 1};
     if (cache) p.c = kv4_dev(cache);
     // 16-byte accesses where every row of every tensor starts on 16 bytes.
     const int per16 = a->dtype == L3M_DT_F32 ? 4 : 8;
@@ -746,7 +798,7 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
     if (with_k) at |= (uintptr_t)a->k, ld |= a->k_ld;
     if (with_k && a->k_out) at |= (uintptr_t)a->k_out, ld |= a->k_out_ld;
     if (with_v) at |= (uintptr_t)a->v, ld |= a->v_ld;
-    p.vec = !(at & 15) && ld % per16 == 0;
+    const bool vec = !(at & 15) && ld % per16 == 0;
     const int rope = a->rope && a->rot_dim ? a->rope : 0;
     const int ng = (a->head_dim + kKvBlock - 1) / kKvBlock, lpr = ng == 1 ? 4 : ng == 2 ? 8 : ng <= 4 ? 16 : 32;
     const int rpw = 32 / lpr;
@@ -765,10 +817,14 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
     auto go = [&](auto t, auto r) {
         typedef decltype(t) T;
         constexpr int R = decltype(r)::value;
-        if (lpr == 4) return launch_early(qkv_kernel<T, 4, R>, grid, kQkvThreads, 0, s, p);
-        if (lpr == 8) return launch_early(qkv_kernel<T, 8, R>, grid, kQkvThreads, 0, s, p);
-        if (lpr == 16) return launch_early(qkv_kernel<T, 16, R>, grid, kQkvThreads, 0, s, p);
-        return launch_early(qkv_kernel<T, 32, R>, grid, kQkvThreads, 0, s, p);
+        auto run = [&](auto v) {
+            constexpr bool V = decltype(v)::value;
+            if (lpr == 4) return launch_early(qkv_kernel<T, 4, R, V>, grid, kQkvThreads, 0, s, p);
+            if (lpr == 8) return launch_early(qkv_kernel<T, 8, R, V>, grid, kQkvThreads, 0, s, p);
+            if (lpr == 16) return launch_early(qkv_kernel<T, 16, R, V>, grid, kQkvThreads, 0, s, p);
+            return launch_early(qkv_kernel<T, 32, R, V>, grid, kQkvThreads, 0, s, p);
+        };
+        return vec ? run(std::true_type{}) : run(std::false_type{});
     };
     auto by_rope = [&](auto t) {
         if (rope == 0) return go(t, std::integral_constant<int, 0>{});
@@ -786,9 +842,10 @@ L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, 
     if (n == 0 || (!k && !v)) return 0;
     if (!slots) return refuse(me, "slots are required");
     if (((uintptr_t)k | (uintptr_t)v) & (dtype == L3M_DT_F32 ? 3 : 1) || (uintptr_t)slots & 3) return refuse(me, "a pointer is not aligned to its type");
-    const int parts = cache->head_dim / 8;
-    const LoadArgs p = {kv4_dev(cache), cache->dtype == L3M_DT_MXFP4, n, parts, !(((uintptr_t)k | (uintptr_t)v) & 15), (unsigned)(0xffffffffu / parts + 1), k, v, slots};
-    const int grid = (n + 7) / 8;
+    const int parts = cache->head_dim / 8, turns = (2 * cache->n_kv_heads * parts + 31) / 32;
+    const int warps = (int)std::min<long long>(turns, std::max(1LL, (32LL * sm_count() + n - 1) / n));   // a row's turns shared out where rows are few
+    const LoadArgs p = {kv4_dev(cache), cache->dtype == L3M_DT_MXFP4, n, parts, !(((uintptr_t)k | (uintptr_t)v) & 15), warps, (unsigned)(0xffffffffu / parts + 1), k, v, slots};
+    const int grid = (int)(((long long)n * warps + 7) / 8);
     const cudaStream_t s = (cudaStream_t)stream;
     return launched(dtype == L3M_DT_F32 ? launch_early(load_kernel<float>, grid, 256, 0, s, p) : launch_early(load_kernel<__nv_bfloat16>, grid, 256, 0, s, p), me);
 }

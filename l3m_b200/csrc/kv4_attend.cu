@@ -779,7 +779,7 @@ __device__ long long block_sum_scan(long long v, long long *ws, long long *total
 }
 
 template <typename T, int MX, int NG, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(const AttendArgs p) {
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(const __grid_constant__ AttendArgs p) {
     typedef Worker<T, MX, NG, NT> W;
     extern __shared__ __align__(16) uint8_t smem[];
     W w(p, smem);
@@ -878,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
 constexpr int kJoinThreads = 512;
 
 template <typename T, int MX, int NG, int NT>
-__global__ void __launch_bounds__(kJoinThreads) join_kernel(const AttendArgs p, int rows) {
+__global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constant__ AttendArgs p, int rows) {
     typedef Worker<T, MX, NG, NT> W;
     constexpr int LD = W::DP + 4, SIZE = W::NR * LD, PER = W::DP / 4;
     __shared__ float4 sv[kJoinThreads];
