@@ -134,6 +134,7 @@ enum {
     L3M_KV4_NO_ROOM = 4,         // plan: more new tokens than max_tokens
     L3M_KV4_BAD_PAGE = 8,        // a page id or slot outside the cache was left out
     L3M_KV4_BAD_POS = 16,        // qkv: a position outside the rotation table; its row was left out
+    L3M_KV4_TIMEOUT = 32,        // attend: a wait inside the kernel gave up; the rows concerned are NaN
 };
 
 // One step's bookkeeping. Request r holds kv_len[r] tokens in the pages tables[r][0 .. ceil(kv_len/page))

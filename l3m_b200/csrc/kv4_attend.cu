@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdio>
 #include "kv4.cuh"
+#include "kv4_prompt.h"
 
 using namespace l3m;
 
@@ -1054,7 +1055,9 @@ L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, vo
     const int mx = cache->dtype == L3M_DT_MXFP4, two = row_blocks(cache, a) == 2;
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
-    if (a->dtype == L3M_DT_F32) {
+    if (prompt_fits(cache, a)) {
+        e = prompt_attend(cache, a, s);
+    } else if (a->dtype == L3M_DT_F32) {
         if (mx) e = two ? by_blocks<float, 1, 2>(p, s) : by_blocks<float, 1, 1>(p, s);
         else e = two ? by_blocks<float, 0, 2>(p, s) : by_blocks<float, 0, 1>(p, s);
     } else {

@@ -1,0 +1,603 @@
+// Attention of prompt chunks over the paged 4-bit cache on the fifth-generation tensor cores: the variant of
+// l3m_kv4_attend_dev for many query rows per key/value head (the rule is prompt_fits() below). bf16 queries and
+// results, head dims of 2 or 4 blocks.
+//
+// One CTA takes 256 rows (query, head of the group) of one request and kv head, as two tiles of 128, over the whole
+// context in steps of 128 tokens:
+//   4 warps  widen a step's codes to f16 in shared memory: keys K-major, values as they lie (MN-major), swizzled by
+//            128 bytes, two buffers each, the next step's codes under way in registers;
+//   1 thread issues the products: S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory);
+//   8 warps  one thread a row: S from tensor memory, softmax against the row's reference, P back as f16 over S's columns.
+// The two tiles alternate, so that one's products run under the other's softmax. Tensor memory: S (then P) of tile t at
+// columns 128 t, O of tile t at 256 + t * head_dim: all 512 columns, one CTA an SM.
+//
+// Scales. A widened value is an f16 number, code times scale, rounded once; scales are first multiplied by a power of two that
+// brings the context's largest near 2^11 (found in a first pass over the scales alone: 1/9 of the cache), undone in the scores'
+// factor and in the result. Queries are brought to 2^10 by row. P is 2^14 at most: the reference moves when a score
+// passes it by 14 (then to 10 below the largest), which multiplies O by a power of two.
+//
+// Every wait has a limit; a wait that gives up sets a status bit and the CTA's rows become NaN.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <algorithm>
+#include "kv4.cuh"
+#include "kv4_prompt.h"
+
+namespace l3m {
+namespace {
+
+constexpr int kRows = 128, kStep = 128;                 // rows of a tile, tokens of a step
+constexpr int kSoftWarps = 8, kWideWarps = 4;
+constexpr int kPromptThreads = 32 * (kSoftWarps + kWideWarps + 1);
+constexpr float kFloorRef = -1e30f;
+
+struct PromptArgs {
+    l3m_kv4_attend a;
+    Kv4Dev c;
+    int group, row_tiles, vec;
+};
+
+// ---- mbarriers, tensor memory, products
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void bar_init(uint64_t *b, int count) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(smem_u32(b)), "r"(count) : "memory"); }
+__device__ __forceinline__ void bar_arrive(uint64_t *b) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(smem_u32(b)) : "memory"); }
+// True once the barrier's phase `parity` has completed; false if that did not happen within two seconds.
+__device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
+    const uint32_t at = smem_u32(b);
+    unsigned long long begun = 0;
+    for (;;) {
+        uint32_t ok;
+        asm volatile("{ .reg .pred p;\n mbarrier.try_wait.parity.shared.b64 p, [%1], %2, 1000;\n selp.u32 %0, 1, 0, p; }" : "=r"(ok) : "r"(at), "r"(parity) : "memory");
+        if (ok) return true;
+        unsigned long long now;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+        if (!begun) begun = now;
+        if (now - begun > 2000000000ull) return false;
+    }
+}
+// The same for a whole warp, which has to stay together.
+__device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(b, parity)); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(uint64_t *b) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+}
+// d (tensor memory) = or += a . b, f16 operands, f32 accumulators; a in shared or in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    asm volatile("{ .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+__device__ __forceinline__ void tmem_load32(uint32_t *r, uint32_t at) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, "
+        "%29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]),
+          "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(at));
+}
+__device__ __forceinline__ void tmem_load16(uint32_t *r, uint32_t at) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+                   "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(at));
+}
+__device__ __forceinline__ void tmem_store16(uint32_t at, const uint32_t *r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(at), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]),
+                 "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+                 : "memory");
+}
+// wait::ld with the loaded registers as operands, so that no use of them moves above it.
+template <int N> __device__ __forceinline__ void tmem_wait_ld(uint32_t *r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; i++) asm volatile("" : "+r"(r[i]));
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Shared-memory operand of rows of 128 bytes swizzled by 128: groups of 8 rows 1024 bytes apart; `lead` bytes between blocks
+// of 64 elements where those run along the product's M or N (values), unused where they run along K.
+__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead) {
+    return (uint64_t)(at >> 4 & 0x3fff) | (uint64_t)(lead >> 4 & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+    const __half2 r = __hmul2(*(const __half2 *)&a, *(const __half2 *)&b);
+    return *(const uint32_t *)&r;
+}
+__device__ __forceinline__ float exp2i(int e) { return __int_as_float((e + 127) << 23); }   // 2^e, -126 <= e <= 127
+// x * 2^e for any e that a result needs: two factors.
+__device__ __forceinline__ float scale2(float x, int e) {
+    const int h = max(min(e, 240), -240) / 2;
+    return x * exp2i(h) * exp2i(max(min(e, 240), -240) - h);
+}
+__device__ __forceinline__ uint32_t e2m1_pair(uint32_t w) {
+    uint32_t d;
+    asm("{ .reg .b8 c, z0, z1, z2;\n mov.b32 {c, z0, z1, z2}, %1;\n cvt.rn.f16x2.e2m1x2 %0, c; }" : "=r"(d) : "r"(w));
+    return d;
+}
+
+// The 8 codes of a word as four f16 pairs, times the scales' pairs: q4_0 pairs nibbles k and k + 4 (s[0] twice), mxfp4
+// the two of byte k (s[0] for bytes 0 and 1, s[1] for 2 and 3).
+template <int MX> __device__ __forceinline__ uint4 widen(uint32_t w, uint32_t s0, uint32_t s1) {
+    uint32_t f[4];
+    if (MX) {
+        f[0] = e2m1_pair(w); f[1] = e2m1_pair(w >> 8);
+        f[2] = e2m1_pair(w >> 16); f[3] = e2m1_pair(w >> 24);
+        return make_uint4(mul2(f[0], s0), mul2(f[1], s0), mul2(f[2], s1), mul2(f[3], s1));
+    }
+    // 1024 + n, and 1024 + 16 n four bits higher, are numbers whose last bits are the code's
+    const uint32_t y = w >> 8;
+    f[0] = (w & 0x000f000fu) | 0x64006400u; f[1] = (w & 0x00f000f0u) | 0x64006400u;
+    f[2] = (y & 0x000f000fu) | 0x64006400u; f[3] = (y & 0x00f000f0u) | 0x64006400u;
+    const __half2 off = __halves2half2(__ushort_as_half(0xe408), __ushort_as_half(0xe408));   // -1032
+    const __half2 s16 = __halves2half2(__ushort_as_half(0x2c00), __ushort_as_half(0x2c00));   // 1/16
+    const __half2 o16 = __halves2half2(__ushort_as_half(0xd480), __ushort_as_half(0xd480));   // -72
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        const __half2 h = *(const __half2 *)&f[k];
+        const __half2 r = k % 2 ? __hfma2(h, s16, o16) : __hadd2(h, off);
+        f[k] = *(const uint32_t *)&r;
+    }
+    return make_uint4(mul2(f[0], s0), mul2(f[1], s0), mul2(f[2], s0), mul2(f[3], s0));
+}
+
+template <int NG>
+struct Smem {
+    static constexpr int DP = 32 * NG, TILE = kRows * DP * 2;   // one operand tile of 128 rows
+    uint8_t q[2][TILE], k[2][TILE], v[2][TILE];
+    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    uint32_t tmem, bad[4][4];             // tokens of a step in no page of the cache, a ring of four steps
+    int k_top, v_top;
+};
+
+// One token's row as it lies in the cache.
+template <int NG, int MX>
+struct Codes {
+    uint32_t k[4 * NG], v[4 * NG], ks[MX ? 1 : NG / 2], vs[MX ? 1 : NG / 2];
+    bool there;
+};
+
+template <int NG, int MX>
+__global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs p) {
+    typedef Smem<NG> S;
+    constexpr int DP = S::DP, SB = MX ? 1 : 2;
+    extern __shared__ uint8_t raw[];
+    S &s = *(S *)(((uintptr_t)raw + 1023) & ~(uintptr_t)1023);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    // ---- what this CTA does: the last rows first, they see most
+    const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
+    const int r = x / per_req, h = (x - r * per_req) / p.row_tiles, rt = p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles);
+    const int start = p.a.q_start[r], nq = p.a.q_start[r + 1] - start, kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
+    const int row0 = rt * 2 * kRows, rows = nq * p.group - row0;           // rows left from this CTA's first
+    if (rows <= 0) return;
+    const int tiles = rows > kRows ? 2 : 1;
+    const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = kv - nq + i0, last = kv - nq + i1;   // the rows' positions
+    const int lo_any = p.a.window ? max(0, first - p.a.window + 1) : 0, hi_any = max(last + 1, 0);      // seen by some row
+    const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;                  // seen by every row
+    const int t0 = lo_any / kStep * kStep, steps = hi_any > lo_any ? (hi_any - t0 + kStep - 1) / kStep : 0;
+    const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
+
+    if (tid == 0) {
+        for (int b = 0; b < 2; b++) {
+            bar_init(&s.k_full[b], 32 * kWideWarps);
+            bar_init(&s.v_full[b], 32 * kWideWarps);
+            bar_init(&s.k_empty[b], 1);
+            bar_init(&s.v_empty[b], 1);
+            bar_init(&s.s_full[b], 1);
+            bar_init(&s.p_full[b], kRows);
+            bar_init(&s.pv_done[b], 1);
+        }
+        s.k_top = s.v_top = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == kSoftWarps + kWideWarps) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_u32(&s.tmem)) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+
+    // The row of token tok: where its tile is, null if its page is none of the cache's.
+    auto tile_of = [&](int tok) -> const uint8_t * {
+        const int blk = tok / p.c.page, off = tok - blk * p.c.page, id = table[blk];
+        return id >= 0 && id < p.c.n_pages ? p.c.data + p.c.tile_at(id, h, off / kKvTile) : nullptr;
+    };
+
+    // ---- the largest scales' exponents
+    {
+        int kt = 0, vt = 0;
+#pragma unroll 4
+        for (int tok = lo_any + tid; tok < hi_any; tok += kPromptThreads) {
+            const uint8_t *tile = tile_of(tok);
+            if (!tile) continue;
+            const int row = tok % p.c.page % kKvTile;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                const uint8_t *ks = tile + 512 * NG + (row * NG + j) * SB, *vs = ks + kKvTile * NG * SB;
+                const int ke = MX ? *ks : *(const uint16_t *)ks >> 10 & 31, ve = MX ? *vs : *(const uint16_t *)vs >> 10 & 31;
+                kt = max(kt, !MX && ke == 31 ? 0 : ke);
+                vt = max(vt, !MX && ve == 31 ? 0 : ve);
+            }
+        }
+        for (int o = 16; o; o >>= 1) {
+            kt = max(kt, __shfl_xor_sync(0xffffffffu, kt, o));
+            vt = max(vt, __shfl_xor_sync(0xffffffffu, vt, o));
+        }
+        if (lane == 0) {
+            atomicMax(&s.k_top, kt);
+            atomicMax(&s.v_top, vt);
+        }
+    }
+    const int tile = warp / 4;                                              // of a softmax warp
+    const int row = tile * kRows + (warp & 3) * 32 + lane, qi = (row0 + row) / p.group, head = h * p.group + (row0 + row) % p.group;
+    const bool live = warp < kSoftWarps && row < rows;
+    const int at = live ? kv - nq + qi : -1;
+    int up = 0;
+    if (warp < kSoftWarps && tile < tiles) {
+        // ---- this thread's query, in the order in which the keys' codes come out of their words
+        const __nv_bfloat16 *src = (const __nv_bfloat16 *)p.a.q + (size_t)(start + qi) * p.a.q_ld + (size_t)head * p.c.dim;
+        float top = 0.0f;
+        uint32_t raw8[DP / 2];
+#pragma unroll
+        for (int c = 0; c < DP / 8; c++) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (live && c * 8 < p.c.dim) {
+                if (p.vec) {
+                    v = *(const uint4 *)(src + c * 8);
+                } else {
+                    const uint16_t *hw = (const uint16_t *)src + c * 8;
+                    v = make_uint4(hw[0] | (uint32_t)hw[1] << 16, hw[2] | (uint32_t)hw[3] << 16, hw[4] | (uint32_t)hw[5] << 16, hw[6] | (uint32_t)hw[7] << 16);
+                }
+            }
+            raw8[4 * c] = v.x; raw8[4 * c + 1] = v.y; raw8[4 * c + 2] = v.z; raw8[4 * c + 3] = v.w;
+#pragma unroll
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw8[4 * c + e] << 16)), fabsf(__uint_as_float(raw8[4 * c + e] & 0xffff0000u))));
+        }
+        up = top > 0.0f ? 9 - max(min(ilogbf(top), 127), -149) : 0;        // |q| * 2^up < 2^10
+        const float f0 = exp2i(up / 2), f1 = exp2i(up - up / 2);
+        const int rr = row & (kRows - 1);
+#pragma unroll
+        for (int c = 0; c < DP / 8; c++) {
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                e[2 * i] = __uint_as_float(raw8[4 * c + i] << 16) * f0 * f1;
+                e[2 * i + 1] = __uint_as_float(raw8[4 * c + i] & 0xffff0000u) * f0 * f1;
+            }
+            const uint4 v = MX ? make_uint4(pack_f16(e[0], e[1]), pack_f16(e[2], e[3]), pack_f16(e[4], e[5]), pack_f16(e[6], e[7]))
+                               : make_uint4(pack_f16(e[0], e[4]), pack_f16(e[1], e[5]), pack_f16(e[2], e[6]), pack_f16(e[3], e[7]));
+            *(uint4 *)(s.q[tile] + c / 8 * (kRows * 128) + rr * 128 + ((c % 8 ^ rr & 7) << 4)) = v;
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read what was written here
+    }
+    __syncthreads();
+    const uint32_t tmem = s.tmem;
+    // q4_0: d < 2^(top - 14), brought below 2^11. mxfp4: 2^(top - 127), brought to 2^11.
+    const int k_up = MX ? 11 + 127 - s.k_top : 25 - s.k_top, v_up = MX ? 11 + 127 - s.v_top : 25 - s.v_top;
+    bool ok = true;
+
+    if (warp >= kSoftWarps && warp < kSoftWarps + kWideWarps) {
+        // ---- widening: thread = token of the step
+        const int tk = tid - 32 * kSoftWarps;
+        typedef Codes<NG, MX> C;
+        auto fetch = [&](C &c, int j) {
+            const int tok = t0 + j * kStep + tk;
+            const uint8_t *tl = j < steps && tok >= lo_any && tok < hi_any ? tile_of(tok) : nullptr;
+            c.there = tl != nullptr;
+            if (!tl) return;
+            const int row16 = tok % p.c.page % kKvTile;
+            const uint8_t *ks = tl + row16 * 16 * NG, *vs = ks + 256 * NG, *sc = tl + 512 * NG + row16 * NG * SB;
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                const uint4 a = __ldg((const uint4 *)ks + i), b = __ldg((const uint4 *)vs + i);
+                c.k[4 * i] = a.x; c.k[4 * i + 1] = a.y; c.k[4 * i + 2] = a.z; c.k[4 * i + 3] = a.w;
+                c.v[4 * i] = b.x; c.v[4 * i + 1] = b.y; c.v[4 * i + 2] = b.z; c.v[4 * i + 3] = b.w;
+            }
+            if (MX) {
+                c.ks[0] = NG == 4 ? *(const uint32_t *)sc : *(const uint16_t *)sc;
+                c.vs[0] = NG == 4 ? *(const uint32_t *)(sc + kKvTile * NG) : *(const uint16_t *)(sc + kKvTile * NG);
+            } else {
+#pragma unroll
+                for (int i = 0; i < NG / 2; i++) {
+                    c.ks[i] = ((const uint32_t *)sc)[i];
+                    c.vs[i] = ((const uint32_t *)(sc + kKvTile * NG * 2))[i];
+                }
+            }
+        };
+        // Scales [NG] as f16 pairs of the same scale twice (pair j), brought up by 2^by. edge: what is not finite counts as 0.
+        auto scale_of = [&](const uint32_t *w, int j, int by, bool edge) -> float {
+            if (MX) {
+                const int e = (int)(w[0] >> (8 * j) & 0xff) + by - 127;
+                return e < -24 ? 0.0f : exp2i(min(e, 15));
+            }
+            uint32_t hbits = w[j / 2] >> (16 * (j % 2)) & 0xffff;
+            if (edge && (hbits & 0x7c00) == 0x7c00) hbits = 0;
+            return scale2(__half2float(__ushort_as_half((unsigned short)hbits)), by);
+        };
+        C cur, next;
+        fetch(cur, 0);
+        for (int j = 0; j < steps && ok; j++) {
+            const int b = j & 1, tok0 = t0 + j * kStep;
+            const bool edge = tok0 < whole_lo || tok0 + kStep > whole_hi;
+            fetch(next, j + 1);
+            if (j >= 2) ok = warp_wait(&s.k_empty[b], (j / 2 - 1) & 1);
+            const int tok = tok0 + tk;
+            const bool wanted = tok >= lo_any && tok < hi_any;
+            const uint32_t miss = __ballot_sync(0xffffffffu, wanted && !cur.there);
+            if (lane == 0) s.bad[j & 3][warp - kSoftWarps] = miss;
+            if (wanted && !cur.there && p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
+            uint8_t *kd = s.k[b] + tk * 128, *vd = s.v[b] + tk * 128;
+            const int sw = tk & 7;
+#pragma unroll
+            for (int g = 0; g < NG; g++) {
+                const float d = cur.there ? scale_of(cur.ks, g, k_up, edge) : 0.0f;
+                const uint32_t d2 = pack_f16(d, d);
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    const uint4 v = cur.there ? widen<MX>(cur.k[t * NG + g], d2, d2) : make_uint4(0, 0, 0, 0);
+                    const int c = 4 * g + t;
+                    *(uint4 *)(kd + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&s.k_full[b]);
+            if (j >= 2) ok = warp_wait(&s.v_empty[b], (j / 2 - 1) & 1) && ok;
+#pragma unroll
+            for (int q2 = 0; q2 < NG / 2; q2++) {
+                const float d0 = cur.there ? scale_of(cur.vs, 2 * q2, v_up, edge) : 0.0f, d1 = cur.there ? scale_of(cur.vs, 2 * q2 + 1, v_up, edge) : 0.0f;
+                const uint32_t s0 = MX ? pack_f16(d0, d0) : pack_f16(d0, d1), s1 = pack_f16(d1, d1);
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    const int c = g * (NG / 2) + q2;
+                    const uint4 v = cur.there ? widen<MX>(cur.v[c], s0, s1) : make_uint4(0, 0, 0, 0);
+                    *(uint4 *)(vd + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(&s.v_full[b]);
+            cur = next;
+        }
+    } else if (warp == kSoftWarps + kWideWarps) {
+        // ---- the products
+        if (lane == 0 && steps) {
+            constexpr uint32_t base = 1u << 4 | (kRows / 16) << 24;         // f32 accumulators, f16 operands, M 128
+            constexpr uint32_t qk = base | (kStep / 8) << 17, pv = base | (DP / 8) << 17 | 1u << 16;   // N; bit 16: b runs along N
+            auto score = [&](int j, int t) {
+                const uint32_t qa = smem_u32(s.q[t]), ka = smem_u32(s.k[j & 1]);
+#pragma unroll
+                for (int c = 0; c < DP / 16; c++) {
+                    const uint32_t off = c / 4 * (kRows * 128) + c % 4 * 32;
+                    mma_ss(tmem + t * 128, operand(qa + off, 16), operand(ka + off, 16), qk, c > 0);
+                }
+                tc_commit(&s.s_full[t]);
+            };
+            ok = bar_wait(&s.k_full[0], 0);
+            tc_after();
+            for (int t = 0; t < tiles && ok; t++) score(0, t);
+            if (ok) tc_commit(&s.k_empty[0]);
+            for (int j = 0; j < steps && ok; j++) {
+                for (int t = 0; t < tiles && ok; t++) {
+                    if (t == 0) ok = bar_wait(&s.v_full[j & 1], j / 2 & 1);
+                    ok = ok && bar_wait(&s.p_full[t], j & 1);
+                    if (!ok) break;
+                    tc_after();
+                    const uint32_t va = smem_u32(s.v[j & 1]);
+#pragma unroll
+                    for (int c = 0; c < kStep / 16; c++)
+                        mma_ts(tmem + 256 + t * DP, tmem + t * 128 + c * 8, operand(va + c * 2048, kRows * 128), pv, j > 0 || c > 0);
+                    tc_commit(&s.pv_done[t]);
+                    if (t == tiles - 1) tc_commit(&s.v_empty[j & 1]);
+                    if (j + 1 < steps) {
+                        if (t == 0) {
+                            ok = bar_wait(&s.k_full[(j + 1) & 1], (j + 1) / 2 & 1);
+                            tc_after();
+                        }
+                        if (ok) {
+                            score(j + 1, t);
+                            if (t == tiles - 1) tc_commit(&s.k_empty[(j + 1) & 1]);
+                        }
+                    }
+                }
+            }
+        }
+        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    } else if (tile < tiles) {
+        // ---- softmax: thread = row
+        const uint32_t mine = tmem + tile * 128 + ((uint32_t)(warp & 3) << 21);     // lane 32 * (warp % 4) in the upper half
+        const uint32_t mine_o = tmem + 256 + tile * DP + ((uint32_t)(warp & 3) << 21);
+        const float mult = scale2(p.a.scale * 1.4426950408889634f, -up - k_up);
+        float ref = kFloorRef, sum = 0.0f;
+        const int low = p.a.window ? at - p.a.window + 1 : 0;
+        for (int j = 0; j < steps && ok; j++) {
+            ok = warp_wait(&s.s_full[tile], j & 1);
+            if (!ok) break;
+            tc_after();
+            const int tok0 = t0 + j * kStep;
+            const uint32_t *bad = s.bad[j & 3];
+            const bool edge = tok0 < whole_lo || tok0 + kStep > whole_hi || (bad[0] | bad[1] | bad[2] | bad[3]);
+            uint32_t sc[2][32];
+            tmem_load32(sc[0], mine);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                uint32_t *v = sc[c & 1];
+                tmem_wait_ld<32>(v);
+                if (c < 3) tmem_load32(sc[(c + 1) & 1], mine + 32 * (c + 1));
+                float z[32], high = kFloorRef;
+                if (edge) {
+                    const uint32_t miss = bad[c];
+                    const int a = tok0 + 32 * c;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const bool seen = a + i <= at && a + i >= low && !(miss >> i & 1);
+                        z[i] = seen ? fmaf(__uint_as_float(v[i]), mult, -ref) : -INFINITY;
+                        high = fmaxf(high, z[i]);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        z[i] = fmaf(__uint_as_float(v[i]), mult, -ref);
+                        high = fmaxf(high, z[i]);
+                    }
+                }
+                if (__any_sync(0xffffffffu, high > 14.0f)) {
+                    // Rows whose reference is passed: a new one, an integer, 10 below the chunk's largest
+                    float m = -INFINITY;
+#pragma unroll
+                    for (int i = 0; i < 32; i++)
+                        if (z[i] != -INFINITY) m = fmaxf(m, __uint_as_float(v[i]) * mult);
+                    float f = 1.0f;
+                    if (high > 14.0f) {
+                        const float to = ceilf(m) - 10.0f;
+                        f = ex2(ref - to);
+                        ref = to;
+                    }
+                    sum *= f;
+                    if (j > 0) {
+                        ok = warp_wait(&s.pv_done[tile], (j - 1) & 1) && ok;
+                        tc_after();
+#pragma unroll 1
+                        for (int d = 0; d < DP; d += 16) {
+                            uint32_t o[16];
+                            tmem_load16(o, mine_o + d);
+                            tmem_wait_ld<16>(o);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            tmem_store16(mine_o + d, o);
+                        }
+                    }
+                    const uint32_t f2 = pack_f16(f, f);
+#pragma unroll 1
+                    for (int d = 0; d < c; d++) {                            // this step's P so far
+                        uint32_t o[16];
+                        tmem_load16(o, mine + 16 * d);
+                        tmem_wait_ld<16>(o);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) o[i] = mul2(o[i], f2);
+                        tmem_store16(mine + 16 * d, o);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i++) z[i] = z[i] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[i]), mult, -ref);
+                }
+                uint32_t pr[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const float e0 = ex2(z[2 * i]), e1 = ex2(z[2 * i + 1]);
+                    sum += e0 + e1;
+                    pr[i] = pack_f16(e0, e1);
+                }
+                tmem_store16(mine + 16 * c, pr);
+            }
+            tmem_wait_st();
+            tc_before();
+            bar_arrive(&s.p_full[tile]);
+        }
+        // ---- the rows' results
+        if (steps) ok = warp_wait(&s.pv_done[tile], (steps - 1) & 1) && ok;
+        tc_after();
+        const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+        __nv_bfloat16 *dst = (__nv_bfloat16 *)p.a.out + (size_t)(start + qi) * p.a.out_ld + (size_t)head * p.c.dim;
+#pragma unroll
+        for (int c = 0; c < DP / 16; c++) {                                  // 16 columns: 4 dims of each of 4 (2) blocks
+            uint32_t o[16];
+            if (steps) {
+                tmem_load16(o, mine_o + 16 * c);
+                tmem_wait_ld<16>(o);
+            }
+#pragma unroll
+            for (int q4 = 0; q4 < 4; q4++) {
+                float e[4];
+                int d;
+                if (NG == 4) {                                               // one part g = c: block q4
+                    d = 32 * q4 + 4 * c;
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int col = MX ? q4 / 2 * 8 + q4 % 2 * 4 + k : q4 / 2 * 8 + 2 * k + q4 % 2;
+                        e[k] = __uint_as_float(o[col]);
+                    }
+                } else {                                                     // two parts g = 2 c, 2 c + 1: blocks 0 and 1
+                    d = 32 * (q4 % 2) + 4 * (2 * c + q4 / 2);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const int col = q4 / 2 * 8 + (MX ? q4 % 2 * 4 + k : 2 * k + q4 % 2);
+                        e[k] = __uint_as_float(o[col]);
+                    }
+                }
+                if (!live || d >= p.c.dim) continue;
+#pragma unroll
+                for (int k = 0; k < 4; k++) e[k] = !ok ? __uint_as_float(0x7fffffffu) : inv == 0.0f ? 0.0f : scale2(e[k] * inv, -v_up);
+                if (p.vec) {
+                    __nv_bfloat162 two[2] = {__floats2bfloat162_rn(e[0], e[1]), __floats2bfloat162_rn(e[2], e[3])};
+                    *(uint2 *)(dst + d) = *(const uint2 *)two;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; k++) dst[d + k] = __float2bfloat16_rn(e[k]);
+                }
+            }
+        }
+    }
+    if (!ok && p.a.status) atomicOr((int *)p.a.status, L3M_KV4_TIMEOUT);
+    tc_before();
+    __syncthreads();
+    if (warp == kSoftWarps + kWideWarps) {
+        tc_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+template <int NG, int MX>
+cudaError_t launch(const PromptArgs &p, cudaStream_t s) {
+    const int smem = (int)sizeof(Smem<NG>) + 1024;
+    cudaError_t e = cudaFuncSetAttribute(prompt_kernel<NG, MX>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    cudaLaunchAttribute early;
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)((long long)p.a.n_req * p.c.n_kv * p.row_tiles));
+    cfg.blockDim = dim3(kPromptThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cfg.attrs = &early;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, prompt_kernel<NG, MX>, p);
+}
+
+long long prompt_ctas(const l3m_kv4 *c, const l3m_kv4_attend *a) {
+    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
+    return (rows + 2 * kRows - 1) / (2 * kRows) * a->n_req * c->n_kv_heads;
+}
+
+}  // namespace
+
+bool prompt_fits(const l3m_kv4 *c, const l3m_kv4_attend *a) {
+    const int ng = (c->head_dim + kKvBlock - 1) / kKvBlock;
+    if (a->dtype != L3M_DT_BF16 || (ng != 2 && ng != 4)) return false;
+    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
+    return rows >= 96 && prompt_ctas(c, a) >= 32 && prompt_ctas(c, a) < 0x7fffffff;
+}
+
+cudaError_t prompt_attend(const l3m_kv4 *c, const l3m_kv4_attend *a, cudaStream_t s) {
+    PromptArgs p = {*a, kv4_dev(c), a->n_heads / c->n_kv_heads, 0, 0};
+    p.row_tiles = (int)(((long long)a->max_q * p.group + 2 * kRows - 1) / (2 * kRows));
+    p.vec = !(((uintptr_t)a->q | (uintptr_t)a->out) & 15) && (a->q_ld | a->out_ld) % 8 == 0;
+    const bool mx = c->dtype == L3M_DT_MXFP4;
+    if (p.c.ng == 2) return mx ? launch<2, 1>(p, s) : launch<2, 0>(p, s);
+    return mx ? launch<4, 1>(p, s) : launch<4, 0>(p, s);
+}
+
+}  // namespace l3m
