@@ -3,13 +3,15 @@
 // results, head dims of 2 or 4 blocks.
 //
 // One CTA takes 256 rows (query, head of the group) of one request and kv head, as two tiles of 128, over the whole
-// context in steps of 128 tokens:
-//   4 warps  widen a step's codes to f16 in shared memory: keys K-major, values as they lie (MN-major), swizzled by
-//            128 bytes, two buffers each, the next step's codes under way in registers;
-//   1 thread issues the products: S = Q K^T (both operands in shared memory) and O += P V (P in tensor memory);
+// context, 128 tokens widened at a time and multiplied 64 at a time:
+//   8 warps  widen a step's codes to f16 in shared memory, 4 the keys (K-major), 4 the values (as they lie, MN-major), swizzled
+//            by 128 bytes, two buffers each, the next step's codes under way in registers;
+//   2 warps  issue the products, one for each tile: S = Q K^T (both operands in shared memory) and O += P V (P in tensor
+//            memory); by one warp for both, its waits and issues were the longest chain (238 us against what stands in the table);
 //   8 warps  one thread a row: S from tensor memory, softmax against the row's reference, P back as f16 over S's columns.
-// The two tiles alternate, so that one's products run under the other's softmax. Tensor memory: S (then P) of tile t at
-// columns 128 t, O of tile t at 256 + t * head_dim: all 512 columns, one CTA an SM.
+// S has two halves of 64 tokens a tile, so that the next half's scores are formed while one goes through the softmax, and the two
+// tiles alternate. Tensor memory: S (then P) of tile t, half u at columns 128 t + 64 u, O of tile t at 256 + t * head_dim: all 512
+// columns, one CTA an SM.
 //
 // Scales. A widened value is an f16 number, code times scale, rounded once; scales are first multiplied by a power of two that
 // brings the context's largest near 2^11 (found in a first pass over the scales alone: 1/9 of the cache), undone in the scores'
@@ -26,10 +28,9 @@
 namespace l3m {
 namespace {
 
-constexpr int kRows = 128, kStep = 128;                 // rows of a tile, tokens of a step
-constexpr int kSoftWarps = 8, kWideWarps = 4;
-constexpr int kPromptThreads = 32 * (kSoftWarps + kWideWarps + 1);
-constexpr float kFloorRef = -1e30f;
+constexpr int kRows = 128, kStep = 128, kHalf = 64;     // rows of a tile, tokens that are widened at a time, tokens of a product
+constexpr int kSoftWarps = 8, kWideWarps = 8;          // half of the latter for keys, half for values
+constexpr int kPromptThreads = 32 * (kSoftWarps + kWideWarps + 2);
 
 struct PromptArgs {
     l3m_kv4_attend a;
@@ -60,15 +61,28 @@ __device__ __forceinline__ bool bar_wait(uint64_t *b, uint32_t parity) {
 __device__ __forceinline__ bool warp_wait(uint64_t *b, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(b, parity)); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t *b) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(b)) : "memory");
+// The products' operands are uniform over the warp and one lane issues: the whole warp runs this code, so that the
+// operands can stay in uniform registers (issued from a divergent branch a product took 125 cycles, whatever its size).
+__device__ __forceinline__ uint32_t elect_one() {
+    uint32_t is;
+    asm volatile("{ .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p; }" : "=r"(is));
+    return is;
 }
+__device__ __forceinline__ void tc_commit(uint32_t lead, uint32_t bar) {
+    asm volatile("{ .reg .pred l;\n setp.ne.u32 l, %1, 0;\n @l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0]; }" ::"r"(bar), "r"(lead) : "memory");
+}
+// Shared-memory operand of rows of 128 bytes swizzled by 128, groups of 8 rows 1024 bytes apart. Low word: address, and the bytes between
+// blocks of 64 elements where those run along the product's M or N (values; unused where they run along K).
+constexpr uint32_t kOperandHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t operand(uint32_t at, uint32_t lead) { return (at >> 4 & 0x3fff) | (lead >> 4) << 16; }
 // d (tensor memory) = or += a . b, f16 operands, f32 accumulators; a in shared or in tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{ .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p; }" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void mma_ss(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{ .reg .pred l, p;\n .reg .b64 x, y;\n setp.ne.u32 l, %6, 0;\n setp.ne.u32 p, %4, 0;\n mov.b64 x, {%1, %5};\n mov.b64 y, {%2, %5};\n"
+                 " @l tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p; }" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "n"(kOperandHigh), "r"(lead) : "memory");
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    asm volatile("{ .reg .pred p;\n setp.ne.u32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+__device__ __forceinline__ void mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, uint32_t add) {
+    asm volatile("{ .reg .pred l, p;\n .reg .b64 y;\n setp.ne.u32 l, %6, 0;\n setp.ne.u32 p, %4, 0;\n mov.b64 y, {%2, %5};\n"
+                 " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p; }" ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(add), "n"(kOperandHigh), "r"(lead) : "memory");
 }
 __device__ __forceinline__ void tmem_load32(uint32_t *r, uint32_t at) {
     asm volatile(
@@ -98,16 +112,22 @@ template <int N> __device__ __forceinline__ void tmem_wait_ld(uint32_t *r) {
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Shared-memory operand of rows of 128 bytes swizzled by 128: groups of 8 rows 1024 bytes apart; `lead` bytes between blocks
-// of 64 elements where those run along the product's M or N (values), unused where they run along K.
-__device__ __forceinline__ uint64_t operand(uint32_t at, uint32_t lead) {
-    return (uint64_t)(at >> 4 & 0x3fff) | (uint64_t)(lead >> 4 & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
-
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+// Two at a time: z = (x, y) * m + c; s += (x, y).
+__device__ __forceinline__ void fma_two(float *z, float x, float y, float m, float c) {
+    asm("{ .reg .b64 a, b, d;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %4};\n mov.b64 d, {%5, %5};\n fma.rn.f32x2 d, a, b, d;\n mov.b64 {%0, %1}, d; }" : "=f"(z[0]), "=f"(z[1]) : "f"(x), "f"(y), "f"(m), "f"(c));
+}
+__device__ __forceinline__ void add_two(float *s, float x, float y) {
+    asm("{ .reg .b64 a, b;\n mov.b64 a, {%0, %1};\n mov.b64 b, {%2, %3};\n add.rn.f32x2 a, a, b;\n mov.b64 {%0, %1}, a; }" : "+f"(s[0]), "+f"(s[1]) : "f"(x), "f"(y));
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t d;
@@ -159,15 +179,16 @@ template <int NG>
 struct Smem {
     static constexpr int DP = 32 * NG, TILE = kRows * DP * 2;   // one operand tile of 128 rows
     uint8_t q[2][TILE], k[2][TILE], v[2][TILE];
-    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2], s_full[2], p_full[2], pv_done[2];
+    uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
+    uint64_t s_full[2][2], p_full[2][2], pv_done[2];      // [tile][half]
     uint32_t tmem, bad[4][4];             // tokens of a step in no page of the cache, a ring of four steps
     int k_top, v_top;
 };
 
-// One token's row as it lies in the cache.
+// One token's keys or values as they lie in the cache.
 template <int NG, int MX>
 struct Codes {
-    uint32_t k[4 * NG], v[4 * NG], ks[MX ? 1 : NG / 2], vs[MX ? 1 : NG / 2];
+    uint32_t w[4 * NG], sc[MX ? 1 : NG / 2];
     bool there;
 };
 
@@ -190,17 +211,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = kv - nq + i0, last = kv - nq + i1;   // the rows' positions
     const int lo_any = p.a.window ? max(0, first - p.a.window + 1) : 0, hi_any = max(last + 1, 0);      // seen by some row
     const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;                  // seen by every row
-    const int t0 = lo_any / kStep * kStep, steps = hi_any > lo_any ? (hi_any - t0 + kStep - 1) / kStep : 0;
+    const int t0 = lo_any / kStep * kStep, steps = hi_any > lo_any ? (hi_any - t0 + kStep - 1) / kStep : 0, halves = hi_any > lo_any ? (hi_any - t0 + kHalf - 1) / kHalf : 0;
     const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
 
     if (tid == 0) {
         for (int b = 0; b < 2; b++) {
-            bar_init(&s.k_full[b], 32 * kWideWarps);
-            bar_init(&s.v_full[b], 32 * kWideWarps);
-            bar_init(&s.k_empty[b], 1);
-            bar_init(&s.v_empty[b], 1);
-            bar_init(&s.s_full[b], 1);
-            bar_init(&s.p_full[b], kRows);
+            bar_init(&s.k_full[b], kStep);
+            bar_init(&s.v_full[b], kStep);
+            bar_init(&s.k_empty[b], tiles);
+            bar_init(&s.v_empty[b], tiles);
+            for (int u = 0; u < 2; u++) {
+                bar_init(&s.s_full[b][u], 1);
+                bar_init(&s.p_full[b][u], kRows);
+            }
             bar_init(&s.pv_done[b], 1);
         }
         s.k_top = s.v_top = 0;
@@ -251,10 +274,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     if (warp < kSoftWarps && tile < tiles) {
         // ---- this thread's query, in the order in which the keys' codes come out of their words
         const __nv_bfloat16 *src = (const __nv_bfloat16 *)p.a.q + (size_t)(start + qi) * p.a.q_ld + (size_t)head * p.c.dim;
-        float top = 0.0f;
-        uint32_t raw8[DP / 2];
-#pragma unroll
-        for (int c = 0; c < DP / 8; c++) {
+        auto piece = [&](int c) {                                            // 8 dims
             uint4 v = make_uint4(0, 0, 0, 0);
             if (live && c * 8 < p.c.dim) {
                 if (p.vec) {
@@ -264,24 +284,32 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                     v = make_uint4(hw[0] | (uint32_t)hw[1] << 16, hw[2] | (uint32_t)hw[3] << 16, hw[4] | (uint32_t)hw[5] << 16, hw[6] | (uint32_t)hw[7] << 16);
                 }
             }
-            raw8[4 * c] = v.x; raw8[4 * c + 1] = v.y; raw8[4 * c + 2] = v.z; raw8[4 * c + 3] = v.w;
+            return v;
+        };
+        float top = 0.0f;
+#pragma unroll 4
+        for (int c = 0; c < DP / 8; c++) {
+            const uint4 v = piece(c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(raw8[4 * c + e] << 16)), fabsf(__uint_as_float(raw8[4 * c + e] & 0xffff0000u))));
+            for (int e = 0; e < 4; e++) top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
         }
         up = top > 0.0f ? 9 - max(min(ilogbf(top), 127), -149) : 0;        // |q| * 2^up < 2^10
         const float f0 = exp2i(up / 2), f1 = exp2i(up - up / 2);
         const int rr = row & (kRows - 1);
-#pragma unroll
+#pragma unroll 4
         for (int c = 0; c < DP / 8; c++) {
+            const uint4 v = piece(c);
+            const uint32_t w[4] = {v.x, v.y, v.z, v.w};
             float e[8];
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                e[2 * i] = __uint_as_float(raw8[4 * c + i] << 16) * f0 * f1;
-                e[2 * i + 1] = __uint_as_float(raw8[4 * c + i] & 0xffff0000u) * f0 * f1;
+                e[2 * i] = __uint_as_float(w[i] << 16) * f0 * f1;
+                e[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u) * f0 * f1;
             }
-            const uint4 v = MX ? make_uint4(pack_f16(e[0], e[1]), pack_f16(e[2], e[3]), pack_f16(e[4], e[5]), pack_f16(e[6], e[7]))
+            const uint4 f = MX ? make_uint4(pack_f16(e[0], e[1]), pack_f16(e[2], e[3]), pack_f16(e[4], e[5]), pack_f16(e[6], e[7]))
                                : make_uint4(pack_f16(e[0], e[4]), pack_f16(e[1], e[5]), pack_f16(e[2], e[6]), pack_f16(e[3], e[7]));
-            *(uint4 *)(s.q[tile] + c / 8 * (kRows * 128) + rr * 128 + ((c % 8 ^ rr & 7) << 4)) = v;
+            *(uint4 *)(s.q[tile] + c / 8 * (kRows * 128) + rr * 128 + ((c % 8 ^ rr & 7) << 4)) = f;
         }
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");        // the products read what was written here
     }
@@ -293,221 +321,200 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
 
     if (warp >= kSoftWarps && warp < kSoftWarps + kWideWarps) {
         // ---- widening: thread = token of the step
-        const int tk = tid - 32 * kSoftWarps;
+        const int tk = tid & (kStep - 1);
+        const bool values = warp >= kSoftWarps + kWideWarps / 2;
+        const int by = values ? v_up : k_up, code_at = values ? 256 * NG : 0, scale_at = 512 * NG + (values ? kKvTile * NG * SB : 0);
         typedef Codes<NG, MX> C;
-        auto fetch = [&](C &c, int j) {
+        // A token's tile is found a step before its codes are read, its codes are read a step before they are widened.
+        auto find = [&](int j) -> const uint8_t * {
             const int tok = t0 + j * kStep + tk;
-            const uint8_t *tl = j < steps && tok >= lo_any && tok < hi_any ? tile_of(tok) : nullptr;
+            return j < steps && tok >= lo_any && tok < hi_any ? tile_of(tok) : nullptr;
+        };
+        auto fetch = [&](C &c, const uint8_t *tl, int j) {
             c.there = tl != nullptr;
             if (!tl) return;
-            const int row16 = tok % p.c.page % kKvTile;
-            const uint8_t *ks = tl + row16 * 16 * NG, *vs = ks + 256 * NG, *sc = tl + 512 * NG + row16 * NG * SB;
+            const int row16 = (t0 + j * kStep + tk) % p.c.page % kKvTile;
+            const uint8_t *codes = tl + code_at + row16 * 16 * NG, *sc = tl + scale_at + row16 * NG * SB;
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                const uint4 a = __ldg((const uint4 *)ks + i), b = __ldg((const uint4 *)vs + i);
-                c.k[4 * i] = a.x; c.k[4 * i + 1] = a.y; c.k[4 * i + 2] = a.z; c.k[4 * i + 3] = a.w;
-                c.v[4 * i] = b.x; c.v[4 * i + 1] = b.y; c.v[4 * i + 2] = b.z; c.v[4 * i + 3] = b.w;
+                const uint4 a = __ldg((const uint4 *)codes + i);
+                c.w[4 * i] = a.x; c.w[4 * i + 1] = a.y; c.w[4 * i + 2] = a.z; c.w[4 * i + 3] = a.w;
             }
             if (MX) {
-                c.ks[0] = NG == 4 ? *(const uint32_t *)sc : *(const uint16_t *)sc;
-                c.vs[0] = NG == 4 ? *(const uint32_t *)(sc + kKvTile * NG) : *(const uint16_t *)(sc + kKvTile * NG);
+                c.sc[0] = NG == 4 ? *(const uint32_t *)sc : *(const uint16_t *)sc;
             } else {
 #pragma unroll
-                for (int i = 0; i < NG / 2; i++) {
-                    c.ks[i] = ((const uint32_t *)sc)[i];
-                    c.vs[i] = ((const uint32_t *)(sc + kKvTile * NG * 2))[i];
-                }
+                for (int i = 0; i < NG / 2; i++) c.sc[i] = ((const uint32_t *)sc)[i];
             }
         };
-        // Scales [NG] as f16 pairs of the same scale twice (pair j), brought up by 2^by. edge: what is not finite counts as 0.
-        auto scale_of = [&](const uint32_t *w, int j, int by, bool edge) -> float {
+        // Block j's scale brought up by 2^by. edge: what is not finite counts as 0.
+        auto scale_of = [&](const C &c, int j, bool edge) -> float {
             if (MX) {
-                const int e = (int)(w[0] >> (8 * j) & 0xff) + by - 127;
+                const int e = (int)(c.sc[0] >> (8 * j) & 0xff) + by - 127;
                 return e < -24 ? 0.0f : exp2i(min(e, 15));
             }
-            uint32_t hbits = w[j / 2] >> (16 * (j % 2)) & 0xffff;
+            uint32_t hbits = c.sc[j / 2] >> (16 * (j % 2)) & 0xffff;
             if (edge && (hbits & 0x7c00) == 0x7c00) hbits = 0;
             return scale2(__half2float(__ushort_as_half((unsigned short)hbits)), by);
         };
         C cur, next;
-        fetch(cur, 0);
+        fetch(cur, find(0), 0);
+        const uint8_t *ahead = find(1);
         for (int j = 0; j < steps && ok; j++) {
-            const int b = j & 1, tok0 = t0 + j * kStep;
+            const int b = j & 1, tok0 = t0 + j * kStep, sw = tk & 7;
             const bool edge = tok0 < whole_lo || tok0 + kStep > whole_hi;
-            fetch(next, j + 1);
-            if (j >= 2) ok = warp_wait(&s.k_empty[b], (j / 2 - 1) & 1);
-            const int tok = tok0 + tk;
-            const bool wanted = tok >= lo_any && tok < hi_any;
-            const uint32_t miss = __ballot_sync(0xffffffffu, wanted && !cur.there);
-            if (lane == 0) s.bad[j & 3][warp - kSoftWarps] = miss;
-            if (wanted && !cur.there && p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
-            uint8_t *kd = s.k[b] + tk * 128, *vd = s.v[b] + tk * 128;
-            const int sw = tk & 7;
+            fetch(next, ahead, j + 1);
+            ahead = find(j + 2);
+            if (j >= 2) ok = warp_wait(values ? &s.v_empty[b] : &s.k_empty[b], (j / 2 - 1) & 1);
+            uint8_t *dst = (values ? s.v[b] : s.k[b]) + tk * 128;
+            if (!values) {
+                const bool wanted = tok0 + tk >= lo_any && tok0 + tk < hi_any;
+                const uint32_t miss = __ballot_sync(0xffffffffu, wanted && !cur.there);
+                if (lane == 0) s.bad[j & 3][warp - kSoftWarps] = miss;
+                if (wanted && !cur.there && p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
 #pragma unroll
-            for (int g = 0; g < NG; g++) {
-                const float d = cur.there ? scale_of(cur.ks, g, k_up, edge) : 0.0f;
-                const uint32_t d2 = pack_f16(d, d);
+                for (int g = 0; g < NG; g++) {
+                    const float d = cur.there ? scale_of(cur, g, edge) : 0.0f;
+                    const uint32_t d2 = pack_f16(d, d);
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const uint4 v = cur.there ? widen<MX>(cur.k[t * NG + g], d2, d2) : make_uint4(0, 0, 0, 0);
-                    const int c = 4 * g + t;
-                    *(uint4 *)(kd + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
+                    for (int t = 0; t < 4; t++) {
+                        const uint4 v = cur.there ? widen<MX>(cur.w[t * NG + g], d2, d2) : make_uint4(0, 0, 0, 0);
+                        const int c = 4 * g + t;
+                        *(uint4 *)(dst + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
+                    }
                 }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            bar_arrive(&s.k_full[b]);
-            if (j >= 2) ok = warp_wait(&s.v_empty[b], (j / 2 - 1) & 1) && ok;
+            } else {
 #pragma unroll
-            for (int q2 = 0; q2 < NG / 2; q2++) {
-                const float d0 = cur.there ? scale_of(cur.vs, 2 * q2, v_up, edge) : 0.0f, d1 = cur.there ? scale_of(cur.vs, 2 * q2 + 1, v_up, edge) : 0.0f;
-                const uint32_t s0 = MX ? pack_f16(d0, d0) : pack_f16(d0, d1), s1 = pack_f16(d1, d1);
+                for (int q2 = 0; q2 < NG / 2; q2++) {
+                    const float d0 = cur.there ? scale_of(cur, 2 * q2, edge) : 0.0f, d1 = cur.there ? scale_of(cur, 2 * q2 + 1, edge) : 0.0f;
+                    const uint32_t s0 = MX ? pack_f16(d0, d0) : pack_f16(d0, d1), s1 = pack_f16(d1, d1);
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    const int c = g * (NG / 2) + q2;
-                    const uint4 v = cur.there ? widen<MX>(cur.v[c], s0, s1) : make_uint4(0, 0, 0, 0);
-                    *(uint4 *)(vd + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
-                }
-            }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            bar_arrive(&s.v_full[b]);
-            cur = next;
-        }
-    } else if (warp == kSoftWarps + kWideWarps) {
-        // ---- the products
-        if (lane == 0 && steps) {
-            constexpr uint32_t base = 1u << 4 | (kRows / 16) << 24;         // f32 accumulators, f16 operands, M 128
-            constexpr uint32_t qk = base | (kStep / 8) << 17, pv = base | (DP / 8) << 17 | 1u << 16;   // N; bit 16: b runs along N
-            auto score = [&](int j, int t) {
-                const uint32_t qa = smem_u32(s.q[t]), ka = smem_u32(s.k[j & 1]);
-#pragma unroll
-                for (int c = 0; c < DP / 16; c++) {
-                    const uint32_t off = c / 4 * (kRows * 128) + c % 4 * 32;
-                    mma_ss(tmem + t * 128, operand(qa + off, 16), operand(ka + off, 16), qk, c > 0);
-                }
-                tc_commit(&s.s_full[t]);
-            };
-            ok = bar_wait(&s.k_full[0], 0);
-            tc_after();
-            for (int t = 0; t < tiles && ok; t++) score(0, t);
-            if (ok) tc_commit(&s.k_empty[0]);
-            for (int j = 0; j < steps && ok; j++) {
-                for (int t = 0; t < tiles && ok; t++) {
-                    if (t == 0) ok = bar_wait(&s.v_full[j & 1], j / 2 & 1);
-                    ok = ok && bar_wait(&s.p_full[t], j & 1);
-                    if (!ok) break;
-                    tc_after();
-                    const uint32_t va = smem_u32(s.v[j & 1]);
-#pragma unroll
-                    for (int c = 0; c < kStep / 16; c++)
-                        mma_ts(tmem + 256 + t * DP, tmem + t * 128 + c * 8, operand(va + c * 2048, kRows * 128), pv, j > 0 || c > 0);
-                    tc_commit(&s.pv_done[t]);
-                    if (t == tiles - 1) tc_commit(&s.v_empty[j & 1]);
-                    if (j + 1 < steps) {
-                        if (t == 0) {
-                            ok = bar_wait(&s.k_full[(j + 1) & 1], (j + 1) / 2 & 1);
-                            tc_after();
-                        }
-                        if (ok) {
-                            score(j + 1, t);
-                            if (t == tiles - 1) tc_commit(&s.k_empty[(j + 1) & 1]);
-                        }
+                    for (int g = 0; g < 8; g++) {
+                        const int c = g * (NG / 2) + q2;
+                        const uint4 v = cur.there ? widen<MX>(cur.w[c], s0, s1) : make_uint4(0, 0, 0, 0);
+                        *(uint4 *)(dst + c / 8 * (kRows * 128) + ((c % 8 ^ sw) << 4)) = v;
                     }
                 }
             }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            bar_arrive(values ? &s.v_full[b] : &s.k_full[b]);
+            cur = next;
         }
-        ok = __shfl_sync(0xffffffffu, (int)ok, 0);
+    } else if (warp >= kSoftWarps + kWideWarps) {
+        // ---- the products of tile t
+        const uint32_t t = __shfl_sync(0xffffffffu, warp - kSoftWarps - kWideWarps, 0);
+        if (steps && t < tiles) {
+            const uint32_t lead = elect_one(), nh = __shfl_sync(0xffffffffu, halves, 0);
+            constexpr uint32_t base = 1u << 4 | (kRows / 16) << 24;         // f32 accumulators, f16 operands, M 128
+            constexpr uint32_t qk = base | (kHalf / 8) << 17, pv = base | (DP / 8) << 17 | 1u << 16;   // N; bit 16: b runs along N
+            constexpr uint32_t kBlock = kRows * 128 >> 4, kHalfRows = kHalf * 128 >> 4, kTile = S::TILE >> 4;   // in the operands' units
+            const uint32_t q0 = operand(smem_u32(s.q), 16), k0 = operand(smem_u32(s.k), 16), v0 = operand(smem_u32(s.v), kRows * 128);
+            const uint32_t s_bar = smem_u32(s.s_full), pv_bar = smem_u32(s.pv_done), ke_bar = smem_u32(s.k_empty), ve_bar = smem_u32(s.v_empty);
+            // Half u's scores, two halves ahead of the softmax. All of tensor memory is this CTA's: it begins at 0.
+            auto score = [&](uint32_t u) {
+                const uint32_t qa = q0 + t * kTile, ka = k0 + (u / 2 & 1) * kTile + (u & 1) * kHalfRows, d = t * 128 + (u & 1) * kHalf;
+#pragma unroll
+                for (int c = 0; c < DP / 16; c++) mma_ss(lead, d, qa + c / 4 * kBlock + c % 4 * 2, ka + c / 4 * kBlock + c % 4 * 2, qk, c > 0);
+                tc_commit(lead, s_bar + (t * 2 + (u & 1)) * 8);
+                if (u & 1 || u == nh - 1) tc_commit(lead, ke_bar + (u / 2 & 1) * 8);
+            };
+            ok = tmem == 0 && warp_wait(&s.k_full[0], 0);
+            tc_after();
+            for (uint32_t u = 0; u < min(2u, nh) && ok; u++) score(u);
+            for (uint32_t u = 0; u < nh && ok; u++) {
+                if (!(u & 1)) ok = warp_wait(&s.v_full[u / 2 & 1], u / 4 & 1);
+                ok = ok && warp_wait(&s.p_full[t][u & 1], u / 2 & 1);
+                if (!ok) break;
+                tc_after();
+                const uint32_t va = v0 + (u / 2 & 1) * kTile + (u & 1) * kHalfRows, pa = t * 128 + (u & 1) * kHalf;
+#pragma unroll
+                for (int c = 0; c < kHalf / 16; c++) mma_ts(lead, 256 + t * DP, pa + c * 8, va + c * (2048 >> 4), pv, u > 0 || c > 0);
+                tc_commit(lead, pv_bar + t * 8);
+                if (u & 1 || u == nh - 1) tc_commit(lead, ve_bar + (u / 2 & 1) * 8);
+                if (u + 2 >= nh) continue;
+                if (!(u & 1)) ok = warp_wait(&s.k_full[(u + 2) / 2 & 1], (u + 2) / 4 & 1);
+                ok = ok && warp_wait(&s.pv_done[t], u & 1);                  // S of half u + 2 takes the columns of P of half u
+                if (!ok) break;
+                tc_after();
+                score(u + 2);
+            }
+        }
     } else if (tile < tiles) {
         // ---- softmax: thread = row
         const uint32_t mine = tmem + tile * 128 + ((uint32_t)(warp & 3) << 21);     // lane 32 * (warp % 4) in the upper half
         const uint32_t mine_o = tmem + 256 + tile * DP + ((uint32_t)(warp & 3) << 21);
         const float mult = scale2(p.a.scale * 1.4426950408889634f, -up - k_up);
-        float ref = kFloorRef, sum = 0.0f;
+        float ref = 0.0f, sum = 0.0f;
+        bool fresh = true;                                                   // the row has seen nothing yet
         const int low = p.a.window ? at - p.a.window + 1 : 0;
-        for (int j = 0; j < steps && ok; j++) {
-            ok = warp_wait(&s.s_full[tile], j & 1);
+        for (int u = 0; u < halves && ok; u++) {
+            ok = warp_wait(&s.s_full[tile][u & 1], u / 2 & 1);
             if (!ok) break;
             tc_after();
-            const int tok0 = t0 + j * kStep;
-            const uint32_t *bad = s.bad[j & 3];
-            const bool edge = tok0 < whole_lo || tok0 + kStep > whole_hi || (bad[0] | bad[1] | bad[2] | bad[3]);
-            uint32_t sc[2][32];
-            tmem_load32(sc[0], mine);
+            const int tok0 = t0 + u * kHalf;
+            const uint32_t here = mine + (u & 1) * kHalf;
+            const uint32_t bad0 = s.bad[u / 2 & 3][u % 2 * 2], bad1 = s.bad[u / 2 & 3][u % 2 * 2 + 1];
+            uint32_t v[64];
+            tmem_load32(v, here);
+            tmem_load32(v + 32, here + 32);
+            tmem_wait_ld<64>(v);
+            float z[64], top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                uint32_t *v = sc[c & 1];
-                tmem_wait_ld<32>(v);
-                if (c < 3) tmem_load32(sc[(c + 1) & 1], mine + 32 * (c + 1));
-                float z[32], high = kFloorRef;
-                if (edge) {
-                    const uint32_t miss = bad[c];
-                    const int a = tok0 + 32 * c;
+            for (int i = 0; i < 64; i += 2) fma_two(z + i, __uint_as_float(v[i]), __uint_as_float(v[i + 1]), mult, -ref);
+            if (tok0 < whole_lo || tok0 + kHalf > whole_hi || (bad0 | bad1)) {
+                // the tokens of this half that the row sees
+                const int from = low - tok0, to = at - tok0;
+                unsigned long long seen = ~((unsigned long long)bad1 << 32 | bad0);
+                seen &= to < 0 ? 0ull : to > 62 ? ~0ull : (2ull << to) - 1ull;
+                seen &= from > 63 ? 0ull : from < 1 ? ~0ull : ~0ull << from;
+                const uint32_t lo32 = (uint32_t)seen, hi32 = (uint32_t)(seen >> 32);
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const bool seen = a + i <= at && a + i >= low && !(miss >> i & 1);
-                        z[i] = seen ? fmaf(__uint_as_float(v[i]), mult, -ref) : -INFINITY;
-                        high = fmaxf(high, z[i]);
-                    }
-                } else {
+                for (int i = 0; i < 64; i++) z[i] = (i < 32 ? lo32 >> i : hi32 >> (i - 32)) & 1 ? z[i] : -INFINITY;
+            }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        z[i] = fmaf(__uint_as_float(v[i]), mult, -ref);
-                        high = fmaxf(high, z[i]);
-                    }
-                }
-                if (__any_sync(0xffffffffu, high > 14.0f)) {
-                    // Rows whose reference is passed: a new one, an integer, 10 below the chunk's largest
-                    float m = -INFINITY;
-#pragma unroll
-                    for (int i = 0; i < 32; i++)
-                        if (z[i] != -INFINITY) m = fmaxf(m, __uint_as_float(v[i]) * mult);
-                    float f = 1.0f;
-                    if (high > 14.0f) {
-                        const float to = ceilf(m) - 10.0f;
-                        f = ex2(ref - to);
-                        ref = to;
-                    }
-                    sum *= f;
-                    if (j > 0) {
-                        ok = warp_wait(&s.pv_done[tile], (j - 1) & 1) && ok;
-                        tc_after();
+            for (int i = 0; i < 64; i += 2) top[i / 2 % 4] = max3(top[i / 2 % 4], z[i], z[i + 1]);
+            const float high = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+            const bool move = high > 14.0f || (fresh && high > -INFINITY);
+            if (__any_sync(0xffffffffu, move)) {
+                // Rows whose reference is passed: a new one, a whole number above the old, 10 below the largest
+                float by = 0.0f;
+                if (move) by = ceilf(high) - 10.0f;
+                const float f = fresh ? 1.0f : ex2(-by);
+                ref += by;
+                fresh = fresh && !move;
+                sum *= f;
+                if (u > 0) {
+                    ok = warp_wait(&s.pv_done[tile], (u - 1) & 1) && ok;
+                    tc_after();
 #pragma unroll 1
-                        for (int d = 0; d < DP; d += 16) {
-                            uint32_t o[16];
-                            tmem_load16(o, mine_o + d);
-                            tmem_wait_ld<16>(o);
-#pragma unroll
-                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            tmem_store16(mine_o + d, o);
-                        }
-                    }
-                    const uint32_t f2 = pack_f16(f, f);
-#pragma unroll 1
-                    for (int d = 0; d < c; d++) {                            // this step's P so far
+                    for (int d = 0; d < DP; d += 16) {
                         uint32_t o[16];
-                        tmem_load16(o, mine + 16 * d);
+                        tmem_load16(o, mine_o + d);
                         tmem_wait_ld<16>(o);
 #pragma unroll
-                        for (int i = 0; i < 16; i++) o[i] = mul2(o[i], f2);
-                        tmem_store16(mine + 16 * d, o);
+                        for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_store16(mine_o + d, o);
                     }
-#pragma unroll
-                    for (int i = 0; i < 32; i++) z[i] = z[i] == -INFINITY ? -INFINITY : fmaf(__uint_as_float(v[i]), mult, -ref);
                 }
-                uint32_t pr[16];
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float e0 = ex2(z[2 * i]), e1 = ex2(z[2 * i + 1]);
-                    sum += e0 + e1;
-                    pr[i] = pack_f16(e0, e1);
-                }
-                tmem_store16(mine + 16 * c, pr);
+                for (int i = 0; i < 64; i++) z[i] -= by;
             }
+            float part[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < 32; i++) {
+                const float e0 = ex2(z[2 * i]), e1 = ex2(z[2 * i + 1]);
+                add_two(part + i % 2 * 2, e0, e1);
+                v[i] = pack_f16(e0, e1);
+            }
+            sum += part[0] + part[1] + (part[2] + part[3]);
+            tmem_store16(here, v);
+            tmem_store16(here + 16, v + 16);
             tmem_wait_st();
             tc_before();
-            bar_arrive(&s.p_full[tile]);
+            bar_arrive(&s.p_full[tile][u & 1]);
         }
         // ---- the rows' results
-        if (steps) ok = warp_wait(&s.pv_done[tile], (steps - 1) & 1) && ok;
+        if (halves) ok = warp_wait(&s.pv_done[tile], (halves - 1) & 1) && ok;
         tc_after();
         const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
         __nv_bfloat16 *dst = (__nv_bfloat16 *)p.a.out + (size_t)(start + qi) * p.a.out_ld + (size_t)head * p.c.dim;
