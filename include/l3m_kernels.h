@@ -194,7 +194,8 @@ L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, 
 // Causal attention of a batch over the cache: request r's queries are rows q_start[r] .. q_start[r+1) of q, the
 // newest tokens of its kv_len[r] cached ones (kv_total of the plan, after l3m_qkv_rope_dev stored them). The query at position p sees
 // positions 0 .. p, with a window only those above p - window. A query that sees nothing (kv_len 0) gets
-// zeros; rows outside q_start's range stay as they were. Positions in pages with an id outside the cache are not seen. out may not overlap q.
+// zeros; rows outside q_start's range stay as they were. Positions in pages with an id outside the cache are not seen. Scales that are
+// not finite (the store writes none) leave queries alone that do not see them; what sees them is not defined. out may not overlap q.
 typedef struct {
     int   dtype;                 // of q and out: L3M_DT_F32 or L3M_DT_BF16
     int   n_heads;               // a multiple of n_kv_heads: query head h reads kv head h / (n_heads / n_kv_heads)

@@ -514,6 +514,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             bar_arrive(&s.p_full[tile][u & 1]);
         }
         // ---- the rows' results
+        // (the last half's scores said that the products of the third last half were done: the two behind it one by one,
+        // a wait for a phase two ahead would pass at once)
+        if (halves > 1) ok = warp_wait(&s.pv_done[tile], (halves - 2) & 1) && ok;
         if (halves) ok = warp_wait(&s.pv_done[tile], (halves - 1) & 1) && ok;
         tc_after();
         const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
