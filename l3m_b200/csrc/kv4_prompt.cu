@@ -507,6 +507,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 v[i] = pack_f16(e0, e1);
             }
             sum += part[0] + part[1] + (part[2] + part[3]);
+            if (u > 0 && u == halves - 1) {
+                // The products before the last, while the last wait for this warp's P: a parity tells one phase from the next, not from the one behind that
+                ok = warp_wait(&s.pv_done[tile], (u - 1) & 1) && ok;
+            }
             tmem_store16(here, v);
             tmem_store16(here + 16, v + 16);
             tmem_wait_st();
@@ -514,9 +518,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             bar_arrive(&s.p_full[tile][u & 1]);
         }
         // ---- the rows' results
-        // (the last half's scores said that the products of the third last half were done: the two behind it one by one,
-        // a wait for a phase two ahead would pass at once)
-        if (halves > 1) ok = warp_wait(&s.pv_done[tile], (halves - 2) & 1) && ok;
         if (halves) ok = warp_wait(&s.pv_done[tile], (halves - 1) & 1) && ok;
         tc_after();
         const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
