@@ -241,11 +241,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         return id >= 0 && id < p.c.n_pages ? p.c.data + p.c.tile_at(id, h, off / kKvTile) : nullptr;
     };
 
-    // ---- the largest scales' exponents
-    {
+    // ---- the largest scales' exponents, while the softmax's warps bring in the queries
+    if (warp >= kSoftWarps) {
         int kt = 0, vt = 0;
-#pragma unroll 4
-        for (int tok = lo_any + tid; tok < hi_any; tok += kPromptThreads) {
+#pragma unroll 8
+        for (int tok = lo_any + tid - 32 * kSoftWarps; tok < hi_any; tok += kPromptThreads - 32 * kSoftWarps) {
             const uint8_t *tile = tile_of(tok);
             if (!tile) continue;
             const int row = tok % p.c.page % kKvTile;
