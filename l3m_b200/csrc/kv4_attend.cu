@@ -1034,7 +1034,7 @@ extern "C" {
 
 L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend *a) {
     if (attend_error(cache, a)) return 0;
-    if (a->max_kv <= kSplitFrom) return 16;
+    if (a->max_kv <= kSplitFrom || prompt_fits(cache, a)) return 16;
     const int ng = (cache->head_dim + kKvBlock - 1) / kKvBlock, nt = row_blocks(cache, a);
     return (size_t)kMaxSms * ctas_per_sm(ng, nt) * (2 * sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
 }

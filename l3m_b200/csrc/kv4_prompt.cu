@@ -1,5 +1,5 @@
 // Attention of prompt chunks over the paged 4-bit cache on the fifth-generation tensor cores: the variant of
-// l3m_kv4_attend_dev for many query rows per key/value head (the rule is prompt_fits() below). bf16 queries and
+// l3m_kv4_attend_dev for thousands of query rows (the rule is prompt_fits() below). bf16 queries and
 // results, head dims of 2 or 4 blocks.
 //
 // One CTA takes 256 rows (query, head of the group) of one request and kv head, as two tiles of 128, over the whole
@@ -7,7 +7,7 @@
 //   8 warps  widen a step's codes to f16 in shared memory, 4 the keys (K-major), 4 the values (as they lie, MN-major), swizzled
 //            by 128 bytes, two buffers each, the next step's codes under way in registers;
 //   2 warps  issue the products, one for each tile: S = Q K^T (both operands in shared memory) and O += P V (P in tensor
-//            memory); by one warp for both, its waits and issues were the longest chain (238 us against what stands in the table);
+//            memory); one warp for both was the longest chain;
 //   8 warps  one thread a row: S from tensor memory, softmax against the row's reference, P back as f16 over S's columns.
 // S has two halves of 64 tokens a tile, so that the next half's scores are formed while one goes through the softmax, and the two
 // tiles alternate. Tensor memory: S (then P) of tile t, half u at columns 128 t + 64 u, O of tile t at 256 + t * head_dim: all 512
@@ -28,6 +28,7 @@
 namespace l3m {
 namespace {
 
+constexpr int kSms = 148;
 constexpr int kRows = 128, kStep = 128, kHalf = 64;     // rows of a tile, tokens that are widened at a time, tokens of a product
 constexpr int kSoftWarps = 8, kWideWarps = 8;          // half of the latter for keys, half for values
 constexpr int kPromptThreads = 32 * (kSoftWarps + kWideWarps + 2);
@@ -205,7 +206,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
     const int r = x / per_req, h = (x - r * per_req) / p.row_tiles, rt = p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles);
     const int start = p.a.q_start[r], nq = p.a.q_start[r + 1] - start, kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
-    const int row0 = rt * 2 * kRows, rows = nq * p.group - row0;           // rows left from this CTA's first
+    const int row0 = rt * 2 * kRows, rows = min(nq, p.a.max_q) * p.group - row0;           // rows left from this CTA's first
     if (rows <= 0) return;
     const int tiles = rows > kRows ? 2 : 1;
     const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = kv - nq + i0, last = kv - nq + i1;   // the rows' positions
@@ -588,18 +589,19 @@ cudaError_t launch(const PromptArgs &p, cudaStream_t s) {
     return cudaLaunchKernelEx(&cfg, prompt_kernel<NG, MX>, p);
 }
 
-long long prompt_ctas(const l3m_kv4 *c, const l3m_kv4_attend *a) {
-    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
-    return (rows + 2 * kRows - 1) / (2 * kRows) * a->n_req * c->n_kv_heads;
-}
-
 }  // namespace
 
+// When: a CTA here takes as long for one row as for 256, and the CTAs run in waves of one an SM; the kernel of kv4_attend.cu takes time by
+// the row, whichever request or head it is of. Measured, contexts of 512 to 16384, the rows at which both take as long:
+// 5300 to 7600 a wave at a head dim of 128, 10000 to 13700 at 64. At 16384 tokens, 8 kv heads and 128 dims: 1024 rows a head of one request 393 us here and
+// 525 there, of 8 requests 789 and 3988; 256 rows of 2 requests 395 and 278, of one 391 and 151.
 bool prompt_fits(const l3m_kv4 *c, const l3m_kv4_attend *a) {
     const int ng = (c->head_dim + kKvBlock - 1) / kKvBlock;
-    if (a->dtype != L3M_DT_BF16 || (ng != 2 && ng != 4)) return false;
-    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
-    return rows >= 96 && prompt_ctas(c, a) >= 32 && prompt_ctas(c, a) < 0x7fffffff;
+    if (a->dtype != L3M_DT_BF16 || (ng != 2 && ng != 4) || a->n_req > 1 << 20) return false;
+    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads), lines = (long long)a->n_req * c->n_kv_heads;
+    if (rows >= 1 << 24 || lines >= 1 << 30) return false;
+    const long long ctas = (rows + 2 * kRows - 1) / (2 * kRows) * lines, waves = (ctas + kSms - 1) / kSms;
+    return rows && lines && ctas < 0x7fffffff && rows * lines >= waves * (ng == 4 ? 6400 : 12500);
 }
 
 cudaError_t prompt_attend(const l3m_kv4 *c, const l3m_kv4_attend *a, cudaStream_t s) {

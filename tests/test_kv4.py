@@ -127,3 +127,16 @@ def test_scratch_size(lib):
     assert lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend())) >= 16
     assert lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend(n_heads=3))) == 0
     assert lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend(q=None, out=None, scratch=None, scratch_bytes=0))) >= 16
+
+
+def test_scratch_size_of_prompt_chunks(lib):
+    """Long contexts need scratch for their split, but for bf16 chunks of thousands of rows at 33 .. 64 and 97 .. 128 dims, which are not split."""
+    def size(dim, **kw):
+        c = cache(head_dim=dim, n_kv_heads=4)
+        return lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend(**dict(dict(n_heads=16, dtype=1, n_req=4, max_q=1024, max_blocks=4096, max_kv=65536), **kw))))
+    assert size(128) == size(104) == size(64) == size(40) == 16
+    for kw in (dict(dtype=0), dict(max_q=8), dict(n_req=1, max_q=256)):
+        assert size(128, **kw) > 16
+    assert size(96) > 16 and size(32) > 16 and size(136) > 16
+    assert size(128, n_req=1 << 21) > 16 and size(128, max_q=1 << 30) > 16
+    assert size(128, max_q=0) > 16 and size(128, n_req=0) > 16
