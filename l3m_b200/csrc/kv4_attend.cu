@@ -123,20 +123,21 @@ __device__ __forceinline__ float load_f32(const __nv_bfloat16 *p) { return __bfl
 __device__ __forceinline__ void store_f32(float *p, float x) { *p = x; }
 __device__ __forceinline__ void store_f32(__nv_bfloat16 *p, float x) { *p = __float2bfloat16_rn(x); }
 
-constexpr int kWarps = 6, kThreads = 32 * kWarps;
 constexpr int kStages = 4;               // tiles of a warp's ring: two pairs
 constexpr int kMaxSms = 160;
 constexpr float kFloor = -1e30f;         // the reference of a row that has seen nothing
 
-// Resident CTAs per SM that the registers of a variant allow.
-constexpr int ctas_per_sm(int ng, int nt) { return ng * nt <= 5 ? 2 : 1; }
+constexpr int kCtas = 2;                 // resident CTAs per SM
+// Warps of a CTA: as many as the registers of a variant allow: 12 on an SM at 166 each, 8 at 255. (Of the latter, one CTA of 6 warps
+// took 103 us where two of 4 take 81, one of 4 108: 32 requests of 1000 tokens, 5 queries each, f32, 32 heads to 8 of 128.)
+constexpr int warps_of(int ng, int nt) { return ng * nt <= 5 ? 6 : 4; }
 
 struct Segment { int r, h, rt; };
 
 // One piece of a segment (request r, kv head h, row tile rt): cache tiles [a, b), by the CTA's warps. Scores are
 // computed transposed, S^T = K Q^T (16 tokens x 8 rows a product), so that a decode step's few rows pad to 8, not 16, and
 // O^T = V^T P^T follows from it with one 8x8 transposition per 8 tokens. Each warp keeps its own softmax reference and
-// sums over its tiles a + warp, a + warp + 4, ...; the warps are joined at the end.
+// sums over its pairs of tiles, every kWarps-th of the piece; the warps are joined at the end.
 //
 // Codes go into the products as the integers they are, so that the cache's values suffer no rounding. For q4_0 and bf16 results a
 // nibble in the low byte of a half is an f16 subnormal, n * 2^-24 (or n * 2^-20 four bits higher): one mask, no conversion. Its offset
@@ -147,6 +148,7 @@ struct Segment { int r, h, rt; };
 // split in two f16 for float ones.
 template <typename T, int MX, int NG, int NT>
 struct Worker {
+    static constexpr int kWarps = warps_of(NG, NT), kThreads = 32 * kWarps;
     static constexpr bool PREC = sizeof(T) == 4;
     static constexpr bool SUBN = !PREC && !MX;
     static constexpr int NR = 8 * NT, DP = 32 * NG, SB = MX ? 1 : 2;
@@ -623,7 +625,7 @@ struct Worker {
         const int lo_any = p.a.window ? first - p.a.window + 1 : 0, hi_any = last + 1;
         const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;   // seen by every row
         uint8_t *ring = smem + warp * RING;
-        const int pairs = (b - a + 1) / 2, n = warp < pairs ? (pairs - warp + kWarps - 1) / kWarps : 0;      // this warp's pairs of tiles: warp, warp + 4, ...
+        const int pairs = (b - a + 1) / 2, n = warp < pairs ? (pairs - warp + kWarps - 1) / kWarps : 0;      // this warp's pairs of tiles: warp, warp + kWarps, ...
         int where = -1;                                                      // lane i: the number in the cache of tile i % 2 of pair 16 * (k / 16) + i / 2
         auto locate = [&](int k) {
             const int tl = a + 2 * (warp + (k + lane / 2) * kWarps) + lane % 2;
@@ -761,7 +763,7 @@ __device__ __forceinline__ Request request_of(const AttendArgs &p, int r, int nr
     return q;
 }
 
-__device__ long long block_sum_scan(long long v, long long *ws, long long *total) {
+template <int kWarps> __device__ long long block_sum_scan(long long v, long long *ws, long long *total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int o = 1; o < 32; o <<= 1) {
         const long long u = __shfl_up_sync(0xffffffffu, v, o);
@@ -780,8 +782,9 @@ __device__ long long block_sum_scan(long long v, long long *ws, long long *total
 }
 
 template <typename T, int MX, int NG, int NT>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(const __grid_constant__ AttendArgs p) {
+__global__ void __launch_bounds__(32 * warps_of(NG, NT), kCtas) attend_kernel(const __grid_constant__ AttendArgs p) {
     typedef Worker<T, MX, NG, NT> W;
+    constexpr int kWarps = W::kWarps, kThreads = W::kThreads;
     extern __shared__ __align__(16) uint8_t smem[];
     W w(p, smem);
     const int n_req = p.a.n_req, heads = p.c.n_kv;
@@ -804,7 +807,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
                 const Request q = request_of(p, i, W::NR);
                 n = (long long)q.tiles * q.rts * heads;
             }
-            block_sum_scan(n, ws, &sum);
+            block_sum_scan<W::kWarps>(n, ws, &sum);
             total += sum;
         }
         share = (total + gridDim.x - 1) / gridDim.x;
@@ -819,7 +822,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(NG, NT)) attend_kernel(c
                 const Request q = request_of(p, i, W::NR);
                 n = (long long)q.tiles * q.rts * heads;
             }
-            const long long upto = base + block_sum_scan(n, ws, &sum);
+            const long long upto = base + block_sum_scan<W::kWarps>(n, ws, &sum);
             if (upto - n <= u0 && u0 < upto) {
                 found = i;
                 found_at = upto - n;
@@ -971,11 +974,11 @@ cudaError_t launch(AttendArgs p, cudaStream_t s) {
     typedef Worker<T, MX, NG, NT> W;
     cudaError_t e = cudaFuncSetAttribute(attend_kernel<T, MX, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, W::SMEM);
     if (e != cudaSuccess) return e;
-    const int workers = sm_count() * ctas_per_sm(NG, NT);
+    const int workers = sm_count() * kCtas;
     p.row_tiles = (int)(((long long)p.a.max_q * p.group + W::NR - 1) / W::NR);
     p.split = p.a.max_kv > kSplitFrom ? kLeastShare : 0;
     p.desc = (int4 *)p.a.scratch;
-    p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * ctas_per_sm(NG, NT) * 2 * sizeof(int4));
+    p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * kCtas * 2 * sizeof(int4));
     const long long segs = (long long)p.a.n_req * p.c.n_kv * p.row_tiles;
     const int grid = p.split ? workers : (int)std::min<long long>(segs, 1 << 20);
     // Both launches are programmatic: their CTAs may come up while what precedes them drains, and wait for it.
@@ -984,7 +987,7 @@ cudaError_t launch(AttendArgs p, cudaStream_t s) {
     early.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
-    cfg.blockDim = dim3(kThreads);
+    cfg.blockDim = dim3(W::kThreads);
     cfg.dynamicSmemBytes = W::SMEM;
     cfg.stream = s;
     cfg.attrs = &early;
@@ -1036,7 +1039,7 @@ L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend
     if (attend_error(cache, a)) return 0;
     if (a->max_kv <= kSplitFrom || prompt_fits(cache, a)) return 16;
     const int ng = (cache->head_dim + kKvBlock - 1) / kKvBlock, nt = row_blocks(cache, a);
-    return (size_t)kMaxSms * ctas_per_sm(ng, nt) * (2 * sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
+    return (size_t)kMaxSms * kCtas * (2 * sizeof(int4) + part_floats(8 * nt, ng) * sizeof(float));
 }
 
 L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, void *stream) {
