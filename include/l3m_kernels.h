@@ -121,7 +121,7 @@ L3M_API int l3m_chain_cycles_dev(int steps, double *cycles_per_step);
 typedef struct {
     void *data;                  // n_pages * l3m_kv4_page_bytes() bytes of device memory, 16-byte aligned
     int   dtype;                 // L3M_DT_Q4_0 or L3M_DT_MXFP4
-    int   n_pages;               // n_pages * page < 2^31
+    int   n_pages;               // n_pages * page < 2^31, n_pages * n_kv_heads * page / 16 < 2^31
     int   page;                  // tokens per page, a multiple of 16, at most 4096
     int   n_kv_heads, head_dim;  // head_dim a multiple of 8, 8 .. 256
 } l3m_kv4;
@@ -130,9 +130,9 @@ L3M_API size_t l3m_kv4_page_bytes(int dtype, int n_kv_heads, int head_dim, int p
 // Bits that the calls below OR into their *status (device memory, NULL: not reported). The caller zeroes it.
 enum {
     L3M_KV4_NO_PAGES = 1,        // plan: the free list ran out
-    L3M_KV4_BAD_LENGTH = 2,      // plan: a negative kv_len, a length beyond max_blocks * page, or a bad n_free
+    L3M_KV4_BAD_LENGTH = 2,      // plan: a negative kv_len, a length beyond max_blocks * page or 2^31 - page, or a bad n_free
     L3M_KV4_NO_ROOM = 4,         // plan: more new tokens than max_tokens
-    L3M_KV4_BAD_PAGE = 8,        // a page id or slot outside the cache was left out
+    L3M_KV4_BAD_PAGE = 8,        // a page id or slot outside the cache was left out (plan: slot -1)
     L3M_KV4_BAD_POS = 16,        // qkv: a position outside the rotation table; its row was left out
     L3M_KV4_TIMEOUT = 32,        // attend: a wait inside the kernel gave up; the rows concerned are NaN
 };
@@ -148,7 +148,7 @@ enum {
 typedef struct {
     int n_req;                   // 0 .. 16384
     int max_blocks;              // entries of a table row
-    int max_tokens;              // entries of slot and pos
+    int max_tokens;              // entries of slot and pos, at most 2^30
     int page, n_pages;
     const int32_t *kv_len, *new_len;
     int32_t *tables;             // [n_req][max_blocks]
@@ -200,10 +200,10 @@ typedef struct {
     int   dtype;                 // of q and out: L3M_DT_F32 or L3M_DT_BF16
     int   n_heads;               // a multiple of n_kv_heads: query head h reads kv head h / (n_heads / n_kv_heads)
     int   n_req, max_blocks;
-    int   max_q;                 // at least every request's number of queries
+    int   max_q;                 // at least every request's number of queries (more are not looked at); max_q * n_heads <= 2^30
     int   max_kv;                // at least every kv_len; at most max_blocks * page
     int   window;                // 0: none
-    float scale;                 // of the scores, finite
+    float scale;                 // of the scores, below 2^127 in magnitude
     const void *q;
     void *out;
     int64_t q_ld, out_ld;        // elements from token to token

@@ -72,7 +72,7 @@ __device__ int last_not_above(const int *a, int n, int x) {
 }
 
 __device__ __forceinline__ bool bad_lengths(const l3m_kv4_plan &a, long long kv, long long count) {
-    return kv < 0 || (kv + count + a.page - 1) / a.page > a.max_blocks || kv + count > 0x7fffffff;
+    return kv < 0 || (kv + count + a.page - 1) / a.page > a.max_blocks || kv + count + a.page > 0x7fffffff;
 }
 
 // Every CTA sums the requests' lengths for itself (a few microseconds at most: they fit one SM's
@@ -178,7 +178,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(const __grid_constan
                 pos = kv + (t - start[r]);
                 const int block = pos / a.page;
                 const int id = block < held ? a.tables[(size_t)r * a.max_blocks + block] : popped(used[r] + block - held);
-                slot = id * a.page + (pos - block * a.page);
+                if (id >= 0 && id < a.n_pages) slot = id * a.page + (pos - block * a.page);
+                else if (a.status) atomicOr((int *)a.status, L3M_KV4_BAD_PAGE);
             }
         }
         a.pos[t] = pos;
@@ -740,6 +741,7 @@ L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream) {
     if (!a) return refuse(me, "arguments are required");
     if (a->n_req < 0 || a->n_req > kPlanMaxReq) return refuse(me, "n_req must be 0 to 16384");
     if (a->page < kKvTile || a->page > 4096 || a->page % kKvTile) return refuse(me, "page must be a multiple of 16 from 16 to 4096");
+    if (a->max_tokens > 1 << 30) return refuse(me, "max_tokens must be at most 2^30");
     if (a->max_blocks < 0 || a->max_tokens < 0 || a->n_pages < 0 || (int64_t)a->n_pages * a->page > 0x7fffffff)
         return refuse(me, "max_blocks, max_tokens and n_pages must not be negative, n_pages * page below 2^31");
     if (!a->n_free || !a->n_free_out || !a->q_start || (a->n_pages && !a->free_pages) || (a->max_tokens && (!a->slot || !a->pos)) ||
@@ -784,7 +786,7 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
         return refuse(me, "a token stride is smaller than its heads");
     const uintptr_t mask = a->dtype == L3M_DT_F32 ? 3 : 1;
     if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out | (uintptr_t)a->k_out) & mask) ||
-        (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm | (uintptr_t)a->rope_table | (uintptr_t)a->pos | (uintptr_t)a->slot) & 3))
+        (((uintptr_t)a->q_norm | (uintptr_t)a->k_norm | (uintptr_t)a->rope_table | (uintptr_t)a->pos | (uintptr_t)a->slot | (uintptr_t)a->status) & 3))
         return refuse(me, "a pointer is not aligned to its type");
     if (!a->n_heads && !with_k && !with_v) return 0;
     if (a->rope && ((uintptr_t)a->rope_table & 7)) return refuse(me, "rope_table must be 8-byte aligned");

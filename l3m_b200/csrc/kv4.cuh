@@ -43,6 +43,7 @@ inline const char *kv4_shape_error(const l3m_kv4 *c) {
 inline const char *kv4_error(const l3m_kv4 *c) {
     if (const char *e = kv4_shape_error(c)) return e;
     if (!c->data || ((uintptr_t)c->data & 15)) return "the cache's data must be 16-byte aligned device memory";
+    if ((int64_t)c->n_pages * c->n_kv_heads * (c->page / kKvTile) > 0x7fffffff) return "the cache must have fewer than 2^31 tiles";
     return nullptr;
 }
 

@@ -754,7 +754,7 @@ struct Request { int start, nq, kv, lo, tiles, rts; };            // cache tiles
 __device__ __forceinline__ Request request_of(const AttendArgs &p, int r, int nr) {
     Request q;
     q.start = p.a.q_start[r];
-    q.nq = max(p.a.q_start[r + 1] - q.start, 0);
+    q.nq = min(max(p.a.q_start[r + 1] - q.start, 0), p.a.max_q);
     q.kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
     const int lo = p.a.window ? max(0, q.kv - q.nq - p.a.window + 1) : 0;
     q.lo = lo / kKvTile;
@@ -1027,6 +1027,7 @@ const char *attend_error(const l3m_kv4 *c, const l3m_kv4_attend *a) {
     if (a->dtype != L3M_DT_F32 && a->dtype != L3M_DT_BF16) return "dtype must be f32 or bf16";
     if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % c->n_kv_heads) return "n_heads must be a positive multiple of n_kv_heads";
     if (a->n_req < 0 || a->max_blocks < 0 || a->max_q < 0 || a->max_kv < 0 || a->window < 0) return "a count is negative";
+    if ((int64_t)a->max_q * a->n_heads > 1 << 30) return "max_q * n_heads must be at most 2^30";
     if (a->max_kv > (int64_t)a->max_blocks * c->page) return "max_kv must not exceed max_blocks * page";
     return nullptr;
 }
@@ -1046,20 +1047,22 @@ L3M_API int l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, vo
     const char *me = "l3m_kv4_attend_dev";
     if (const char *why = attend_error(cache, a)) return refuse(me, why);
     if (const char *why = kv4_error(cache)) return refuse(me, why);
-    if (!std::isfinite(a->scale)) return refuse(me, "scale must be finite");
+    if (!(std::fabs(a->scale) < 0x1p127f)) return refuse(me, "scale must be finite and below 2^127");
     if (!a->n_req || !a->max_q) return 0;
     if (!a->q || !a->out || !a->q_start || !a->kv_len || (a->max_blocks && !a->tables)) return refuse(me, "a pointer is missing");
     const int64_t width = (int64_t)a->n_heads * cache->head_dim;
     if (a->q_ld < width || a->out_ld < width) return refuse(me, "a token stride is smaller than its heads");
-    if (((uintptr_t)a->q | (uintptr_t)a->out) & (a->dtype == L3M_DT_F32 ? 3 : 1) || ((uintptr_t)a->q_start | (uintptr_t)a->kv_len | (uintptr_t)a->tables) & 3)
+    if (((uintptr_t)a->q | (uintptr_t)a->out) & (a->dtype == L3M_DT_F32 ? 3 : 1) || ((uintptr_t)a->q_start | (uintptr_t)a->kv_len | (uintptr_t)a->tables | (uintptr_t)a->status) & 3)
         return refuse(me, "a pointer is not aligned to its type");
     if (!a->scratch || a->scratch_bytes < l3m_kv4_attend_scratch(cache, a) || ((uintptr_t)a->scratch & 15)) return refuse(me, "scratch is too small or not 16-byte aligned");
-    AttendArgs p = {*a, kv4_dev(cache), a->n_heads / cache->n_kv_heads, 0, 0, nullptr, nullptr};
+    l3m_kv4_attend b = *a;
+    if (b.window >= b.max_kv) b.window = 0;                                  // it leaves nothing out
+    AttendArgs p = {b, kv4_dev(cache), a->n_heads / cache->n_kv_heads, 0, 0, nullptr, nullptr};
     const int mx = cache->dtype == L3M_DT_MXFP4, two = row_blocks(cache, a) == 2;
     const cudaStream_t s = (cudaStream_t)stream;
     cudaError_t e;
     if (prompt_fits(cache, a)) {
-        e = prompt_attend(cache, a, s);
+        e = prompt_attend(cache, &b, s);
     } else if (a->dtype == L3M_DT_F32) {
         if (mx) e = two ? by_blocks<float, 1, 2>(p, s) : by_blocks<float, 1, 1>(p, s);
         else e = two ? by_blocks<float, 0, 2>(p, s) : by_blocks<float, 0, 1>(p, s);

@@ -205,8 +205,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     // ---- what this CTA does: the last rows first, they see most
     const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
     const int r = x / per_req, h = (x - r * per_req) / p.row_tiles, rt = p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles);
-    const int start = p.a.q_start[r], nq = p.a.q_start[r + 1] - start, kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
-    const int row0 = rt * 2 * kRows, rows = min(nq, p.a.max_q) * p.group - row0;           // rows left from this CTA's first
+    const int start = p.a.q_start[r], nq = min(max(p.a.q_start[r + 1] - start, 0), p.a.max_q), kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
+    const int row0 = rt * 2 * kRows, rows = nq * p.group - row0;           // rows left from this CTA's first
     if (rows <= 0) return;
     const int tiles = rows > kRows ? 2 : 1;
     const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = kv - nq + i0, last = kv - nq + i1;   // the rows' positions

@@ -39,7 +39,7 @@ def plan(kv_len, new_len, tables, free_pages, n_free, page, max_tokens):
         kv, count = int(kv_len[r]), max(int(new_len[r]), 0)
         held, after = -(-kv // page), -(-(kv + count) // page)
         q_start[r + 1] = q_start[r] + count
-        bad = kv < 0 or after > width
+        bad = kv < 0 or after > width or kv + count + page > 2 ** 31 - 1
         need = 0 if bad else after - held
         first, wanted = wanted, wanted + need
         status |= BAD_LENGTH if bad else 0
@@ -53,7 +53,9 @@ def plan(kv_len, new_len, tables, free_pages, n_free, page, max_tokens):
         total[r] = kv + count
         for i in range(count):
             pos[q_start[r] + i] = kv + i
-            slot[q_start[r] + i] = tables[r, (kv + i) // page] * page + (kv + i) % page
+            there = 0 <= tables[r, (kv + i) // page] < n_pages
+            slot[q_start[r] + i] = tables[r, (kv + i) // page] * page + (kv + i) % page if there else -1
+            status |= 0 if there else BAD_PAGE
     return dict(tables=tables, free_pages=stack, n_free_out=left, q_start=q_start, kv_total=total, slot=slot, pos=pos, status=status)
 
 

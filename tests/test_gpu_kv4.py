@@ -145,6 +145,16 @@ def test_plan_returning_more_pages_than_the_pool_has(api):
     same_plan(api.plan(kv, new, tables, free, 5, 16, 32), want)
 
 
+def test_plan_leaves_out_pages_that_are_none(api):
+    """Ids outside the cache in a request's own pages or on the free list: their slots are -1, nothing wraps into the cache."""
+    for bad in (6, -3, 1 << 28, -(1 << 31), (1 << 31) - 1):
+        kv, new = np.array([14, 20, 0], np.int32), np.array([3, 2, 20], np.int32)
+        tables, free = np.array([[bad, -1, -1], [3, 4, -1], [-1, -1, -1]], np.int32), np.array([0, 1, bad, 2, 5, 5], np.int32)
+        want = ref.plan(kv, new, tables, free, 5, 16, 30)
+        assert want["status"] == ref.BAD_PAGE and (want["slot"][:2] == -1).all()
+        same_plan(api.plan(kv, new, tables, free, 5, 16, 30), want)
+
+
 def test_plan_of_no_requests(api):
     got = api.plan(np.zeros(0), np.zeros(0), np.zeros((0, 4), np.int32), np.arange(6), 6, 16, 3)
     assert got["n_free_out"] == 6 and list(got["q_start"]) == [0] and list(got["slot"]) == [-1] * 3 and got["status"] == 0
@@ -476,6 +486,20 @@ def test_attend_rows_that_see_nothing_and_rows_of_nobody(api, dtype):
         assert (want[:2] == 0).all() and (want[2:6] == 0).all() and (want[6] != 0).any()
         check_attend(out[:n], want[:n], spread[:n], dtype)
         assert st.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_attend_windows_beyond_everything(api, dtype):
+    """A window as long as the context or as long as an int goes leaves nothing out, for queries before position 0 either."""
+    rng = np.random.default_rng(31)
+    lens, news = [40, 3, 600], [1, 30, 9]
+    tables, q_start, n_pages = batch(rng, lens, news, 16)
+    host = random_cache(rng, ref.Q4, n_pages, 2, 16, 64)
+    q, q64 = queries(api, rng, int(q_start[-1]), 4, 64, dtype)
+    want, spread = ref.attend(q64, q_start, lens, tables, host, ref.Q4, 64, 16, 2, 0.125)
+    for window in (600, 1 << 30, (1 << 31) - 1):
+        out, _ = api.attend(api.cache(api.put(host), ref.Q4, 16, 2, 64), q, q_start, lens, tables, 0.125, window)
+        check_attend(out, want, spread, dtype)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])

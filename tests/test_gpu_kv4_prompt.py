@@ -140,6 +140,17 @@ def test_prompt_rows_that_see_nothing_and_rows_of_nobody(api, cdtype):
     check(out[:n], want[:n], tol[:n])
 
 
+def test_prompt_windows_beyond_everything(api):
+    rng = np.random.default_rng(13)
+    lens, news, heads, kh, dim, page = [200, 50, 333], [130, 140, 128], 40, 40, 64, 16
+    tables, q_start, n_pages = batch(rng, lens, news, page)
+    host = random_cache(rng, ref.Q4, n_pages, kh, page, dim)
+    q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, BF16)
+    want, tol = want_and_tolerance(q64, q_start, lens, tables, host, ref.Q4, dim, page, kh, 0.125)
+    for window in (333, (1 << 31) - 1):
+        check(api.attend(api.cache(api.put(host), ref.Q4, page, kh, dim), q, q_start, lens, tables, 0.125, window)[0], want, tol)
+
+
 @pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
 @pytest.mark.parametrize("window", [0, 21])
 def test_prompt_ignores_what_nobody_sees(api, cdtype, window):

@@ -1,6 +1,7 @@
 """The paged 4-bit cache's entry points on the CPU: sizes, and every refusal (arguments are checked before anything touches a GPU)."""
 import ctypes as C
 
+import numpy as np
 import pytest
 
 import kv4_ref as ref
@@ -42,7 +43,7 @@ def plan(**kw):
 
 
 @pytest.mark.parametrize("change,why", [
-    (dict(n_req=-1), b"n_req"), (dict(n_req=16385), b"n_req"), (dict(page=8), b"page"), (dict(page=40), b"page"), (dict(max_tokens=-1), b"negative"), (dict(max_blocks=-1), b"negative"),
+    (dict(n_req=-1), b"n_req"), (dict(n_req=16385), b"n_req"), (dict(page=8), b"page"), (dict(page=40), b"page"), (dict(max_tokens=-1), b"negative"), (dict(max_tokens=(1 << 30) + 1), b"2^30"), (dict(max_blocks=-1), b"negative"),
     (dict(n_pages=-1), b"negative"), (dict(n_pages=1 << 28), b"2^31")] + [(dict([(f, None)]), b"missing") for f in
     ("kv_len", "new_len", "tables", "free_pages", "n_free", "n_free_out", "q_start", "kv_total", "slot", "pos")] + [
     (dict(n_free_out=64 * 5), b"must not be"), (dict(kv_total=64), b"must not be"), (dict(kv_total=128), b"must not be"), (dict(kv_len=66), b"aligned")])
@@ -63,7 +64,7 @@ def qkv(**kw):
     (dict(rot_dim=63), b"rot_dim"), (dict(rot_dim=66), b"rot_dim"), (dict(rope_table=None), b"table"), (dict(rope_table=68), b"8-byte"), (dict(eps=-1.0), b"eps"), (dict(eps=float("nan")), b"eps"),
     (dict(n_kv_heads=4), b"another"), (dict(head_dim=32, rot_dim=32), b"another"), (dict(k=None), b"needs"), (dict(v=None), b"needs"), (dict(slot=None), b"needs"), (dict(pos=None), b"pos"),
     (dict(q=None), b"q_out"), (dict(q_out=None), b"q_out"), (dict(q_ld=255), b"stride"), (dict(k_ld=127), b"stride"), (dict(v_ld=127), b"stride"), (dict(q_out_ld=255), b"stride"),
-    (dict(k_out_ld=127), b"stride"), (dict(q=66), b"aligned"), (dict(q_norm=66), b"aligned"), (dict(pos=66), b"aligned"), (dict(dtype=1, v=65), b"aligned")])
+    (dict(k_out_ld=127), b"stride"), (dict(q=66), b"aligned"), (dict(q_norm=66), b"aligned"), (dict(pos=66), b"aligned"), (dict(status=66), b"aligned"), (dict(dtype=1, v=65), b"aligned")])
 def test_qkv_refuses(lib, change, why):
     c = cache()
     assert lib.l3m_qkv_rope_dev(C.byref(c), C.byref(qkv(**change)), None) == -1
@@ -84,7 +85,7 @@ def attend(**kw):
 
 @pytest.mark.parametrize("change,why", [
     (dict(dtype=3), b"dtype"), (dict(n_heads=3), b"n_heads"), (dict(n_heads=0), b"n_heads"), (dict(n_req=-1), b"negative"), (dict(max_q=-1), b"negative"), (dict(max_kv=-1), b"negative"),
-    (dict(window=-1), b"negative"), (dict(max_kv=65), b"max_kv"), (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(q=None), b"missing"), (dict(out=None), b"missing"),
+    (dict(window=-1), b"negative"), (dict(max_q=(1 << 28) + 1), b"2^30"), (dict(scale=-3e38), b"scale"), (dict(status=66), b"aligned"), (dict(max_kv=65), b"max_kv"), (dict(scale=float("inf")), b"scale"), (dict(scale=float("nan")), b"scale"), (dict(q=None), b"missing"), (dict(out=None), b"missing"),
     (dict(q_start=None), b"missing"), (dict(kv_len=None), b"missing"), (dict(tables=None), b"missing"), (dict(q_ld=255), b"stride"), (dict(out_ld=255), b"stride"), (dict(q=66), b"aligned"),
     (dict(tables=65), b"aligned"), (dict(scratch=None), b"scratch"), (dict(scratch=72), b"scratch"), (dict(scratch_bytes=1), b"scratch")])
 def test_attend_refuses(lib, change, why):
@@ -99,6 +100,21 @@ def test_bad_caches_are_refused(lib, change, why):
     for call in (lambda: lib.l3m_kv4_attend_dev(C.byref(c), C.byref(attend()), None), lambda: lib.l3m_qkv_rope_dev(C.byref(c), C.byref(qkv()), None),
                  lambda: lib.l3m_kv4_load_dev(C.byref(c), 0, 64, 64, 64, 1, None)):
         assert call() == -1 and why in lib.l3m_cuda_error(), lib.l3m_cuda_error()
+
+
+def test_a_cache_of_too_many_tiles_is_refused(lib):
+    c = cache(n_pages=1 << 16, n_kv_heads=1 << 15)
+    assert lib.l3m_kv4_load_dev(C.byref(c), 0, 64, 64, 64, 1, None) == -1 and b"2^31 tiles" in lib.l3m_cuda_error()
+
+
+def test_plan_restatement_leaves_out_bad_pages_and_lengths_at_the_end_of_int32():
+    tables = np.array([[7, 1, -1], [2, -1, -1]], np.int32)
+    got = ref.plan(np.array([20, 3], np.int32), np.array([13, 1], np.int32), tables, np.array([0, 3, 4, 5, 0, 0], np.int32), 4, 16, 16)
+    assert got["status"] == 0 and list(got["slot"][:13]) == [1 * 16 + 4 + i for i in range(12)] + [5 * 16]
+    got = ref.plan(np.array([14, 3], np.int32), np.array([3, 1], np.int32), tables, np.array([0, 3, 4, 5, 0, 0], np.int32), 4, 16, 16)
+    assert got["status"] == ref.BAD_PAGE and list(got["slot"][:4]) == [-1, -1, 5 * 16, 2 * 16 + 3]
+    got = ref.plan(np.array([2 ** 31 - 17], np.int32), np.array([1], np.int32), np.zeros((1, 1), np.int32), np.zeros(1, np.int32), 0, 16, 1)
+    assert got["status"] & ref.BAD_LENGTH
 
 
 def test_null_arguments_are_refused(lib):
@@ -138,5 +154,5 @@ def test_scratch_size_of_prompt_chunks(lib):
     for kw in (dict(dtype=0), dict(max_q=8), dict(n_req=1, max_q=256)):
         assert size(128, **kw) > 16
     assert size(96) > 16 and size(32) > 16 and size(136) > 16
-    assert size(128, n_req=1 << 21) > 16 and size(128, max_q=1 << 30) > 16
+    assert size(128, n_req=1 << 21) > 16 and size(128, max_q=1 << 24) > 16
     assert size(128, max_q=0) > 16 and size(128, n_req=0) > 16
