@@ -181,7 +181,7 @@ struct Smem {
     static constexpr int DP = 32 * NG, TILE = kRows * DP * 2;   // one operand tile of 128 rows
     uint8_t q[2][TILE], k[2][TILE], v[2][TILE];
     uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
-    uint64_t s_full[2][2], p_full[2][2], pv_done[2];      // [tile][half]
+    uint64_t s_full[2][2], p_full[2][2], pv_done[2], end[2];   // [tile][half]
     uint32_t tmem, bad[4][4];             // tokens of a step in no page of the cache, a ring of four steps
     int k_top, v_top;
 };
@@ -226,6 +226,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 bar_init(&s.p_full[b][u], kRows);
             }
             bar_init(&s.pv_done[b], 1);
+            bar_init(&s.end[b], 1);
         }
         s.k_top = s.v_top = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -439,6 +440,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
                 tc_after();
                 score(u + 2);
             }
+            // Nothing of this warp's is under way when the CTA ends, whatever ended the loop
+            tc_commit(lead, smem_u32(&s.end[t]));
+            ok = warp_wait(&s.end[t], 0) && ok;
         }
     } else if (tile < tiles) {
         // ---- softmax: thread = row
