@@ -811,7 +811,7 @@ __global__ void __launch_bounds__(32 * warps_of(NG, NT), kCtas) attend_kernel(co
             total += sum;
         }
         share = (total + gridDim.x - 1) / gridDim.x;
-        share = max((share + 2 * kWarps - 1) / (2 * kWarps) * (2 * kWarps), (long long)p.split);
+        share = (share + 2 * kWarps - 1) / (2 * kWarps) * (2 * kWarps);
         u0 = share * blockIdx.x;
         u1 = min(u0 + share, total);
         long long base = 0;
@@ -953,12 +953,20 @@ __global__ void __launch_bounds__(kJoinThreads) join_kernel(const __grid_constan
     }
 }
 
-constexpr int kSplitFrom = 512;           // cached tokens from which segments are shared out
-constexpr int kLeastShare = 16;           // tiles of a worker's share
+// Cached tokens from which the line is cut into even shares, whose pieces a second kernel joins. One token each, 32 heads to 8 of
+// 128, bf16, alone on the GPU: 1 request of 768 tokens 19.5 us cut and 15.3 whole, of 1024 19.5 and 16.4, of 2048 19.5 and 22.9; f32 of 1024
+// 21.5 and 22.5. Longer contexts, and those of uneven lengths, gain more the longer they are: a request of 100000 takes 48 us.
+constexpr int kSplitFrom = 1024;
 
+// Blocks of 8 rows that share a tile's codes, 1 or 2. Two take 5/3 of one's time and fewer warps fit an SM, so they are for rows that
+// fill them, and work enough. Measured, one and two, 32 heads to 8 of 128, f32: 1024 rows of one request over 4096 tokens
+// 241 and 201 us; 16 rows of 16 requests over 2000 (16000 tiles) 53 and 49, of 8 requests 37 and 39; 20 rows of 32 requests over 1000 71 and 82.
+// With 16 heads to 4 of 96: 16 rows of 8 requests over 8192 (16400 tiles) 45 and 47, over 2000 27 and 35.
 int row_blocks(const l3m_kv4 *c, const l3m_kv4_attend *a) {
-    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads);
-    return rows > 8 && (c->head_dim + 31) / 32 <= 4 ? 2 : 1;
+    const long long rows = (long long)a->max_q * (a->n_heads / c->n_kv_heads), one = (rows + 7) / 8, two = (rows + 15) / 16;
+    const double span = a->window ? std::min((double)a->max_kv, (double)a->window + a->max_q) : (double)a->max_kv;
+    const double tiles = (double)a->n_req * c->n_kv_heads * two * (span / kKvTile);
+    return 3 * one > 5 * two && tiles >= 20000 && (c->head_dim + 31) / 32 <= 4 ? 2 : 1;
 }
 
 size_t part_floats(int nr, int ng) { return (size_t)2 * nr * (32 * ng + 4); }
@@ -976,7 +984,7 @@ cudaError_t launch(AttendArgs p, cudaStream_t s) {
     if (e != cudaSuccess) return e;
     const int workers = sm_count() * kCtas;
     p.row_tiles = (int)(((long long)p.a.max_q * p.group + W::NR - 1) / W::NR);
-    p.split = p.a.max_kv > kSplitFrom ? kLeastShare : 0;
+    p.split = p.a.max_kv > kSplitFrom;
     p.desc = (int4 *)p.a.scratch;
     p.part = (float *)((char *)p.a.scratch + (size_t)kMaxSms * kCtas * 2 * sizeof(int4));
     const long long segs = (long long)p.a.n_req * p.c.n_kv * p.row_tiles;

@@ -456,6 +456,34 @@ def test_attend_several_tokens(api, dtype, cdtype, heads, kv_heads, dim):
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(8, 8, 16), (9, 3, 64), (6, 6, 48), (16, 4, 128), (16, 2, 96)])
+def test_attend_many_rows_over_long_tables(api, dtype, cdtype, heads, kv_heads, dim):
+    """Chunks whose rows go 16 to a tile of the cache: work enough by the bounds that the call gives, the tables' width (cut into shares
+    and joined) or the number of requests (whole), while the lengths at hand are of every size."""
+    rng = np.random.default_rng(heads + dim)
+    for lens, news, page, width in (([300, 41, 2, 700, 0, 130], [100, 33, 5, 16, 0, 130], 16, 20000 // kv_heads), ([900, 64], [13, 64], 64, 40000 // kv_heads), (list(rng.integers(1, 200, 400)), [16] * 400, 64, 16)):
+        for window in (0, 150):
+            tables, q_start, n_pages = batch(rng, lens, news, page, width=width)
+            host = random_cache(rng, cdtype, n_pages, kv_heads, page, dim)
+            q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, dtype)
+            out, st = api.attend(api.cache(api.put(host), cdtype, page, kv_heads, dim), q, q_start, lens, tables, dim ** -0.5, window, max_kv=width * page)
+            want, spread = ref.attend(q64, q_start, lens, tables, host, cdtype, dim, page, kv_heads, dim ** -0.5, window)
+            got, extra = out.double().cpu().numpy(), 0.0
+            if dtype == BF16 and cdtype == ref.Q4:
+                # Codes enter as n0 + 16 n1, at most 255, and the parts and the offset are taken off the sums behind: what the f32 sums lose
+                # is relative to 255 P times scale, not to the values (a token whose value is 0 loses it, too). A product of 16 tokens
+                # adds to them with a truncation of 2^-23 of the largest term and one of the sum: 255 * 2^-22 < 2^-14 of
+                # sum(p |scale|) / sum(p) <= the largest scale, for each of a warp's products: two a pair of tiles, every fourth pair at least.
+                scales = np.ascontiguousarray(host[..., 544 * ref.blocks(dim):]).view(np.float16)
+                extra = 2 * -(-max(lens) // (4 * 32)) * 2.0 ** -14 * float(np.abs(scales).max())
+            tol = 2.0 ** -8 * np.abs(want) + 2.0 ** -10 * spread + extra if dtype == BF16 else 2.0 ** -16 * spread
+            bad = ~(np.abs(got - want) <= tol + 1e-30)
+            assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[:4], float(np.abs(got - want)[bad].max()))
+            assert st.item() == 0
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("lens,heads,kv_heads,dim", [([20011], 4, 1, 64), ([9000, 1, 30, 5000], 8, 2, 128), ([4097] * 3, 6, 6, 48)])
 def test_attend_long(api, dtype, lens, heads, kv_heads, dim):
     rng = np.random.default_rng(len(lens))
