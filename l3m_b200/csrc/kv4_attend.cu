@@ -143,6 +143,7 @@ struct Segment { int r, h, rt; };
 // nibble in the low byte of a half is an f16 subnormal, n * 2^-24 (or n * 2^-20 four bits higher): one mask, no conversion. Its offset
 // of 8 is taken off the sum instead: scores start at -8 sum(q), and the sum of P times scale, which the values' offset multiplies,
 // comes from one more product with ones. Float results use n - 8 itself (one more f16 operation), so that nothing cancels.
+// (The sums then hold numbers of 255 P scale, so 2^-23 of those, not of the values, is what a step of 16 tokens loses.)
 // A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
 // them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
 // split in two f16 for float ones.
@@ -781,6 +782,8 @@ template <int kWarps> __device__ long long block_sum_scan(long long v, long long
     return v;
 }
 
+// Bound: instructions beside memory. 64 requests to 8192 tokens, 32 heads to 8 of 128, bf16, q4_0: 105 us for 403 MB, 3.9 TB/s (the
+// same loads without the arithmetic 75 us, the arithmetic on one tile over and over 99); one request of 250001, 16 heads to 2: 34 us for 72 MB.
 template <typename T, int MX, int NG, int NT>
 __global__ void __launch_bounds__(32 * warps_of(NG, NT), kCtas) attend_kernel(const __grid_constant__ AttendArgs p) {
     typedef Worker<T, MX, NG, NT> W;
