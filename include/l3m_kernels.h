@@ -144,7 +144,8 @@ enum {
 // q_start[0 .. n_req] (running sum of the new tokens), kv_total[r] (the length with the new tokens), and
 // for each new token its position and slot; rows behind the last one get -1. A request is left out (kv_total 0,
 // slots and positions -1, no pages taken) when its lengths are bad, when the pages wanted by it and the
-// requests before it exceed the free list and it wants some, or when its rows pass max_tokens; a status bit says so.
+// requests before it exceed the free list and it wants some, or when its rows pass max_tokens; a status bit says so. q_start counts its
+// rows all the same, so it can pass max_tokens: l3m_kv4_attend's max_rows = max_tokens keeps the attention inside its tensors then.
 typedef struct {
     int n_req;                   // 0 .. 16384
     int max_blocks;              // entries of a table row
@@ -211,6 +212,8 @@ typedef struct {
     void  *scratch;              // l3m_kv4_attend_scratch() bytes of device memory, 16-byte aligned, in any state;
     size_t scratch_bytes;        // calls that overlap need one each
     int32_t *status;
+    int   max_rows;              // rows that q and out have: queries of rows behind them are not looked at and nothing is written there.
+                                 // 0: not stated, q_start never passes them (the plan's does where it reports L3M_KV4_NO_ROOM)
 } l3m_kv4_attend;
 L3M_API size_t l3m_kv4_attend_scratch(const l3m_kv4 *cache, const l3m_kv4_attend *a);   // from the integer fields alone
 L3M_API int    l3m_kv4_attend_dev(const l3m_kv4 *cache, const l3m_kv4_attend *a, void *stream);

@@ -57,7 +57,7 @@ class Kv4Attend(C.Structure):
     """l3m_kv4_attend: attention of a batch over the cache."""
     _fields_ = [(f, C.c_int) for f in ("dtype", "n_heads", "n_req", "max_blocks", "max_q", "max_kv", "window")] + [("scale", C.c_float)] + \
                [("q", C.c_void_p), ("out", C.c_void_p), ("q_ld", C.c_int64), ("out_ld", C.c_int64)] + \
-               [(f, C.c_void_p) for f in ("q_start", "kv_len", "tables", "scratch")] + [("scratch_bytes", C.c_size_t), ("status", C.c_void_p)]
+               [(f, C.c_void_p) for f in ("q_start", "kv_len", "tables", "scratch")] + [("scratch_bytes", C.c_size_t), ("status", C.c_void_p), ("max_rows", C.c_int)]
 
 
 GEMV = C.CFUNCTYPE(None, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.POINTER(Vec))

@@ -61,4 +61,18 @@ inline Kv4Dev kv4_dev(const l3m_kv4 *c) {
     return d;
 }
 
+// What request r asks of an attention call: its first row of q, how many of its rows are looked at, its cached tokens, and its
+// first query's position. Rows are cut off at max_q and at the end of q; positions count from the request's own number of them.
+struct Queries { int start, nq, kv, at; };
+__device__ __forceinline__ Queries queries_of(const l3m_kv4_attend &a, int r) {
+    Queries q;
+    q.start = a.q_start[r];
+    const int count = min(max(a.q_start[r + 1] - q.start, 0), 1 << 30);
+    q.nq = min(count, a.max_q);
+    if (a.max_rows) q.nq = min(q.nq, max(a.max_rows - q.start, 0));
+    q.kv = min(max(a.kv_len[r], 0), a.max_kv);
+    q.at = q.kv - count;
+    return q;
+}
+
 }  // namespace l3m

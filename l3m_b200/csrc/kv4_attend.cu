@@ -181,7 +181,7 @@ struct Worker {
     // Row r of a 16-token product is token tau(r): a warp's reads of keys (rows g) and of values (tokens of k = 2t, 2t + 1) then spread over the banks.
     __device__ static int tau(int r) { return (r & 8) | (r & 1 ? 4 + (((r >> 1) & 3) ^ 1) : (r >> 1) & 3); }
 
-    __device__ __forceinline__ void load_rows(int start, int nq, int kv, int h, int rt) {
+    __device__ __forceinline__ void load_rows(int start, int nq, int first, int h, int rt) {
         float m8[NT], cs[NT][NG];
         const float log2e = 1.4426950408889634f;
 #pragma unroll
@@ -256,7 +256,7 @@ struct Worker {
             for (int c = 0; c < 2; c++) {
                 mult[n][c] = __shfl_sync(0xffffffffu, m8[n], 8 * t + 4 * c);
                 const int i = (rt * NR + n * 8 + 2 * t + c) / p.group;
-                pos[n][c] = i < nq ? kv - nq + i : -1;
+                pos[n][c] = i < nq ? first + i : -1;
                 ref[n][c] = kFloor;
                 sum[n][c] = 0.0f;
             }
@@ -619,10 +619,10 @@ struct Worker {
     }
 
     // Cache tiles [a, b) of request r's head h into the rows' sums.
-    __device__ __forceinline__ void run(int r, int h, int rt, int start, int nq, int kv, int a, int b) {
+    __device__ __forceinline__ void run(int r, int h, int rt, const Queries &rq, int a, int b) {
         const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
-        const int i0 = rt * NR / p.group, i1 = min((rt * NR + NR - 1) / p.group, nq - 1);
-        const int first = kv - nq + i0, last = kv - nq + i1;                 // the rows' positions
+        const int i0 = rt * NR / p.group, i1 = min((rt * NR + NR - 1) / p.group, rq.nq - 1);
+        const int first = rq.at + i0, last = rq.at + i1;                     // the rows' positions
         const int lo_any = p.a.window ? first - p.a.window + 1 : 0, hi_any = last + 1;
         const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;   // seen by every row
         uint8_t *ring = smem + warp * RING;
@@ -660,7 +660,7 @@ struct Worker {
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         fetch(0);                                                            // under way while the rows are read
-        load_rows(start, nq, kv, h, rt);
+        load_rows(rq.start, rq.nq, rq.at, h, rt);
         for (int k = 0; k < n; k++) {
             fetch(k + 1);
             asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -750,14 +750,12 @@ struct Worker {
     }
 };
 
-struct Request { int start, nq, kv, lo, tiles, rts; };            // cache tiles [lo, lo + tiles), row tiles
+struct Request : Queries { int lo, tiles, rts; };                 // cache tiles [lo, lo + tiles), row tiles
 
 __device__ __forceinline__ Request request_of(const AttendArgs &p, int r, int nr) {
     Request q;
-    q.start = p.a.q_start[r];
-    q.nq = min(max(p.a.q_start[r + 1] - q.start, 0), p.a.max_q);
-    q.kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
-    const int lo = p.a.window ? max(0, q.kv - q.nq - p.a.window + 1) : 0;
+    (Queries &)q = queries_of(p.a, r);
+    const int lo = p.a.window && q.at > 0 ? max(0, q.at - p.a.window + 1) : 0;
     q.lo = lo / kKvTile;
     q.tiles = max(1, (q.kv + kKvTile - 1) / kKvTile - q.lo);     // one at least: a request whose queries see nothing has rows to write
     q.rts = (q.nq * p.group + nr - 1) / nr;
@@ -863,9 +861,9 @@ __global__ void __launch_bounds__(32 * warps_of(NG, NT), kCtas) attend_kernel(co
         }
         const int h = x / rts, rt = x - h * rts;
         if (rt < q.rts) {
-            const int last = q.kv - q.nq + min((rt * W::NR + W::NR - 1) / p.group, q.nq - 1), top = last >= 0 ? last / kKvTile + 1 : 0;
+            const int last = q.at + min((rt * W::NR + W::NR - 1) / p.group, q.nq - 1), top = last >= 0 ? last / kKvTile + 1 : 0;
             const bool begins = off == 0, ends = off + len == q.tiles;
-            w.run(r, h, rt, q.start, q.nq, q.kv, q.lo + off, min(q.lo + off + len, top));
+            w.run(r, h, rt, q, q.lo + off, min(q.lo + off + len, top));
             w.finish(q.start, q.nq, h, rt, begins && ends ? nullptr : p.part + ((size_t)blockIdx.x * 2 + (begins ? 1 : 0)) * W::NR * (W::DP + 4));
             if (!begins && ends) {
                 desc = make_int4((int)((u0 - off) / share), h, rt, 0);
@@ -1037,7 +1035,7 @@ const char *attend_error(const l3m_kv4 *c, const l3m_kv4_attend *a) {
     if (!a) return "arguments are required";
     if (a->dtype != L3M_DT_F32 && a->dtype != L3M_DT_BF16) return "dtype must be f32 or bf16";
     if (a->n_heads < 1 || a->n_heads > 65535 || a->n_heads % c->n_kv_heads) return "n_heads must be a positive multiple of n_kv_heads";
-    if (a->n_req < 0 || a->max_blocks < 0 || a->max_q < 0 || a->max_kv < 0 || a->window < 0) return "a count is negative";
+    if (a->n_req < 0 || a->max_blocks < 0 || a->max_q < 0 || a->max_kv < 0 || a->window < 0 || a->max_rows < 0) return "a count is negative";
     if ((int64_t)a->max_q * a->n_heads > 1 << 30) return "max_q * n_heads must be at most 2^30";
     if (a->max_kv > (int64_t)a->max_blocks * c->page) return "max_kv must not exceed max_blocks * page";
     return nullptr;

@@ -209,11 +209,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     // ---- what this CTA does: the last rows first, they see most
     const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
     const int r = x / per_req, h = (x - r * per_req) / p.row_tiles, rt = p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles);
-    const int start = p.a.q_start[r], nq = min(max(p.a.q_start[r + 1] - start, 0), p.a.max_q), kv = min(max(p.a.kv_len[r], 0), p.a.max_kv);
+    const Queries rq = queries_of(p.a, r);
+    const int start = rq.start, nq = rq.nq;
     const int row0 = rt * 2 * kRows, rows = nq * p.group - row0;           // rows left from this CTA's first
     if (rows <= 0) return;
     const int tiles = rows > kRows ? 2 : 1;
-    const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = kv - nq + i0, last = kv - nq + i1;   // the rows' positions
+    const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = rq.at + i0, last = rq.at + i1;   // the rows' positions
     const int lo_any = p.a.window ? max(0, first - p.a.window + 1) : 0, hi_any = max(last + 1, 0);      // seen by some row
     const int whole_lo = p.a.window ? last - p.a.window + 1 : 0, whole_hi = first + 1;                  // seen by every row
     const int t0 = lo_any / kStep * kStep, steps = hi_any > lo_any ? (hi_any - t0 + kStep - 1) / kStep : 0, halves = hi_any > lo_any ? (hi_any - t0 + kHalf - 1) / kHalf : 0;
@@ -275,7 +276,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const int tile = warp / 4;                                              // of a softmax warp
     const int row = tile * kRows + (warp & 3) * 32 + lane, qi = (row0 + row) / p.group, head = h * p.group + (row0 + row) % p.group;
     const bool live = warp < kSoftWarps && row < rows;
-    const int at = live ? kv - nq + qi : -1;
+    const int at = live ? rq.at + qi : -1;
     int up = 0;
     if (warp < kSoftWarps && tile < tiles) {
         // ---- this thread's query, in the order in which the keys' codes come out of their words
