@@ -170,7 +170,14 @@ struct Worker {
     float ref[NT][2], sum[NT][2];
     float o[NT][NG][2][4];
     float w[SUBN ? NT : 1][SUBN ? (NG + 1) / 2 : 1][4];                       // two blocks' sums of P times scale: rows 0-7 block 2i, rows 8-15 block 2i + 1
-    int vexp, eref;
+    // The window of the values' scales that a step's products take as they come: exponents base .. base + 15. mxfp4: a base for each block,
+    // four to a word; the block's sums are in units of 2^(base - 113). q4_0: one base for all blocks, which lowers P's limit. For bf16 results it
+    // stays 4 or less, as P itself is held in f16: larger scales than 32 are brought down to the window.
+    uint32_t base4[MX ? SW : 1];
+    int base;
+    static constexpr int kMaxBase = SUBN ? 4 : 16;
+    bool begun;
+    static constexpr int kFirstBase = 115;                                   // scales of 2^-12 to 2^3, as activations have them; another window costs the first step a little
 
     __device__ Worker(const AttendArgs &args, uint8_t *sm) : p(args), smem(sm) {
         warp = threadIdx.x >> 5;
@@ -268,8 +275,10 @@ struct Worker {
                     if (SUBN) w[n][j / 2][e] = 0.0f;
                 }
         }
-        vexp = PREC && !MX ? -16 : 0;                                              // P itself is held in f16 for bf16 results: 2^14 at most
-        eref = 15;
+        base = PREC && !MX ? -16 : 0;
+#pragma unroll
+        for (int i = 0; i < (MX ? SW : 1); i++) base4[i] = 0x01010101u * kFirstBase;
+        begun = false;
     }
 
     __device__ __forceinline__ void scale_rows(int n, float f0, float f1) {
@@ -374,54 +383,37 @@ struct Worker {
         }
         // ---- the values' scales: of this lane's tokens as P's transposed pairs want them, or (float results) as the scores lie
         uint32_t v[U][4][SW];
+        auto load_scales = [&]() {
 #pragma unroll
-        for (int u = 0; u < U; u++)
+            for (int u = 0; u < U; u++)
 #pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (PREC && k % 2) {
+                for (int k = 0; k < 4; k++) {
+                    if (PREC && k % 2) {
 #pragma unroll
-                    for (int i = 0; i < SW; i++) v[u][k][i] = 0;
-                    continue;
-                }
-                const int row = (k % 2 ? t1 : t0) + (k / 2) * 8;
-                if (MX) lds_bytes<NG>(v[u][k], sm + u * TB + VS + row * NG);
-                else lds_halves<NG>(v[u][k], sm + u * TB + VS + row * NG * 2);
-                if (EDGE) {
-                    const int tok = tok0 + u * kKvTile + row;
-                    const bool gone = tok < lo_any || tok >= hi_any;
-#pragma unroll
-                    for (int i = 0; i < SW; i++) {
-                        uint32_t &x = v[u][k][i];
-                        if (!MX) {                                           // infinities and NaN that some row does not see must not meet its zeros
-                            if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u;
-                            if ((x & 0x7c000000u) == 0x7c000000u) x &= 0x0000ffffu;
-                        }
-                        if (gone) x = 0;
+                        for (int i = 0; i < SW; i++) v[u][k][i] = 0;
+                        continue;
                     }
+                    const int row = (k % 2 ? t1 : t0) + (k / 2) * 8;
+                    if (MX) lds_bytes<NG>(v[u][k], sm + u * TB + VS + row * NG);
+                    else lds_halves<NG>(v[u][k], sm + u * TB + VS + row * NG * 2);
+                    if (EDGE) harmless(v[u][k], tok0 + u * kKvTile + row, lo_any, hi_any);
                 }
+        };
+        auto relative = [&]() {                                              // mxfp4: bytes 0 .. 15 are in the window
+            if (MX) {
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int k = 0; k < 4; k += PREC ? 2 : 1)
+#pragma unroll
+                        for (int i = 0; i < SW; i++) v[u][k][i] = EDGE && v[u][k][i] == kGone ? 0 : v[u][k][i] - base4[MX ? i : 0];
             }
-        // ---- does the reference still hold? P <= 2^lim, |scale| < 2^(vexp + 1) (mxfp4: scales are taken relative to eref, vexp stays)
-        bool move;
-        uint32_t any = 0;
-#pragma unroll
-        for (int u = 0; u < U; u++)
-#pragma unroll
-            for (int k = 0; k < 4; k += PREC ? 2 : 1)
-#pragma unroll
-                for (int i = 0; i < SW; i++) {
-                    if (MX) any |= v[u][k][i];                               // at least the largest; eref ends in ones, so that it is that mostly
-                    else if (PREC) any = __vmaxu2(any, v[u][k][i] & 0x7fff7fffu);
-                    else any |= v[u][k][i];
-                }
-        if (MX) {
-            any |= any >> 16;
-            move = (int)((any | any >> 8) & 0xff) > eref;
-        } else if (PREC) {
-            move = (int)max(any >> 10 & 31, any >> 26) - 15 > vexp;
-        } else {
-            move = (any & 0x40004000u) && vexp < 16;
-        }
-        float lim = 14.0f - (float)vexp, z[U][NT][4], high = kFloor;         // the exponents of P
+        };
+        load_scales();
+        relative();
+        // ---- does the reference still hold, do the scales lie in the window?
+        bool far = outside<U>(v);
+        float lim = limit(), z[U][NT][4], high = kFloor;         // the exponents of P
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
@@ -431,32 +423,50 @@ struct Worker {
                     z[u][n][e] = EDGE && s[u][n][e] == -INFINITY ? -INFINITY : fmaf(s[u][n][e], mult[n][e & 1], -ref[n][e & 1]);
                     high = fmaxf(high, z[u][n][e]);
                 }
-        move |= high > lim;
-        if (__any_sync(0xffffffffu, move)) {
-            int top = 0;
+        if (__any_sync(0xffffffffu, far || high > lim)) {
+            if (MX && __any_sync(0xffffffffu, far)) {
+                load_scales();
+                uint32_t top[SW];
 #pragma unroll
-            for (int u = 0; u < U; u++)
+                for (int i = 0; i < SW; i++) {
+                    top[i] = 0;
 #pragma unroll
-                for (int k = 0; k < 4; k++)
+                    for (int u = 0; u < U; u++)
 #pragma unroll
-                    for (int i = 0; i < SW; i++) {
-                        const uint32_t x = v[u][k][i];
-                        if (MX) top = max(max(top, (int)(x & 0xff)), max((int)(x >> 8 & 0xff), max((int)(x >> 16 & 0xff), (int)(x >> 24))));
-                        else top = max(top, max((int)(x >> 10 & 31), (int)(x >> 26 & 31)));
-                    }
+                        for (int k = 0; k < 4; k += PREC ? 2 : 1) top[i] = __vmaxu4(top[i], EDGE && v[u][k][i] == kGone ? 0 : v[u][k][i]);
 #pragma unroll
-            for (int d = 1; d < 32; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
-            float shrink = 1.0f;
-            if (MX) {
-                top = min(top | 3, 254);
-                if (top > eref) {
-                    shrink = top - eref > 126 ? 0.0f : __uint_as_float((uint32_t)(127 - (top - eref)) << 23);
-                    eref = top;
+                    for (int d = 1; d < 32; d <<= 1) top[i] = __vmaxu4(top[i], __shfl_xor_sync(0xffffffffu, top[i], d));
                 }
-            } else {
-                vexp = max(vexp, top - 15);
-                lim = 14.0f - (float)vexp;                                   // raising vexp lowers it
+#pragma unroll
+                for (int j = 0; j < NG; j++) {                               // a block whose base moves gets room for three more below the window's end
+                    const int at = 8 * (j % 4), have = base4[MX ? j / 4 : 0] >> at & 0xff, most = min((int)(top[j / 4] >> at & 0xff), 254);
+                    if (most > have + 15 || (!begun && most < have)) {
+                        const int to = max(min(most - 12, 239), 0);
+                        base4[MX ? j / 4 : 0] += (uint32_t)(to - have) << at;
+                        const float f = !begun || to - have > 126 ? 0.0f : exp2i(have - to);
+#pragma unroll
+                        for (int n = 0; n < NT; n++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                o[n][j][0][e] *= f;
+                                o[n][j][1][e] *= f;
+                            }
+                    }
+                }
+                relative();
+            } else if (!MX && __any_sync(0xffffffffu, far)) {
+                uint32_t top = 0;
+#pragma unroll
+                for (int u = 0; u < U; u++)
+#pragma unroll
+                    for (int k = 0; k < 4; k += PREC ? 2 : 1)
+#pragma unroll
+                        for (int i = 0; i < SW; i++) top = max(top, max(v[u][k][i] >> 10 & 31, v[u][k][i] >> 26 & 31));
+                base = min(max(base, (int)__reduce_max_sync(0xffffffffu, top) - 15), kMaxBase);
+                lim = limit();                                               // raising base lowers it
             }
+            begun = true;
+            far = __any_sync(0xffffffffu, outside<U>(v));
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float f[2];
@@ -483,10 +493,25 @@ struct Worker {
                         for (int e = c; e < 4; e += 2) z[u][n][e] = EDGE && s[u][n][e] == -INFINITY ? -INFINITY : fmaf(s[u][n][e], mult[n][c], -ref[n][c]);
                     sum[n][c] *= f[c];
                 }
-                scale_rows(n, f[0] * shrink, f[1] * shrink);
+                scale_rows(n, f[0], f[1]);
             }
         }
         // ---- probabilities and values
+        if (far) {
+#pragma unroll 1
+            for (int u = 0; u < U; u++) {
+                float zz[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+#pragma unroll
+                    for (int e = 0; e < 4; e++) zz[n][e] = ex2(u ? z[U - 1][n][e] : z[0][n][e]);
+                    sum[n][0] += zz[n][0] + zz[n][2];
+                    sum[n][1] += zz[n][1] + zz[n][3];
+                }
+                far_values<EDGE>(sm + u * TB, zz, tok0 + u * kKvTile, lo_any, hi_any);
+            }
+            return;
+        }
 #pragma unroll
         for (int u = 0; u < U; u++) {
             uint32_t pb[NT][2];
@@ -610,12 +635,155 @@ struct Worker {
             f[k] = *(const uint32_t *)&r;
         }
     }
-    // mxfp4 scales relative to eref: 2^(e - eref).
-    __device__ __forceinline__ float rel_f32(uint32_t e) const { return __uint_as_float((uint32_t)max((int)e - eref + 127, 0) << 23); }
-    __device__ __forceinline__ uint32_t rel_f16(const uint32_t *a, const uint32_t *b, int j) const {
-        const uint32_t x = prmt(a[j / 4], b[j / 4], j % 4 < 2 ? 0x5410 : 0x7632), base = (uint32_t)(eref - 15) * 0x10001u;      // two blocks' bytes of both tokens
+    // mxfp4 scales in the window, e above its base: 2^(e - 14), 2^-14 to 2.
+    __device__ __forceinline__ static float rel_f32(uint32_t e) { return __uint_as_float((e + 113u) << 23); }
+    __device__ __forceinline__ static uint32_t rel_f16(const uint32_t *a, const uint32_t *b, int j) {
+        const uint32_t x = prmt(a[j / 4], b[j / 4], j % 4 < 2 ? 0x5410 : 0x7632);      // two blocks' bytes of both tokens
         const uint32_t e = j % 2 ? prmt(x, 0, 0x4341) : x & 0x00ff00ffu;
-        return __vmaxs2(e, base) * 1024u - base * 1024u;
+        return e * 1024u + 0x04000400u;
+    }
+    // The largest exponent of P: P times a scale has to stay below 2^16 in the products' f16.
+    __device__ __forceinline__ float limit() const { return MX ? 14.0f : 14.0f - (float)base; }
+
+    // Does some scale of this lane's tokens lie outside the window? mxfp4: bytes 0 .. 15 above the base. q4_0: the exponents of f16 scales, for
+    // bf16 results those above the window alone (scales of 2 and more, mostly none): below it P times scale has its 11 bits down to 2^-14.
+    template <int U> __device__ __forceinline__ bool outside(const uint32_t (&v)[U][4][SW]) const {
+        uint32_t any = 0;
+#pragma unroll
+        for (int u = 0; u < U; u++)
+#pragma unroll
+            for (int k = 0; k < 4; k += PREC ? 2 : 1)
+#pragma unroll
+                for (int i = 0; i < SW; i++) {
+                    // a difference below 0 shows in its own high bits, whatever it borrows from the next one
+                    if (MX) any |= v[u][k][i] & (0xf0f0f0f0u >> (NG - 4 * i < 4 ? 8 * (4 * i + 4 - NG) : 0));
+                    else if (PREC) any |= ((v[u][k][i] & 0x7fff7fffu) - (uint32_t)base * 0x04000400u) & (NG - 2 * i < 2 ? 0x0000c000u : 0xc000c000u);
+                    else any |= v[u][k][i] & 0x40004000u;
+                }
+        if (SUBN && any && base > 0) {
+            any = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++)
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int i = 0; i < SW; i++) any = __vmaxu2(any, v[u][k][i] & 0x7fff7fffu);
+            return (int)max(any >> 10 & 31, any >> 26) > base + 15;
+        }
+        return any != 0;
+    }
+
+    // What must not meet the zeros of rows that do not see token tok: a scale that is not finite counts as 0, and so does the scale of a token that
+    // no row sees (mxfp4: kGone, as good as any in the window then).
+    static constexpr uint32_t kGone = 0xffffffffu;
+    __device__ __forceinline__ static void harmless(uint32_t *v, int tok, int lo_any, int hi_any) {
+        const bool gone = tok < lo_any || tok >= hi_any;
+#pragma unroll
+        for (int i = 0; i < SW; i++) {
+            uint32_t &x = v[i];
+            if (MX) {
+#pragma unroll
+                for (int k = 0; k < 32; k += 8)
+                    if ((x >> k & 0xff) == 0xff) x &= ~(0xffu << k);
+                if (gone) x = kGone;
+            } else {
+                if ((x & 0x7c00u) == 0x7c00u) x &= 0xffff0000u;
+                if ((x & 0x7c000000u) == 0x7c000000u) x &= 0x0000ffffu;
+                if (gone) x = 0;
+            }
+        }
+    }
+
+    // A tile whose scales the window does not hold: its values' products by sixteen exponents at a time, each level's brought up to the
+    // window (or down to it, where bf16 results meet q4_0 scales of 32 and more) and added to the sums in 32 bits. So no scale is
+    // lost beside a larger one, of another block, another token, or one that some rows do not see. Two levels take about
+    // twice a tile's time. There are eight levels: what is 2^-112 of the block's largest scale counts as 0, and the sums' 32 bits keep no more.
+    template <bool EDGE> __device__ __forceinline__ void far_values(const uint8_t *tl, const float (&zz)[NT][4], int tok0, int lo_any, int hi_any) {
+        const int ra = tau(g), t1 = 4 + (t ^ 1);
+        constexpr int VS = 512 * NG + 16 * NG * SB;
+        uint32_t pb[NT][2];
+        if (!PREC) {
+#pragma unroll
+            for (int n = 0; n < NT; n++) {
+                pb[n][0] = transpose8(pack_f16(zz[n][0], zz[n][1]));
+                pb[n][1] = transpose8(pack_f16(zz[n][2], zz[n][3]));
+            }
+        }
+        bool more = true;
+#pragma unroll 1
+        for (int lev = SUBN ? -1 : 0; lev < 8 && __any_sync(0xffffffffu, more); lev++) {
+            const float up = exp2i(16 * lev), down = exp2i(-16 * lev);
+            more = SUBN && lev < 0;
+            // A scale brought to the window, as a float; 0 outside this level
+            auto scale = [&](int row, int j) -> float {
+                const int low = (MX ? (int)(base4[MX ? j / 4 : 0] >> (8 * (j % 4)) & 0xff) : base) - 16 * lev;      // exponents low .. low + 15
+                if (EDGE && (tok0 + row < lo_any || tok0 + row >= hi_any)) return 0.0f;
+                if (MX) {
+                    const int e = tl[VS + row * NG + j];
+                    if (EDGE && e == 255) return 0.0f;
+                    more |= e > 0 && e < low;
+                    return e >= low && e <= low + 15 ? exp2i(e - low - 14) : 0.0f;
+                }
+                const uint32_t x = *(const uint16_t *)(tl + VS + (row * NG + j) * 2);
+                const int e = x >> 10 & 31;
+                if (EDGE && e == 31) return 0.0f;
+                more |= (x & 0x7fff) && e < low;
+                return e >= low && e <= low + 15 ? __half2float(__ushort_as_half((unsigned short)x)) * up : 0.0f;
+            };
+            uint32_t c[4][(NG + 1) / 2];
+            const uint8_t *vc = tl + 256 * NG + g * 2 * NG;
+            lds_halves<NG>(c[0], vc + t * 16 * NG);
+            lds_halves<NG>(c[1], vc + t1 * 16 * NG);
+            lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
+            lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                uint32_t fa[4], fb[4];
+                value4(fa, c[0], c[1], j);
+                value4(fb, c[2], c[3], j);
+                uint32_t s0 = 0, s1 = 0;
+                float d0 = 0.0f, d1 = 0.0f;
+                if (PREC) {
+                    d0 = scale(ra, j);
+                    d1 = scale(ra + 8, j);
+                } else {
+                    s0 = pack_f16(scale(t, j), scale(t1, j));
+                    s1 = pack_f16(scale(t + 8, j), scale(t1 + 8, j));
+                }
+#pragma unroll
+                for (int n = 0; n < NT; n++) {
+                    uint32_t b0, b1, l0 = 0, l1 = 0;
+                    if (PREC) {
+                        const float x0 = zz[n][0] * d0, x1 = zz[n][1] * d0, x2 = zz[n][2] * d1, x3 = zz[n][3] * d1;
+                        const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
+                        const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
+                        l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y));
+                        l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
+                        b0 = transpose8(h0);
+                        b1 = transpose8(h1);
+                    } else {
+                        b0 = mul2(pb[n][0], s0);
+                        b1 = mul2(pb[n][1], s1);
+                    }
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (PREC) mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
+                        mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) o[n][j][m][e] = fmaf(acc[e], down, o[n][j][m][e]);
+                    }
+                    if (SUBN) {
+                        constexpr uint32_t one = 0x3c003c00u;
+                        const uint32_t hi = j % 2 ? 0 : one, lo = j % 2 ? one : 0;
+                        float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma(acc, hi, lo, hi, lo, b0, b1);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) w[SUBN ? n : 0][SUBN ? j / 2 : 0][e] = fmaf(acc[e], down, w[SUBN ? n : 0][SUBN ? j / 2 : 0][e]);
+                    }
+                }
+            }
+        }
     }
 
     // Cache tiles [a, b) of request r's head h into the rows' sums.
@@ -697,8 +865,7 @@ struct Worker {
                     row[DP] = ref[n][c];
                     row[DP + 1] = s;
                 }
-                const float unit = MX ? __uint_as_float((uint32_t)eref << 23) : 1.0f;
-#pragma unroll
+                #pragma unroll
                 for (int j = 0; j < NG; j++) {
                     float v[4] = {o[n][j][0][c], o[n][j][0][2 + c], o[n][j][1][c], o[n][j][1][2 + c]};
                     if (SUBN) {
@@ -706,7 +873,10 @@ struct Worker {
                         v[0] = fmaf(v[0] - v[1], 0x1p24f, -off); v[1] = fmaf(v[1], 0x1p20f, -off);
                         v[2] = fmaf(v[2] - v[3], 0x1p24f, -off); v[3] = fmaf(v[3], 0x1p20f, -off);
                     }
-                    if (MX) v[0] *= unit, v[1] *= unit, v[2] *= unit, v[3] *= unit;
+                    if (MX) {
+                        const float unit = exp2i((int)(base4[MX ? j / 4 : 0] >> (8 * (j % 4)) & 0xff) - 113);
+                        v[0] *= unit, v[1] *= unit, v[2] *= unit, v[3] *= unit;
+                    }
                     *(float4 *)(row + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
                 }
             }

@@ -92,3 +92,127 @@ def test_rows_that_are_cut_off_do_not_move_the_others(api, dtype):
         for most in (1, 7, 8, 30, 47, 48, 52, 60):
             out, _ = again(api, cache, max_rows=most)
             assert api.torch.equal(out[:most], want[:most]) and (out[most:] == 123).all()
+
+
+# ---- scales far apart
+
+def scale_cells(host, cdtype, dim, is_v):
+    """The scales of a random cache as a writable view [pages, heads, tiles, 16 tokens, blocks]: f16 numbers or e8m0 bytes."""
+    ng, width = ref.blocks(dim), 2 if cdtype == ref.Q4 else 1
+    lo = 512 * ng + (16 * ng * width if is_v else 0)
+    part = host[..., lo:lo + 16 * ng * width]
+    part = part.view(np.float16) if cdtype == ref.Q4 else part
+    return np.lib.stride_tricks.as_strided(
+        part, part.shape[:3] + (16, ng), part.strides[:3] + (part.strides[3] * ng, part.strides[3]))
+
+
+def of_token(cells, tables, r, t, page):
+    return cells[tables[r, t // page], :, t % page // 16, t % 16]
+
+
+FAR = [(ref.Q4, 8), (ref.Q4, 12), (ref.Q4, 20), (ref.MX, 8), (ref.MX, 12), (ref.MX, 15), (ref.MX, 16), (ref.MX, 17), (ref.MX, 24), (ref.MX, 40)]
+
+
+def far_case(rng, cdtype, lens, news, kh, page, dim):
+    tables, q_start, n_pages = batch(rng, lens, news, page)
+    host = random_cache(rng, cdtype, n_pages, kh, page, dim)
+    return tables, q_start, host, scale_cells(host, cdtype, dim, False), scale_cells(host, cdtype, dim, True)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype,gap", FAR)
+@pytest.mark.parametrize("new", [1, 5, 40])
+@pytest.mark.parametrize("dim,lens", [(64, [75, 40]), (128, [1500]), (160, [90])])
+def test_values_whose_blocks_are_far_apart(api, dtype, cdtype, gap, new, dim, lens):
+    """A head whose blocks of 32 dims differ in size by 2^gap from one to the next, the large one first or last, in all tokens."""
+    rng = np.random.default_rng(gap + new)
+    for order in (1, -1):
+        tables, q_start, host, _, v = far_case(rng, cdtype, lens, [new] * len(lens), 2, 16, dim)
+        step = (np.arange(ref.blocks(dim))[::order] * gap) if cdtype == ref.MX else np.minimum(np.arange(ref.blocks(dim))[::order] * gap, 24)
+        if cdtype == ref.MX:
+            v[...] = np.clip(200 - step - rng.integers(0, 4, v.shape), 1, 254)
+        else:
+            v[...] = (np.exp2(10.0 - step) * rng.uniform(1, 2, v.shape) * rng.choice([-1, 1], v.shape)).astype(np.float16)
+        q, q64 = queries(api, rng, int(q_start[-1]), 4, dim, dtype)
+        out, _ = api.attend(api.cache(api.put(host), cdtype, 16, 2, dim), q, q_start, lens, tables, dim ** -0.5)
+        check_attend(out, *ref.attend(q64, q_start, lens, tables, host, cdtype, dim, 16, 2, dim ** -0.5), dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype,gap", FAR)
+@pytest.mark.parametrize("new", [1, 5, 40])
+@pytest.mark.parametrize("lens", [[75, 40], [1500]])
+def test_values_whose_tokens_are_far_apart(api, dtype, cdtype, gap, new, lens):
+    """A few tokens whose values are 2^gap times the others' and which nobody attends to (their scores are a hundred below), in every block or in
+    one; and tokens that get nearly everything while their values are 2^gap times smaller than the rest."""
+    rng, dim, page = np.random.default_rng(100 + gap + new), 64, 16
+    for kind in ("ignored", "ignored in a block", "favoured"):
+        tables, q_start, host, k, v = far_case(rng, cdtype, lens, [new] * len(lens), 2, page, dim)
+        low = 0.01 if cdtype == ref.Q4 else 110
+        v[...] = (low * rng.uniform(1, 2, v.shape)).astype(np.float16) if cdtype == ref.Q4 else low + rng.integers(0, 3, v.shape)
+        host[..., :512] = 0x99 if cdtype == ref.Q4 else 0x11                  # keys of one code: the scale decides
+        k[...] = 0.01 if cdtype == ref.Q4 else 121
+        for r, n in enumerate(lens):
+            for t in rng.choice(n - new, min(3, n - new), replace=False):
+                at, kt = of_token(v, tables, r, t, page), of_token(k, tables, r, t, page)
+                big = min(low * 2.0 ** gap, 30000.0) if cdtype == ref.Q4 else low + gap
+                if kind == "favoured":
+                    at[...] = low * 2.0 ** -min(gap, 14) if cdtype == ref.Q4 else low - gap
+                    kt[...] = 0.4 if cdtype == ref.Q4 else 127                  # a score of about 0.3 * 40 above the others
+                elif kind == "ignored":
+                    at[...] = big
+                else:
+                    at[:, 0] = big
+                if kind != "favoured":
+                    tile = host[tables[r, t // page], :, 0]
+                    tile[:, t % 16 * 32:t % 16 * 32 + 32] = 0x00 if cdtype == ref.Q4 else 0xFF       # -8 or -6 times the scale
+                    kt[...] = 1.0 if cdtype == ref.Q4 else 127
+        q, q64 = queries(api, rng, int(q_start[-1]), 4, dim, dtype)
+        q, q64 = q.abs(), np.abs(q64)
+        out, _ = api.attend(api.cache(api.put(host), cdtype, page, 2, dim), q, q_start, lens, tables, 0.5)
+        want, spread = ref.attend(q64, q_start, lens, tables, host, cdtype, dim, page, 2, 0.5)
+        # A score is off by 2^-20 of sum |q k| scale at most. That is up to sum |q| * 0.4 * 0.5 here (0.5 * 0.5 with mxfp4), not the 5 of the usual
+        # inputs, where the favoured tokens are concerned; a probability by its own score's and the others' mean.
+        off = 2 * 2.0 ** -20 * 0.25 * np.abs(q64).sum(-1, keepdims=True) if kind == "favoured" else 0
+        # And P times scale is held down to 2^-25 (in f16, or the second of two f16), where the largest P is 2^12 or more and the largest scale up to
+        # four windows' steps below 2 (q4_0: 2^base, with P up to 2^(14 - base)): values of 8 steps are off by 2^-25 * 8 * 2^-12 * 4 of that scale.
+        floor = max(lens) * 2.0 ** -32 * (0.02 if cdtype == ref.Q4 else 2.0 ** (low + 2 - 127)) if kind == "favoured" else 0
+        unit = 2.0 ** (-10 if dtype == BF16 else -16)
+        check_attend(out, want, spread * (1 + off / unit) + floor / unit, dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("heads,new", [(4, 5), (8, 3), (4, 40)])
+def test_scales_that_only_later_queries_see(api, dtype, cdtype, heads, new):
+    """The last new token has the largest scales there are, or ones that are not finite: the queries before it have the results
+    without it, although they share a tile of rows with the query that sees it."""
+    rng, dim, page, lens = np.random.default_rng(new), 64, 16, [75, 1100 + new]
+    for last in ((60000.0, np.inf, np.nan) if cdtype == ref.Q4 else (160, 200, 225, 255)):
+        tables, q_start, host, k, v = far_case(rng, cdtype, lens, [new] * 2, 2, page, dim)
+        q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, dtype)
+        want, spread = ref.attend(q64, q_start, lens, tables, host, cdtype, dim, page, 2, 0.125)
+        for r, n in enumerate(lens):
+            of_token(v, tables, r, n - 1, page)[...] = last
+            if not np.isfinite(last) or last == 255:
+                of_token(k, tables, r, n - 1, page)[...] = last
+        out, _ = api.attend(api.cache(api.put(host), cdtype, page, 2, dim), q, q_start, lens, tables, 0.125)
+        for r in range(2):
+            rows = slice(int(q_start[r]), int(q_start[r + 1]) - 1)
+            check_attend(out[rows], want[rows], spread[rows], dtype)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_values_beyond_the_sums_range_count_as_nothing(api, dtype):
+    """A scale of 2^127 beside ones of 2^-3: the queries that do not see it may lose their values (sums have 32 bits) but get nothing else."""
+    rng, dim, page, lens, new = np.random.default_rng(50), 64, 16, [75, 1140], 40
+    tables, q_start, host, _, v = far_case(rng, ref.MX, lens, [new] * 2, 2, page, dim)
+    q, q64 = queries(api, rng, int(q_start[-1]), 4, dim, dtype)
+    _, spread = ref.attend(q64, q_start, lens, tables, host, ref.MX, dim, page, 2, 0.125)
+    for r, n in enumerate(lens):
+        of_token(v, tables, r, n - 1, page)[...] = 254
+    out, st = api.attend(api.cache(api.put(host), ref.MX, page, 2, dim), q, q_start, lens, tables, 0.125)
+    for r in range(2):
+        rows = slice(int(q_start[r]), int(q_start[r + 1]) - 1)
+        assert (np.abs(out[rows].double().cpu().numpy()) <= spread[rows] * (1 + 2.0 ** -7)).all()
+    assert st.item() == 0
