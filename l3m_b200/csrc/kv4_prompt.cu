@@ -260,8 +260,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             for (int j = 0; j < NG; j++) {
                 const uint8_t *ks = tile + 512 * NG + (row * NG + j) * SB, *vs = ks + kKvTile * NG * SB;
                 const int ke = MX ? *ks : *(const uint16_t *)ks >> 10 & 31, ve = MX ? *vs : *(const uint16_t *)vs >> 10 & 31;
-                kt = max(kt, !MX && ke == 31 ? 0 : ke);
-                vt = max(vt, !MX && ve == 31 ? 0 : ve);
+                kt = max(kt, ke == (MX ? 255 : 31) ? 0 : ke);               // what is not finite sets no scale for the rest
+                vt = max(vt, ve == (MX ? 255 : 31) ? 0 : ve);
             }
         }
         for (int o = 16; o; o >>= 1) {
@@ -357,8 +357,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         // Block j's scale brought up by 2^by. edge: what is not finite counts as 0.
         auto scale_of = [&](const C &c, int j, bool edge) -> float {
             if (MX) {
-                const int e = (int)(c.sc[0] >> (8 * j) & 0xff) + by - 127;
-                return e < -24 ? 0.0f : exp2i(min(e, 15));
+                const int bits = (int)(c.sc[0] >> (8 * j) & 0xff), e = bits + by - 127;
+                return e < -24 || (edge && bits == 255) ? 0.0f : exp2i(min(e, 15));
             }
             uint32_t hbits = c.sc[j / 2] >> (16 * (j % 2)) & 0xffff;
             if (edge && (hbits & 0x7c00) == 0x7c00) hbits = 0;

@@ -216,3 +216,60 @@ def test_values_beyond_the_sums_range_count_as_nothing(api, dtype):
         rows = slice(int(q_start[r]), int(q_start[r + 1]) - 1)
         assert (np.abs(out[rows].double().cpu().numpy()) <= spread[rows] * (1 + 2.0 ** -7)).all()
     assert st.item() == 0
+
+
+# ---- prompt chunks
+
+def prompt_want(q, q_start, kv_len, tables, data, cdtype, dim, page, n_kv, scale, window=0):
+    """want_and_tolerance() of test_gpu_kv4_prompt.py without the terms that are relative to the cache's largest scale: what keys and values lose as
+    f16 numbers is 2^-11 of themselves, however large another one is. P is off by 2^-34 of a row's largest, or by all of itself."""
+    heads, n_pages = q.shape[1], data.shape[0]
+    want, tol = np.full(q.shape, np.nan), np.full(q.shape, np.nan)
+    for r in range(len(kv_len)):
+        lo, hi, kv = int(q_start[r]), int(q_start[r + 1]), int(kv_len[r])
+        tok, pos = np.arange(kv), kv - (hi - lo) + np.arange(hi - lo)
+        seen = tok[None] <= pos[:, None]
+        if window:
+            seen &= tok[None] > pos[:, None] - window
+        slots = tables[r][tok // page].astype(np.int64) * page + tok % page
+        for h in range(n_kv):
+            g = slice(h * (heads // n_kv), (h + 1) * (heads // n_kv))
+            k, v = (ref.get_rows(data, slots, h, is_v, cdtype, dim, page) for is_v in (0, 1))
+            with np.errstate(invalid="ignore"):
+                k, v = np.where(np.isfinite(k), k, 0), np.where(np.isfinite(v), v, 0)
+            qq, mask = q[lo:hi, g], seen[:, None]
+            s = np.where(mask, np.einsum("qgd,td->qgt", qq, k) * scale, -np.inf)
+            m = s.max(-1, keepdims=True)
+            p = np.exp(s - np.where(np.isfinite(m), m, 0))
+            total = p.sum(-1, keepdims=True)
+            p /= np.where(total > 0, total, 1)
+            e = scale * ((2.0 ** -11 + 2.0 ** -17) * np.einsum("qgd,td->qgt", np.abs(qq), np.abs(k)) + 2.0 ** -34 * np.abs(qq).max(-1)[..., None] * np.abs(k).sum(-1)) + 2.0 ** -20
+            e = np.where(mask & (p > 0), e, 0) * (1 + 2.0 ** -6)
+            w = p @ v
+            want[lo:hi, g] = w
+            tol[lo:hi, g] = 2.0 ** -8 * np.abs(w) + (p * (e + (p * e).sum(-1, keepdims=True) + 2.0 ** -10 + 2.0 ** -19) + np.minimum(p, 2.0 ** -34)) @ np.abs(v)
+    return want, tol
+
+
+def takes_prompt_kernel(api, cache):
+    """The last call went to the kernel for prompt chunks: it alone needs no scratch for long contexts."""
+    a = api.keep[3]
+    longer = api.l3m.Kv4Attend(dtype=a.dtype, n_heads=a.n_heads, n_req=a.n_req, max_q=a.max_q, max_blocks=1 << 12, max_kv=1 << 16)
+    return api.lib.l3m_kv4_attend_scratch(C.byref(cache), C.byref(longer)) == 16
+
+
+@pytest.mark.parametrize("dim,heads,kh", [(64, 64, 64), (128, 32, 32)])
+@pytest.mark.parametrize("at", [160, 101, 199])
+def test_prompt_rows_before_an_mxfp4_scale_that_is_not_finite(api, dim, heads, kh, at):
+    rng, page, lens, new = np.random.default_rng(at), 16, [200, 150], 100
+    tables, q_start, host, k, v = far_case(rng, ref.MX, lens, [new] * 2, kh, page, dim)
+    q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, BF16)
+    want, tol = prompt_want(q64, q_start, lens, tables, host, ref.MX, dim, page, kh, 0.125)
+    for cells in (k, v):
+        of_token(cells, tables, 0, at, page)[...] = 255
+    cache = api.cache(api.put(host), ref.MX, page, kh, dim)
+    out, _ = api.attend(cache, q, q_start, lens, tables, 0.125)
+    assert takes_prompt_kernel(api, cache)
+    before = at - (lens[0] - new)
+    check_prompt(out[:before], want[:before], tol[:before])
+    check_prompt(out[new:], want[new:], tol[new:])
