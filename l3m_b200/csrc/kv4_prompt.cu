@@ -15,7 +15,7 @@
 //
 // Scales. A widened value is an f16 number, code times scale, rounded once; scales are first multiplied by a power of two that
 // brings the context's largest near 2^11 (found in a first pass over the scales alone: 1/9 of the cache), undone in the scores'
-// factor and in the result. Queries are brought to 2^10 by row. P is 2^14 at most: the reference moves when a score
+// factor and in the result. Where the smallest would then lose bits (kReach below), plain_rows() takes the CTA's rows. Queries are brought to 2^10 by row. P is 2^14 at most: the reference moves when a score
 // passes it by 14 (then to 10 below the largest), which multiplies O by a power of two.
 //
 // Bound: the tensor pipe inside a CTA (75% of its rate while one runs), the last wave of CTAs outside. 2 chunks of 1024 over up to
@@ -187,7 +187,7 @@ struct Smem {
     uint64_t k_full[2], v_full[2], k_empty[2], v_empty[2];
     uint64_t s_full[2][2], p_full[2][2], pv_done[2], end[2];   // [tile][half]
     uint32_t tmem, bad[4][4];             // tokens of a step in no page of the cache, a ring of four steps
-    int k_top, v_top;
+    int k_top, v_top, k_low, v_low;       // the largest and the smallest exponent of the scales
 };
 
 // One token's keys or values as they lie in the cache.
@@ -196,6 +196,158 @@ struct Codes {
     uint32_t w[4 * NG], sc[MX ? 1 : NG / 2];
     bool there;
 };
+
+// What a CTA does: its request, kv head and first row. The last rows first, they see most.
+__device__ __forceinline__ void place(const PromptArgs &p, int &r, int &h, int &row0) {
+    const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
+    r = x / per_req;
+    h = (x - r * per_req) / p.row_tiles;
+    row0 = (p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles)) * 2 * kRows;
+}
+
+// A CTA's rows in 32 bits, for contexts whose scales lie further apart than widened numbers reach. A warp takes 8 rows at a time over the whole
+// context, 32 tokens at a step: a lane forms one token's scores, then sums 4 dims of the values. It decodes a token for 8 rows, not 256, without
+// tensor cores: 2 chunks of 1024 over 6000 tokens, 32 heads to 8 of 128, mxfp4, 19 ms in place of 248 us. buf: 8 rows' queries and probabilities a warp.
+template <int NG, int MX>
+__device__ __noinline__ void plain_rows(const PromptArgs &p, int k_up, int v_up, float *buf) {
+    constexpr int R = 8, DP = 32 * NG, SB = MX ? 1 : 2, kWarps = kPromptThreads / 32;
+    static_assert(kWarps * R * (DP + 32) * 4 <= 4 * kRows * DP * 2, "the warps' buffers fit the operands'");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int r, h, row0;
+    place(p, r, h, row0);
+    const Queries rq = queries_of(p.a, r);
+    const int rows = min(rq.nq * p.group - row0, 2 * kRows);
+    float *q = buf + warp * R * (DP + 32), *prob = q + R * DP;
+    const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
+    // A scale's value times 2^up; 0 for what is not finite.
+    auto scale = [&](const uint8_t *at, int up) -> float {
+        if (MX) return *at == 255 ? 0.0f : scale2(exp2i(*at - 127), up);
+        const uint32_t x = *(const uint16_t *)at;
+        return (x & 0x7c00) == 0x7c00 ? 0.0f : scale2(__half2float(__ushort_as_half((unsigned short)x)), up);
+    };
+    auto code = [](uint32_t n) -> float {
+        if (!MX) return (float)(int)n - 8.0f;
+        const float m = (float)(0xC8643210u >> 4 * (n & 7) & 15) * 0.5f;
+        return n & 8 ? -m : m;
+    };
+    for (int g0 = warp * R; g0 < rows; g0 += kWarps * R) {
+        int at[R];                                                           // the rows' positions
+        float mult[R], m[R], l[R], o[R][4];
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            const int row = row0 + g0 + i, qi = row / p.group, head = h * p.group + row - qi * p.group;
+            const bool live = g0 + i < rows;
+            const __nv_bfloat16 *src = (const __nv_bfloat16 *)p.a.q + (size_t)(rq.start + qi) * p.a.q_ld + (size_t)head * p.c.dim;
+            float x[NG], top = 0.0f;
+#pragma unroll
+            for (int j = 0; j < NG; j++) {
+                x[j] = live && 32 * j + lane < p.c.dim ? __bfloat162float(src[32 * j + lane]) : 0.0f;
+                top = fmaxf(top, fabsf(x[j]));
+            }
+#pragma unroll
+            for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const int up = top > 0.0f ? 9 - max(min(ilogbf(top), 127), -149) : 0;
+#pragma unroll
+            for (int j = 0; j < NG; j++) q[i * DP + 32 * j + lane] = scale2(x[j], up);
+            mult[i] = scale2(p.a.scale * 1.4426950408889634f, -up - k_up);
+            at[i] = live ? rq.at + qi : -1;
+            m[i] = -INFINITY;
+            l[i] = 0.0f;
+#pragma unroll
+            for (int d = 0; d < 4; d++) o[i][d] = 0.0f;
+        }
+        __syncwarp();
+        const int i1 = min(g0 + R, rows) - 1, first = rq.at + (row0 + g0) / p.group, last = rq.at + (row0 + i1) / p.group;
+        const int lo = p.a.window ? max(0, first - p.a.window + 1) : 0, hi = last + 1;
+#pragma unroll 1
+        for (int t0 = lo & ~31; t0 < hi; t0 += 32) {
+            const int tok = t0 + lane;
+            const uint8_t *tile = nullptr;
+            if (tok >= lo && tok < hi) {
+                const int blk = tok / p.c.page, off = tok - blk * p.c.page, id = table[blk];
+                if (id >= 0 && id < p.c.n_pages) tile = p.c.data + p.c.tile_at(id, h, off / kKvTile);
+                else if (p.a.status) atomicOr((int *)p.a.status, L3M_KV4_BAD_PAGE);
+            }
+            const int row16 = tok % p.c.page % kKvTile;
+            float s[R];
+#pragma unroll
+            for (int i = 0; i < R; i++) s[i] = 0.0f;
+            if (tile) {
+#pragma unroll 1
+                for (int j = 0; j < NG; j++) {
+                    const float d = scale(tile + 512 * NG + (row16 * NG + j) * SB, k_up);
+                    float acc[R];
+#pragma unroll
+                    for (int i = 0; i < R; i++) acc[i] = 0.0f;
+#pragma unroll 1
+                    for (int t = 0; t < 4; t++) {
+                        const uint32_t w = ((const uint32_t *)(tile + row16 * 16 * NG))[t * NG + j];
+                        float c[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) c[e] = code(w >> 4 * e & 15);
+#pragma unroll
+                        for (int i = 0; i < R; i++) {
+                            const float4 a = *(const float4 *)(q + i * DP + 32 * j + 8 * t), b = *(const float4 *)(q + i * DP + 32 * j + 8 * t + 4);
+                            acc[i] = fmaf(a.x, c[0], fmaf(a.y, c[1], fmaf(a.z, c[2], fmaf(a.w, c[3], acc[i]))));
+                            acc[i] = fmaf(b.x, c[4], fmaf(b.y, c[5], fmaf(b.z, c[6], fmaf(b.w, c[7], acc[i]))));
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < R; i++) s[i] = fmaf(acc[i], d, s[i]);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < R; i++) {
+                const bool seen = tile && tok <= at[i] && !(p.a.window && tok <= at[i] - p.a.window);
+                const float z = seen ? s[i] * mult[i] : -INFINITY;
+                float top = z;
+#pragma unroll
+                for (int d = 16; d; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                if (top > m[i]) {
+                    const float f = m[i] == -INFINITY ? 0.0f : ex2(m[i] - top);
+                    m[i] = top;
+                    l[i] *= f;
+#pragma unroll
+                    for (int d = 0; d < 4; d++) o[i][d] *= f;
+                }
+                const float e = seen ? ex2(z - m[i]) : 0.0f;
+                l[i] += e;
+                prob[i * 32 + lane] = e;
+            }
+            __syncwarp();
+            // the values: lane = 4 dims, part lane / NG of block lane % NG
+#pragma unroll 1
+            for (int t = 0; t < 32; t++) {
+                const uint8_t *from = (const uint8_t *)__shfl_sync(0xffffffffu, (unsigned long long)tile, t);
+                if (!from || lane >= 8 * NG) continue;
+                const int vrow = (t0 + t) % p.c.page % kKvTile, j = lane % NG;
+                const uint32_t w = ((const uint16_t *)(from + 256 * NG + vrow * 16 * NG))[lane];
+                const float d = scale(from + 512 * NG + kKvTile * NG * SB + (vrow * NG + j) * SB, v_up);
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) v[e] = code(w >> 4 * e & 15) * d;
+#pragma unroll
+                for (int i = 0; i < R; i++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) o[i][e] = fmaf(prob[i * 32 + t], v[e], o[i][e]);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int i = 0; i < R; i++) {
+            float total = l[i];
+#pragma unroll
+            for (int d = 16; d; d >>= 1) total += __shfl_xor_sync(0xffffffffu, total, d);
+            const int row = row0 + g0 + i, qi = row / p.group, head = h * p.group + row - qi * p.group, d0 = 32 * (lane % NG) + 4 * (lane / NG);
+            if (g0 + i >= rows || lane >= 8 * NG || d0 >= p.c.dim) continue;
+            __nv_bfloat16 *dst = (__nv_bfloat16 *)p.a.out + (size_t)(rq.start + qi) * p.a.out_ld + (size_t)head * p.c.dim + d0;
+            const float inv = total != 0.0f ? 1.0f / total : 0.0f;
+#pragma unroll
+            for (int e = 0; e < 4; e++) dst[e] = __float2bfloat16_rn(inv == 0.0f ? 0.0f : scale2(o[i][e] * inv, -v_up));
+        }
+    }
+}
 
 template <int NG, int MX>
 __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_constant__ PromptArgs p) {
@@ -206,12 +358,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- what this CTA does: the last rows first, they see most
-    const int x = blockIdx.x, per_req = p.c.n_kv * p.row_tiles;
-    const int r = x / per_req, h = (x - r * per_req) / p.row_tiles, rt = p.row_tiles - 1 - (x - r * per_req - h * p.row_tiles);
+    int r, h, row0;
+    place(p, r, h, row0);
     const Queries rq = queries_of(p.a, r);
     const int start = rq.start, nq = rq.nq;
-    const int row0 = rt * 2 * kRows, rows = nq * p.group - row0;           // rows left from this CTA's first
+    const int rows = nq * p.group - row0;                                  // rows left from this CTA's first
     if (rows <= 0) return;
     const int tiles = rows > kRows ? 2 : 1;
     const int i0 = row0 / p.group, i1 = min((row0 + 2 * kRows - 1) / p.group, nq - 1), first = rq.at + i0, last = rq.at + i1;   // the rows' positions
@@ -234,6 +385,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
             bar_init(&s.end[b], 1);
         }
         s.k_top = s.v_top = 0;
+        s.k_low = s.v_low = 1 << 20;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == kSoftWarps + kWideWarps) {
@@ -248,29 +400,68 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
         return id >= 0 && id < p.c.n_pages ? p.c.data + p.c.tile_at(id, h, off / kKvTile) : nullptr;
     };
 
-    // ---- the largest scales' exponents, while the softmax's warps bring in the queries
+    // ---- the scales' exponents, while the softmax's warps bring in the queries
     if (warp >= kSoftWarps) {
-        int kt = 0, vt = 0;
-#pragma unroll 8
-        for (int tok = lo_any + tid - 32 * kSoftWarps; tok < hi_any; tok += kPromptThreads - 32 * kSoftWarps) {
-            const uint8_t *tile = tile_of(tok);
-            if (!tile) continue;
-            const int row = tok % p.c.page % kKvTile;
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                const uint8_t *ks = tile + 512 * NG + (row * NG + j) * SB, *vs = ks + kKvTile * NG * SB;
-                const int ke = MX ? *ks : *(const uint16_t *)ks >> 10 & 31, ve = MX ? *vs : *(const uint16_t *)vs >> 10 & 31;
-                kt = max(kt, ke == (MX ? 255 : 31) ? 0 : ke);               // what is not finite sets no scale for the rest
-                vt = max(vt, ve == (MX ? 255 : 31) ? 0 : ve);
+        // Largest and smallest in 16-bit pairs: e8m0 bytes, or the bits of f16 numbers without their signs. A scale of 0 or one that is not finite sets
+        // nothing for the rest: a pass that meets one is done again one by one.
+        uint32_t kt = 0, vt = 0, kl = 0, vl = 0, odd = 0;
+        auto count = [&](uint32_t x, uint32_t &top, uint32_t &low) {
+            if (MX) {
+                odd |= (((x - 0x01010101u) & ~x) | ((~x - 0x01010101u) & x)) & 0x80808080u;
+                const uint32_t y = x & 0x00ff00ffu, z = x >> 8 & 0x00ff00ffu;
+                top = __vmaxu2(top, __vmaxu2(y, z));
+                low = __vminu2(low, __vminu2(y, z));
+            } else {
+                x &= 0x7fff7fffu;
+                odd |= ((x + 0x04000400u) | ((x - 0x00010001u) & ~x)) & 0x80008000u;
+                top = __vmaxu2(top, x);
+                low = __vminu2(low, x);
             }
-        }
-        for (int o = 16; o; o >>= 1) {
-            kt = max(kt, __shfl_xor_sync(0xffffffffu, kt, o));
-            vt = max(vt, __shfl_xor_sync(0xffffffffu, vt, o));
-        }
+        };
+        auto count_good = [](uint32_t x, uint32_t &top, uint32_t &low) {
+#pragma unroll
+            for (int k = 0; k < 32; k += 8 * SB) {
+                const uint32_t e = x >> k & (MX ? 0xff : 0x7fff);
+                if (e && e < (MX ? 255 : 0x7c00)) top = __vmaxu2(top, e), low = __vminu2(low, e | 0xffff0000u);
+            }
+        };
+        auto scan = [&](auto each) {
+            kt = vt = odd = 0;
+            kl = vl = ~0u;
+#pragma unroll 8
+            for (int tok = lo_any + tid - 32 * kSoftWarps; tok < hi_any; tok += kPromptThreads - 32 * kSoftWarps) {
+                const uint8_t *tile = tile_of(tok);
+                if (!tile) continue;
+                const int row = tok % p.c.page % kKvTile;
+                const uint8_t *ks = tile + 512 * NG + row * NG * SB, *vs = ks + kKvTile * NG * SB;
+                if constexpr (NG * SB == 2) {                                // two bytes, twice
+                    each(*(const uint16_t *)ks * 0x00010001u, kt, kl);
+                    each(*(const uint16_t *)vs * 0x00010001u, vt, vl);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < NG * SB / 4; i++) {
+                        each(((const uint32_t *)ks)[i], kt, kl);
+                        each(((const uint32_t *)vs)[i], vt, vl);
+                    }
+                }
+            }
+        };
+        scan(count);
+        if (odd) scan(count_good);
+        auto exponent = [](uint32_t x) { return MX || x >= 0x400 ? (int)(MX ? x : x >> 10) : 22 - __clz(x); };      // an f16 subnormal's by its highest bit, -9 .. 0
+        kt = __reduce_max_sync(0xffffffffu, max(kt & 0xffff, kt >> 16));
+        vt = __reduce_max_sync(0xffffffffu, max(vt & 0xffff, vt >> 16));
+        kl = __reduce_min_sync(0xffffffffu, min(kl & 0xffff, kl >> 16));
+        vl = __reduce_min_sync(0xffffffffu, min(vl & 0xffff, vl >> 16));
         if (lane == 0) {
-            atomicMax(&s.k_top, kt);
-            atomicMax(&s.v_top, vt);
+            if (kt) {
+                atomicMax(&s.k_top, max(exponent(kt), 0));
+                atomicMin(&s.k_low, exponent(kl));
+            }
+            if (vt) {
+                atomicMax(&s.v_top, max(exponent(vt), 0));
+                atomicMin(&s.v_low, exponent(vl));
+            }
         }
     }
     const int tile = warp / 4;                                              // of a softmax warp
@@ -324,9 +515,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) prompt_kernel(const __grid_
     const uint32_t tmem = s.tmem;
     // q4_0: d < 2^(top - 14), brought below 2^11. mxfp4: 2^(top - 127), brought to 2^11.
     const int k_up = MX ? 11 + 127 - s.k_top : 25 - s.k_top, v_up = MX ? 11 + 127 - s.v_top : 25 - s.v_top;
+    // What f16 holds below the largest without loss: mxfp4's numbers of two bits down to 2^-24 (0.5 times 2^-34 of the largest scale 2^11), q4_0's
+    // code times scale with 11 bits down to 2^-14 (a scale of 2^-24 of the largest)
+    constexpr int kReach = MX ? 34 : 24;
     bool ok = true;
 
-    if (warp >= kSoftWarps && warp < kSoftWarps + kWideWarps) {
+    if (s.k_top - s.k_low > kReach && s.k_low <= s.k_top || s.v_top - s.v_low > kReach && s.v_low <= s.v_top) {
+        plain_rows<NG, MX>(p, k_up, v_up, (float *)s.k);
+    } else if (warp >= kSoftWarps && warp < kSoftWarps + kWideWarps) {
         // ---- widening: thread = token of the step
         const int tk = tid & (kStep - 1);
         const bool values = warp >= kSoftWarps + kWideWarps / 2;

@@ -273,3 +273,88 @@ def test_prompt_rows_before_an_mxfp4_scale_that_is_not_finite(api, dim, heads, k
     before = at - (lens[0] - new)
     check_prompt(out[:before], want[:before], tol[:before])
     check_prompt(out[new:], want[new:], tol[new:])
+
+
+WIDE = [(ref.Q4, 20), (ref.Q4, 28), (ref.MX, 20), (ref.MX, 33), (ref.MX, 35), (ref.MX, 60)]
+
+
+@pytest.mark.parametrize("cdtype,gap", WIDE)
+@pytest.mark.parametrize("window", [0, 37])
+@pytest.mark.parametrize("dim,heads,kh,lens,new", [(64, 64, 32, [300, 150], 100), (104, 48, 16, [200, 130], 130), (128, 32, 32, [260, 120], 120), (48, 90, 30, [129, 257], 129)])
+def test_prompt_scales_far_apart(api, cdtype, gap, window, dim, heads, kh, lens, new):
+    """Values' blocks 2^gap apart in all tokens; tokens whose values are 2^gap times the others' and which nobody attends to; and keys whose blocks are
+    far apart, with queries that are zero in the large one. Below and above the reach of widened numbers, which is 2^24 (q4_0) and 2^34 (mxfp4)."""
+    rng, page = np.random.default_rng(gap + dim), 16
+    ng = ref.blocks(dim)
+    for kind in ("value blocks", "ignored tokens", "key blocks"):
+        tables, q_start, host, k, v = far_case(rng, cdtype, lens, [new] * 2, kh, page, dim)
+        q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, BF16)
+        scale = float(np.float32(0.125))
+        if kind == "ignored tokens":
+            q, q64 = q.abs(), np.abs(q64)
+            for r, n in enumerate(lens):
+                for t in rng.choice(n, 5, replace=False):
+                    of_token(v, tables, r, t, page)[...] = 0.001 * 2.0 ** min(gap, 25) if cdtype == ref.Q4 else 124 + gap
+                    tile = host[tables[r, t // page], :, t % page // 16]
+                    tile[:, t % 16 * 16 * ng:t % 16 * 16 * ng + 16 * ng] = 0x00 if cdtype == ref.Q4 else 0xFF
+                    of_token(k, tables, r, t, page)[...] = 4.0 if cdtype == ref.Q4 else 130
+            if cdtype == ref.Q4:
+                ordinary = np.abs(v) < 30
+                v[...] = np.where(ordinary, v * np.float16(2.0 ** -9), v)
+        else:
+            cells = v if kind == "value blocks" else k
+            for j in range(1, ng):
+                cells[..., j] = (cells[..., j] * 2.0 ** (-gap / 2)).astype(np.float16) if cdtype == ref.Q4 else cells[..., j] - gap // 2
+            cells[..., 0] = cells[..., 0] * np.float16(2.0 ** (gap / 2)) if cdtype == ref.Q4 else cells[..., 0] + (gap + 1) // 2
+            if kind == "key blocks":
+                q[..., :32] = 0
+                q64 = q.double().cpu().numpy()
+                scale = float(np.float32(0.1 * 2.0 ** (gap / 2)))
+        cache = api.cache(api.put(host), cdtype, page, kh, dim)
+        out, st = api.attend(cache, q, q_start, lens, tables, scale, window)
+        assert takes_prompt_kernel(api, cache) and st.item() == 0
+        check_prompt(out, *prompt_want(q64, q_start, lens, tables, host, cdtype, dim, page, kh, scale, window), norm=False)
+
+
+@pytest.mark.parametrize("cdtype,big", [(ref.Q4, 60000.0), (ref.MX, 160), (ref.MX, 200), (ref.MX, 254)])
+def test_prompt_scales_that_only_later_queries_see(api, cdtype, big):
+    """A token in the middle of a chunk with the largest scales there are: the queries before it, in the same tiles of rows, do not know."""
+    rng, dim, page, lens, new, heads, kh = np.random.default_rng(3), 64, 16, [200, 150], 100, 64, 64
+    for at in (101, 160, 199):
+        tables, q_start, host, k, v = far_case(rng, cdtype, lens, [new] * 2, kh, page, dim)
+        if cdtype == ref.Q4:
+            k *= np.float16(2.0 ** -12)
+            v *= np.float16(2.0 ** -12)
+        scale = 0.125 * (4096 if cdtype == ref.Q4 else 1)
+        q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, BF16)
+        want, tol = prompt_want(q64, q_start, lens, tables, host, cdtype, dim, page, kh, scale)
+        for cells in (k, v):
+            of_token(cells, tables, 0, at, page)[...] = big
+        cache = api.cache(api.put(host), cdtype, page, kh, dim)
+        out, _ = api.attend(cache, q, q_start, lens, tables, scale)
+        assert takes_prompt_kernel(api, cache)
+        before = at - (lens[0] - new)
+        check_prompt(out[:before], want[:before], tol[:before], norm=False)
+        check_prompt(out[new:], want[new:], tol[new:], norm=False)
+
+
+def test_prompt_scales_far_apart_with_strides_bad_pages_and_rows_that_see_nothing(api, torch):
+    """The same contexts where they meet the rest: spare columns, odd addresses, pages outside the cache, more queries than tokens."""
+    rng, dim, page, lens, news, heads, kh = np.random.default_rng(4), 48, 16, [0, 3, 250, 180], [60, 70, 133, 100], 60, 30
+    tables, q_start, host, k, v = far_case(rng, ref.MX, lens, news, kh, page, dim)
+    v[..., 0] += 60
+    tables[2, 3], tables[2, 15] = -1, host.shape[0]
+    q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, BF16)
+    rows, width, cache = q.shape[0], heads * dim, api.cache(api.put(host), ref.MX, page, kh, dim)
+    flat = torch.full((rows * (width + 13) + 1,), float("nan"), dtype=torch.bfloat16, device="cuda")
+    qs = flat.as_strided((rows, heads, dim), (width + 13, dim, 1), 1)
+    qs.copy_(q)
+    space = torch.full((rows * (width + 13) + 1,), 5.0, dtype=torch.bfloat16, device="cuda")
+    out, st = api.attend(cache, qs, q_start, lens, tables, 0.2, out=space.as_strided((rows, heads, dim), (width + 13, dim, 1), 1))
+    assert takes_prompt_kernel(api, cache) and st.item() == ref.BAD_PAGE
+    assert (space[1:].view(rows, width + 13)[:, width:] == 5).all() and (out[:60] == 0).all() and (out[60:127] == 0).all()
+    want, spread = ref.attend(q64, q_start, lens, tables, host, ref.MX, dim, page, kh, float(np.float32(0.2)))
+    # plain sums in 32 bits: a score of |q k| scale below 2^4 is off by 2^-17 at most, a probability by 2^-16, and the result is rounded to bf16
+    assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * spread).all()
+    api.attend(cache, q, q_start, lens, tables, 0.2)
+    assert torch.equal(api.keep[5], out)
