@@ -31,6 +31,7 @@ int launched(cudaError_t e, const char *entry) {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMaxReq = 16384;
+constexpr size_t plan_smem(int n_req) { return (size_t)3 * (n_req + 1) * 4 + n_req; }
 
 struct PlanArgs {
     l3m_kv4_plan a;
@@ -760,8 +761,9 @@ L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream) {
          (uintptr_t)a->q_start | (uintptr_t)a->kv_total | (uintptr_t)a->slot | (uintptr_t)a->pos | (uintptr_t)a->status) & 3)
         return refuse(me, "a pointer is not aligned to its type");
     PlanArgs p = {*a};
-    const size_t smem = (size_t)3 * (a->n_req + 1) * 4 + a->n_req;
-    const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    // The limit is the function's, not the call's: always the same, so that no other host thread's call lowers it before this one's launch.
+    const size_t smem = plan_smem(a->n_req);
+    const cudaError_t e = cudaFuncSetAttribute(plan_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)plan_smem(kPlanMaxReq));
     if (e != cudaSuccess) return l3m_error_cuda(e, me);
     const int threads = a->n_req <= 128 && a->max_tokens <= 2048 ? 128 : kPlanThreads;
     const int grid = std::max(1, std::min(sm_count(), (a->max_tokens + threads - 1) / threads));

@@ -358,3 +358,43 @@ def test_prompt_scales_far_apart_with_strides_bad_pages_and_rows_that_see_nothin
     assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(want) + 2.0 ** -14 * spread).all()
     api.attend(cache, q, q_start, lens, tables, 0.2)
     assert torch.equal(api.keep[5], out)
+
+
+# ---- plan
+
+def test_plans_of_two_host_threads(api, torch):
+    """Two threads plan steps of very different sizes on streams of their own, many times: no call of one is refused for the other's, and both
+    have their results."""
+    import threading
+    rng, page, jobs = np.random.default_rng(60), 16, []
+    for n in (16384, 1):
+        kv, new = rng.integers(0, 33, n).astype(np.int32), np.ones(n, np.int32)
+        held, after = -(-kv // page), -(-(kv + 1) // page)
+        order = rng.permutation(int(after.sum()) + 5).astype(np.int32)
+        tables = np.full((n, 3), -1, np.int32)
+        tables[np.arange(3)[None] < held[:, None]] = order[:int(held.sum())]
+        free = np.concatenate((order[int(held.sum()):], np.full(int(held.sum()), -1, np.int32)))
+        n_free = len(order) - int(held.sum())
+        want = ref.plan(kv, new, tables, free, n_free, page, n)
+        t = {k: api.put(np.asarray(v, np.int32)) for k, v in dict(kv_len=kv, new_len=new, tables=tables, free_pages=free, n_free=[n_free]).items()}
+        for k, size in dict(n_free_out=1, q_start=n + 1, kv_total=n, slot=n, pos=n, status=1).items():
+            t[k] = torch.zeros(size, dtype=torch.int32, device="cuda")
+        jobs.append((api.l3m.Kv4Plan(n_req=n, max_blocks=3, max_tokens=n, page=page, n_pages=len(free), **{k: v.data_ptr() for k, v in t.items()}), t, want, torch.cuda.Stream(), []))
+    torch.cuda.synchronize()
+
+    def work(args, stream, bad):
+        for _ in range(3000):
+            if api.lib.l3m_kv4_plan_dev(C.byref(args), stream.cuda_stream):
+                bad.append(api.lib.l3m_cuda_error())
+
+    threads = [threading.Thread(target=work, args=(args, stream, bad)) for args, _, _, stream, bad in jobs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    torch.cuda.synchronize()
+    for _, t, want, _, bad in jobs:
+        assert not bad, bad[:3]
+        for k in ("tables", "q_start", "kv_total", "slot", "pos"):
+            assert np.array_equal(t[k].cpu().numpy(), want[k]), k
+        assert t["n_free_out"].item() == want["n_free_out"] and t["status"].item() == 0
