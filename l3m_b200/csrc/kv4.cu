@@ -266,7 +266,9 @@ struct QkvArgs {
     int chunks, per_chunk;                // warps per token and the groups each takes
 };
 
-__device__ __forceinline__ double finite(double x) { return x != x ? 0.0 : fmin(fmax(x, -(double)FLT_MAX), (double)FLT_MAX); }
+__device__ __forceinline__ double finite(double x) { return x != x ? 0.0 : isinf(x) ? copysign((double)FLT_MAX, x) : x; }
+// A mean square, eps included, whose square root 32 bits have: sums of squares lose nothing above and do not overflow below.
+__device__ __forceinline__ bool sound(float mean) { return mean > 0x1p-100f && mean < 0x1p100f; }
 
 // What a lane stores of its row: the codes of its 8 values and its block's scale bits.
 struct Held { unsigned codes, scale; };
@@ -317,15 +319,16 @@ template <int KIND> __device__ __forceinline__ void put_row(const QkvArgs &p, co
     }
 }
 
-// Group g by the definition, in 64 bits: for rows whose 32-bit values lie too near a border.
+// Group g by the definition, in 64 bits: for rows whose 32-bit values lie too near a border, or whose squares leave 32 bits' range.
 template <typename T, int LPR, int ROPE, int KIND>
 __device__ __noinline__ void exact_rows(const QkvArgs &p, int tok, Place to, const float *turn, int g) {
     const l3m_qkv &a = p.a;
     const int wl = threadIdx.x & 31, lane = wl & (LPR - 1), d0 = lane * 8, h = g * (32 / LPR) + wl / LPR, D = a.head_dim;
-    const int rot = KIND == kKey && ROPE ? a.rot_dim : 0, half = rot / 2;
-    const bool live = h < a.n_kv_heads, mine = live && d0 < D;
-    const T *src = (const T *)(KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kKey ? a.k_ld : a.v_ld) + (size_t)h * D;
-    const float *w = KIND == kKey ? a.k_norm : nullptr;
+    const int rot = KIND != kValue && ROPE ? a.rot_dim : 0, half = rot / 2;
+    const bool live = h < (KIND == kQuery ? a.n_heads : a.n_kv_heads), mine = live && d0 < D;
+    const T *src = (const T *)(KIND == kQuery ? a.q : KIND == kKey ? a.k : a.v) + (size_t)tok * (KIND == kQuery ? a.q_ld : KIND == kKey ? a.k_ld : a.v_ld) + (size_t)h * D;
+    const float *w = KIND == kQuery ? a.q_norm : KIND == kKey ? a.k_norm : nullptr;
+    T *out = KIND == kValue ? nullptr : (T *)(KIND == kQuery ? a.q_out : a.k_out);
     double u[8], ss = 0.0, f = 1.0;
 #pragma unroll 1
     for (int e = 0; e < 8; e++) {
@@ -346,12 +349,13 @@ __device__ __noinline__ void exact_rows(const QkvArgs &p, int tok, Place to, con
     for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
     if (w) f = 1.0 / sqrt(ss / D + (double)a.eps);
     __syncwarp();                                                        // in place: every lane has read its row
-    if (KIND == kKey && a.k_out && mine) {
+    if (KIND != kValue && out && mine) {
         float x[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = (float)(u[e] * f);
-        store8<false>((T *)a.k_out + (size_t)tok * a.k_out_ld + (size_t)h * D + d0, x, 1.0f);
+        store8<false>(out + (size_t)tok * (KIND == kQuery ? a.q_out_ld : a.k_out_ld) + (size_t)h * D + d0, x, 1.0f);
     }
+    if (KIND == kQuery || !to.tile) return;
     f = finite(f);
     double top = 0.0;
     int at = 0;
@@ -469,13 +473,16 @@ struct RowWorker {
             src += step;
             if (g + 1 < g1 && h + RPW < heads && in) next.template load<VEC>(src);
             float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value
+            bool near = false;
             if (KIND != kValue && w) {
                 float ss = 0.0f;
 #pragma unroll
                 for (int e = 0; e < 8; e++) ss = fmaf(u[e], u[e], ss);
 #pragma unroll
                 for (int o = LPR / 2; o; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                f = rsqrtf(fmaf(ss, inv_d, a.eps));
+                const float mean = fmaf(ss, inv_d, a.eps);
+                near = !sound(mean);
+                f = rsqrtf(mean);
 #pragma unroll
                 for (int e = 0; e < 8; e++) u[e] *= wt[e];
             }
@@ -511,13 +518,14 @@ struct RowWorker {
             }
             Held held = {0, 0};
             if (KIND != kQuery && to.tile) {
-                bool near;
-                held = quantise<KIND>(u, size, f, w, &near);
-                if (__any_sync(0xffffffffu, near && live)) {
-                    left |= 1ull << (g - g0);
-                    if (KIND == kKey && out) out += step;
-                    continue;
-                }
+                bool close;
+                held = quantise<KIND>(u, size, f, w, &close);
+                near |= close;
+            }
+            if ((KIND != kValue || to.tile) && __any_sync(0xffffffffu, near && live)) {
+                left |= 1ull << (g - g0);
+                if (KIND != kValue && out) out += step;
+                continue;
             }
             if (KIND != kValue && out) {
                 __syncwarp();                                                // in place: every lane has read its row
@@ -651,7 +659,8 @@ __global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const __grid_consta
             }
         }
         if (g0 < p.q_groups + p.k_groups) w.rotation(pos);
-        if (g0 < p.q_groups) w.template rows<kQuery>(g0, min(g1, p.q_groups));
+        for (int g = g0; g < min(g1, p.q_groups); g += 64)
+            for (unsigned long long left = w.template rows<kQuery>(g, min(g + 64, min(g1, p.q_groups))); left; left &= left - 1) exact_rows<T, LPR, ROPE, kQuery>(p, tok, w.to, w.turn, g + __ffsll(left) - 1);
         const int k0 = p.q_groups, v0 = p.q_groups + p.k_groups;
         for (int g = max(g0 - k0, 0); g < min(g1, v0) - k0; g += 64)
             for (unsigned long long left = w.template rows<kKey>(g, min(g + 64, min(g1, v0) - k0)); left; left &= left - 1) exact_rows<T, LPR, ROPE, kKey>(p, tok, w.to, w.turn, g + __ffsll(left) - 1);

@@ -6,7 +6,8 @@ import numpy as np
 import pytest
 
 import kv4_ref as ref
-from test_gpu_kv4 import BF16, F32, Api, batch, check_attend, queries, random_cache
+from test_gpu_kv4 import (BF16, F32, Api, batch, check_attend, check_cache, check_rows, qkv_call, qkv_case, qkv_want, queries,
+                          random_cache)
 from test_gpu_kv4_prompt import check as check_prompt
 from test_gpu_kv4_prompt import want_and_tolerance
 
@@ -398,3 +399,47 @@ def test_plans_of_two_host_threads(api, torch):
         for k in ("tables", "q_start", "kv_total", "slot", "pos"):
             assert np.array_equal(t[k].cpu().numpy(), want[k]), k
         assert t["n_free_out"].item() == want["n_free_out"] and t["status"].item() == 0
+
+
+# ---- q, k, v
+
+def put_x(api, c, x):
+    """Other inputs for a case of qkv_case(), as its type holds them."""
+    t = api.torch
+    host = t.from_numpy(x).to(t.float32 if c["dtype"] == F32 else t.bfloat16)
+    c["buf"][c["shift"]:] = host.reshape(-1).cuda()
+    c["x"] = host.double().numpy()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("eps", [1e-5, 1e-38, 0.0])
+@pytest.mark.parametrize("dim,rope,heads,kh", [(64, 0, 3, 2), (64, 2, 3, 2), (128, 1, 5, 3), (256, 2, 1, 1), (24, 2, 9, 5)])
+def test_norms_of_rows_whose_squares_leave_32_bits(api, dtype, cdtype, eps, dim, rope, heads, kh):
+    """Rows from the type's smallest to its largest values, some with one value far above the others: norms, keys and cache are those of the definition
+    in 64 bits, with a cache and without, in place and not."""
+    rng = np.random.default_rng(70 + dim)
+    sizes = [1e-42, 1e-38, 1e-30, 1e-23, 1e-20, 1e-16, 1.0, 1e15, 1e17, 1.5e18, 1e19, 1e25, 1e37, 8e37]
+    for store, in_place in ((True, False), (False, False), (True, True)):
+        c = qkv_case(api, rng, dtype, cdtype, len(sizes) + 4, heads, kh, dim, rope, dim if rope else 0, True)
+        c["eps"] = float(np.float32(eps))
+        x = rng.standard_normal(c["x"].shape).clip(-3, 3)
+        x[np.abs(x) < 0.01] = 0.01
+        x[:len(sizes)] *= np.array(sizes)[:, None]
+        x[-4, ::dim] = 2.0 ** 60
+        x[-3, ::dim] = 2.0 ** 66
+        x[-2] *= np.exp2(rng.integers(-60, 60, x.shape[1]))
+        put_x(api, c, x)
+        q, k, v = qkv_want(c)
+        got_q, got_k, data, status, _ = qkv_call(api, c, store=store, in_place=in_place)
+        assert status == 0
+        for got, (u, f) in ((got_q, q), (got_k, k)):                       # a row of zeros (what bf16 makes of 1e-42) without eps is 0 / 0, stored as 0
+            none = ~np.isfinite(f)
+            got = got.reshape(u.shape)
+            assert np.isnan(got[none]).all()
+            got[none], u[none], f[none] = 0, 0, 1
+            check_rows(got, u, f, c)
+        if store:
+            check_cache(data, c, k, v)
+        else:
+            assert (data == 0x5A).all()
