@@ -415,6 +415,7 @@ struct RowWorker {
     bool in, partial;
     int shift, mate_lane;
     float cs[8], sn[8];                   // cos and sin of this lane's dims, sin with the sign of the mate's term
+    float turn_max;                       // the largest of them in magnitude: tables may carry a factor
     const float *turn;
     Place to;
 
@@ -444,6 +445,11 @@ struct RowWorker {
                     sn[e] = (ROPE == 1 ? e & 1 : d >= half) ? t.y : -t.y;
                 }
             }
+            turn_max = 0.0f;
+            if (p.store) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) turn_max = fmaxf(turn_max, fmaxf(fabsf(cs[e]), fabsf(sn[e])));
+            }
         }
     }
 
@@ -472,7 +478,7 @@ struct RowWorker {
             next.get(u);
             src += step;
             if (g + 1 < g1 && h + RPW < heads && in) next.template load<VEC>(src);
-            float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value
+            float f = 1.0f, size = 0.0f;                                     // size: the largest |a| + |b| behind a value, times the largest |cos| or |sin|
             bool near = false;
             if (KIND != kValue && w) {
                 float ss = 0.0f;
@@ -515,6 +521,7 @@ struct RowWorker {
                     if (KIND == kKey) size = fmaxf(size, fabsf(u[e]) + fabsf(m[e]));
                     u[e] = fmaf(m[e], sn[e], u[e] * cs[e]);
                 }
+                if (KIND == kKey) size *= turn_max;
             }
             Held held = {0, 0};
             if (KIND != kQuery && to.tile) {
@@ -556,7 +563,8 @@ struct RowWorker {
             if (KIND == kKey && ROPE) size = fmaxf(size, __shfl_xor_sync(0xffffffffu, size, o));
         }
         const float mag = fmaxf(hi, -lo);
-        // An upper bound on the error of u: three roundings of |a| + |b| at 2^-24 (the rotation), one of u (the weight).
+        // An upper bound on the error of u: three roundings of (|a| + |b|) max(|cos|, |sin|) at 2^-24 (the weights, a product, the sum); one of u (the
+        // weight) without a rotation.
         const bool exact = KIND == kValue || (!w && !ROPE);
         const float err = exact ? 0.0f : ROPE ? size * 0x1p-22f : mag * 0x1p-23f;
         bool again = !(zero == 0.0f) || (mag < 0x1p-100f && (mag > 0.0f || err > 0.0f)) || mag > 0x1p120f;

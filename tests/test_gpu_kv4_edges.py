@@ -443,3 +443,51 @@ def test_norms_of_rows_whose_squares_leave_32_bits(api, dtype, cdtype, eps, dim,
             check_cache(data, c, k, v)
         else:
             assert (data == 0x5A).all()
+
+
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("factor", [0.01, 1.4, 100.0, 2.0 ** 30])
+@pytest.mark.parametrize("rope,rot", [(1, 128), (2, 128), (2, 96)])
+def test_rotation_tables_that_carry_a_factor(api, cdtype, factor, rope, rot):
+    """cos and sin times a factor, as tables for long contexts have them: codes and scales are still those of exact arithmetic, for rows enough that
+    some lie within the rotation's rounding of a border."""
+    rng = np.random.default_rng(80 + rot)
+    c = qkv_case(api, rng, F32, cdtype, 2500, 1, 4, 128, rope, rot, True, page=64)
+    c["turn"] = (c["turn"] * factor).astype(np.float32)
+    q, k, v = qkv_want(c)
+    got_q, _, data, _, _ = qkv_call(api, c)
+    for is_v, (u, f) in enumerate((k, v)):
+        codes, bits = ref.quantise(u, f, cdtype)
+        want = ref.values(codes, bits, cdtype)
+        for h in range(4):
+            assert np.array_equal(ref.get_rows(data, c["slot"], h, is_v, cdtype, 128, 64), want[:, h])
+    u, f = q
+    pair = np.abs(u)
+    a, b = (slice(0, rot, 2), slice(1, rot, 2)) if rope == 1 else (slice(0, rot // 2), slice(rot // 2, rot))
+    pair[..., a] = pair[..., b] = 2 * (pair[..., a] + pair[..., b])
+    assert (np.abs(got_q.reshape(u.shape) - u * f[..., None]) <= 2.0 ** -24 * np.abs(u * f[..., None]) + 2.0 ** -19 * pair * f[..., None]).all()
+
+
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("factor", [1.0, 1.4, 100.0, 2.0 ** 30])
+@pytest.mark.parametrize("norm", [True, False])
+def test_rotations_that_cancel(api, cdtype, factor, norm):
+    """Keys whose first half cancels in the rotation but for 2^-22 to 2^-12 of it: what is left is a block of its own, with codes and a scale that 32 bits
+    do not have, whatever factor the table carries."""
+    rng = np.random.default_rng(85)
+    c = qkv_case(api, rng, F32, cdtype, 700, 1, 2, 64, 2, 64, norm, page=64)
+    c["turn"] = (c["turn"] * factor).astype(np.float32)
+    x, turn = c["x"].copy(), c["turn"].astype(np.float64)[c["pos"]]
+    w = c["w"][1].astype(np.float64) if norm else np.ones(64)
+    for h in range(2):
+        at = 64 + 64 * h
+        size = rng.standard_normal((700, 32)) * np.exp2(-rng.integers(12, 23, (700, 1)).astype(float))
+        x[:, at:at + 32] = x[:, at + 32:at + 64] * w[32:] * turn[..., 1] * (1 + size) / np.where(np.abs(turn[..., 0]) > 1e-3 * factor, turn[..., 0], factor) / w[:32]
+    put_x(api, c, x)
+    q, k, v = qkv_want(c)
+    _, _, data, _, _ = qkv_call(api, c)
+    for is_v, (u, f) in enumerate((k, v)):
+        codes, bits = ref.quantise(u, f, cdtype)
+        want = ref.values(codes, bits, cdtype)
+        for h in range(2):
+            assert np.array_equal(ref.get_rows(data, c["slot"], h, is_v, cdtype, 64, 64), want[:, h])
