@@ -132,7 +132,7 @@ constexpr int kCtas = 2;                 // resident CTAs per SM
 // took 103 us where two of 4 take 81, one of 4 108: 32 requests of 1000 tokens, 5 queries each, f32, 32 heads to 8 of 128.)
 constexpr int warps_of(int ng, int nt) { return ng * nt <= 5 ? 6 : 4; }
 
-struct Segment { int r, h, rt; };
+constexpr int kMostBase = 4;             // bf16 results over q4_0: the window's base up to which one pass serves, scales below 32
 
 // One piece of a segment (request r, kv head h, row tile rt): cache tiles [a, b), by the CTA's warps. Scores are
 // computed transposed, S^T = K Q^T (16 tokens x 8 rows a product), so that a decode step's few rows pad to 8, not 16, and
@@ -147,6 +147,9 @@ struct Segment { int r, h, rt; };
 // A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
 // them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
 // split in two f16 for float ones.
+template <typename T, int NG, int NT>
+__device__ __noinline__ void far_tiles(const AttendArgs &p, uint8_t *smem, int r, int h, int rt, Queries rq, int a, int b);
+
 template <typename T, int MX, int NG, int NT>
 struct Worker {
     static constexpr int kWarps = warps_of(NG, NT), kThreads = 32 * kWarps;
@@ -155,7 +158,10 @@ struct Worker {
     static constexpr int NR = 8 * NT, DP = 32 * NG, SB = MX ? 1 : 2;
     static constexpr int TB = NG * (512 + 32 * SB);
     static constexpr int RING = kStages * TB;
-    static constexpr int SMEM = kWarps * RING > kWarps * NR * (DP + 4) * 4 ? kWarps * RING : kWarps * NR * (DP + 4) * 4;
+    static constexpr int LD = DP + 4, BUF = kWarps * NR * LD * 4;          // the warps' results, [warp][row][LD]: values, reference, sum
+    // q4_0's bf16 results keep them beside the ring, as a warp may come back to its tiles (run()); the others in its place.
+    static constexpr int BUF_AT = SUBN ? kWarps * RING : 0;
+    static constexpr int SMEM = (BUF_AT + BUF > kWarps * RING ? BUF_AT + BUF : kWarps * RING) + (SUBN ? kWarps * (int)sizeof(AttendArgs) : 0);
     static constexpr int QP = PREC ? 2 : 1;
     static constexpr int NG2 = NG + NG % 2;                                  // blocks, in pairs
     static constexpr int SW = MX ? (NG + 3) / 4 : (NG + 1) / 2;              // words of a row's scales
@@ -171,11 +177,10 @@ struct Worker {
     float o[NT][NG][2][4];
     float w[SUBN ? NT : 1][SUBN ? (NG + 1) / 2 : 1][4];                       // two blocks' sums of P times scale: rows 0-7 block 2i, rows 8-15 block 2i + 1
     // The window of the values' scales that a step's products take as they come: exponents base .. base + 15. mxfp4: a base for each block,
-    // four to a word; the block's sums are in units of 2^(base - 113). q4_0: one base for all blocks, which lowers P's limit. For bf16 results it
-    // stays 4 or less, as P itself is held in f16: larger scales than 32 are brought down to the window.
+    // four to a word; the block's sums are in units of 2^(base - 113). q4_0: one base for all blocks, which lowers P's limit. For bf16 results P itself
+    // is held in f16, so that with a base above 4 (scales of 32 and more) it would have too few bits: the rows are then done again, see run().
     uint32_t base4[MX ? SW : 1];
     int base;
-    static constexpr int kMaxBase = SUBN ? 4 : 16;
     bool begun;
     static constexpr int kFirstBase = 115;                                   // scales of 2^-12 to 2^3, as activations have them; another window costs the first step a little
 
@@ -296,8 +301,8 @@ struct Worker {
     }
 
     // U tiles in shared memory, neighbours in the context. EDGE: some row does not see some of their tokens, which begin at tok0;
-    // [lo_any, hi_any) is seen by some row.
-    template <bool EDGE, int U> __device__ __forceinline__ void step(const uint8_t *sm, int tok0, int lo_any, int hi_any) {
+    // [lo_any, hi_any) is seen by some row. False: their scales do not fit the window, and the tiles have to come one by one, EDGE.
+    template <bool EDGE, int U, bool FAR = false> __device__ __forceinline__ bool step(const uint8_t *sm, int tok0, int lo_any, int hi_any) {
         const int ra = tau(g), t0 = PREC ? ra : t, t1 = 4 + (t ^ 1);
         constexpr int KS = 512 * NG, VS = KS + 16 * NG * SB;
         // ---- scores
@@ -412,7 +417,7 @@ struct Worker {
         load_scales();
         relative();
         // ---- does the reference still hold, do the scales lie in the window?
-        bool far = outside<U>(v);
+        bool far = !FAR && outside<U>(v);
         float lim = limit(), z[U][NT][4], high = kFloor;         // the exponents of P
 #pragma unroll
         for (int u = 0; u < U; u++)
@@ -454,7 +459,7 @@ struct Worker {
                     }
                 }
                 relative();
-            } else if (!MX && __any_sync(0xffffffffu, far)) {
+            } else if (!MX && !FAR && __any_sync(0xffffffffu, far)) {
                 uint32_t top = 0;
 #pragma unroll
                 for (int u = 0; u < U; u++)
@@ -462,11 +467,11 @@ struct Worker {
                     for (int k = 0; k < 4; k += PREC ? 2 : 1)
 #pragma unroll
                         for (int i = 0; i < SW; i++) top = max(top, max(v[u][k][i] >> 10 & 31, v[u][k][i] >> 26 & 31));
-                base = min(max(base, (int)__reduce_max_sync(0xffffffffu, top) - 15), kMaxBase);
+                base = max(base, (int)__reduce_max_sync(0xffffffffu, top) - 15);
                 lim = limit();                                               // raising base lowers it
             }
             begun = true;
-            far = __any_sync(0xffffffffu, outside<U>(v));
+            if (!SUBN) far = __any_sync(0xffffffffu, outside<U>(v));
 #pragma unroll
             for (int n = 0; n < NT; n++) {
                 float f[2];
@@ -497,92 +502,95 @@ struct Worker {
             }
         }
         // ---- probabilities and values
-        if (far) {
-#pragma unroll 1
-            for (int u = 0; u < U; u++) {
-                float zz[NT][4];
+        if constexpr (EDGE && U == 1 && (!SUBN || FAR)) {
+            if (FAR || far) {
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) zz[n][e] = ex2(u ? z[U - 1][n][e] : z[0][n][e]);
-                    sum[n][0] += zz[n][0] + zz[n][2];
-                    sum[n][1] += zz[n][1] + zz[n][3];
+                    for (int e = 0; e < 4; e++) z[0][n][e] = ex2(z[0][n][e]);
+                    sum[n][0] += z[0][n][0] + z[0][n][2];
+                    sum[n][1] += z[0][n][1] + z[0][n][3];
                 }
-                far_values<EDGE>(sm + u * TB, zz, tok0 + u * kKvTile, lo_any, hi_any);
+                far_values(sm, z[0], tok0, lo_any, hi_any);
+                return true;
             }
-            return;
+        } else if (!SUBN && far) {
+            return false;                                                    // nothing has been added yet
         }
+        if constexpr (!FAR) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            uint32_t pb[NT][2];
-#pragma unroll
-            for (int n = 0; n < NT; n++) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) z[u][n][e] = ex2(z[u][n][e]);
-                sum[n][0] += z[u][n][0] + z[u][n][2];
-                sum[n][1] += z[u][n][1] + z[u][n][3];
-                if (!PREC) {
-                    pb[n][0] = transpose8(pack_f16(z[u][n][0], z[u][n][1]));
-                    pb[n][1] = transpose8(pack_f16(z[u][n][2], z[u][n][3]));
-                }
-            }
-            uint32_t c[4][(NG + 1) / 2];
-            const uint8_t *vc = sm + u * TB + 256 * NG + g * 2 * NG;
-            lds_halves<NG>(c[0], vc + t * 16 * NG);
-            lds_halves<NG>(c[1], vc + t1 * 16 * NG);
-            lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
-            lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
-#pragma unroll
-            for (int j = 0; j < NG; j++) {
-                uint32_t fa[4], fb[4];
-                value4(fa, c[0], c[1], j);
-                value4(fb, c[2], c[3], j);
+            for (int u = 0; u < U; u++) {
+                uint32_t pb[NT][2];
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
-                    if (PREC) {
-                        float d0, d1;
-                        if (MX) {
-                            d0 = rel_f32(v[u][0][j / 4] >> (8 * (j % 4)) & 0xff);
-                            d1 = rel_f32(v[u][2][j / 4] >> (8 * (j % 4)) & 0xff);
-                        } else {
-                            const float2 a2 = unpack_f16(v[u][0][j / 2]), b2 = unpack_f16(v[u][2][j / 2]);
-                            d0 = j % 2 ? a2.y : a2.x;
-                            d1 = j % 2 ? b2.y : b2.x;
-                        }
-                        const float x0 = z[u][n][0] * d0, x1 = z[u][n][1] * d0, x2 = z[u][n][2] * d1, x3 = z[u][n][3] * d1;
-                        const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
-                        const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
-                        const uint32_t l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y)), l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
-                        const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
 #pragma unroll
-                        for (int m = 0; m < 2; m++) {                        // a tile's sum by itself: the accumulator of a product is truncated, not rounded
-                            float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
-                            mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+                    for (int e = 0; e < 4; e++) z[u][n][e] = ex2(z[u][n][e]);
+                    sum[n][0] += z[u][n][0] + z[u][n][2];
+                    sum[n][1] += z[u][n][1] + z[u][n][3];
+                    if (!PREC) {
+                        pb[n][0] = transpose8(pack_f16(z[u][n][0], z[u][n][1]));
+                        pb[n][1] = transpose8(pack_f16(z[u][n][2], z[u][n][3]));
+                    }
+                }
+                uint32_t c[4][(NG + 1) / 2];
+                const uint8_t *vc = sm + u * TB + 256 * NG + g * 2 * NG;
+                lds_halves<NG>(c[0], vc + t * 16 * NG);
+                lds_halves<NG>(c[1], vc + t1 * 16 * NG);
+                lds_halves<NG>(c[2], vc + (t + 8) * 16 * NG);
+                lds_halves<NG>(c[3], vc + (t1 + 8) * 16 * NG);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) o[n][j][m][e] += acc[e];
-                        }
-                    } else {
-                        uint32_t d0, d1;
-                        if (MX) {
-                            d0 = rel_f16(v[u][0], v[u][1], j);
-                            d1 = rel_f16(v[u][2], v[u][3], j);
+                for (int j = 0; j < NG; j++) {
+                    uint32_t fa[4], fb[4];
+                    value4(fa, c[0], c[1], j);
+                    value4(fb, c[2], c[3], j);
+#pragma unroll
+                    for (int n = 0; n < NT; n++) {
+                        if (PREC) {
+                            float d0, d1;
+                            if (MX) {
+                                d0 = rel_f32(v[u][0][j / 4] >> (8 * (j % 4)) & 0xff);
+                                d1 = rel_f32(v[u][2][j / 4] >> (8 * (j % 4)) & 0xff);
+                            } else {
+                                const float2 a2 = unpack_f16(v[u][0][j / 2]), b2 = unpack_f16(v[u][2][j / 2]);
+                                d0 = j % 2 ? a2.y : a2.x;
+                                d1 = j % 2 ? b2.y : b2.x;
+                            }
+                            const float x0 = z[u][n][0] * d0, x1 = z[u][n][1] * d0, x2 = z[u][n][2] * d1, x3 = z[u][n][3] * d1;
+                            const uint32_t h0 = pack_f16(x0, x1), h1 = pack_f16(x2, x3);
+                            const float2 u0 = unpack_f16(h0), u1 = unpack_f16(h1);
+                            const uint32_t l0 = transpose8(pack_f16(x0 - u0.x, x1 - u0.y)), l1 = transpose8(pack_f16(x2 - u1.x, x3 - u1.y));
+                            const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
+#pragma unroll
+                            for (int m = 0; m < 2; m++) {                        // a tile's sum by itself: the accumulator of a product is truncated, not rounded
+                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], l0, l1);
+                                mma(acc, fa[2 * m], fa[2 * m + 1], fb[2 * m], fb[2 * m + 1], b0, b1);
+#pragma unroll
+                                for (int e = 0; e < 4; e++) o[n][j][m][e] += acc[e];
+                            }
                         } else {
-                            d0 = pair_of(v[u][0], v[u][1], j);
-                            d1 = pair_of(v[u][2], v[u][3], j);
-                        }
-                        const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
-                        mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
-                        mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
-                        if (SUBN) {
-                            constexpr uint32_t one = 0x3c003c00u;
-                            const uint32_t up = j % 2 ? 0 : one, down = j % 2 ? one : 0;
-                            mma(w[SUBN ? n : 0][SUBN ? j / 2 : 0], up, down, up, down, b0, b1);
+                            uint32_t d0, d1;
+                            if (MX) {
+                                d0 = rel_f16(v[u][0], v[u][1], j);
+                                d1 = rel_f16(v[u][2], v[u][3], j);
+                            } else {
+                                d0 = pair_of(v[u][0], v[u][1], j);
+                                d1 = pair_of(v[u][2], v[u][3], j);
+                            }
+                            const uint32_t b0 = mul2(pb[n][0], d0), b1 = mul2(pb[n][1], d1);
+                            mma(o[n][j][0], fa[0], fa[1], fb[0], fb[1], b0, b1);
+                            mma(o[n][j][1], fa[2], fa[3], fb[2], fb[3], b0, b1);
+                            if (SUBN) {
+                                constexpr uint32_t one = 0x3c003c00u;
+                                const uint32_t up = j % 2 ? 0 : one, down = j % 2 ? one : 0;
+                                mma(w[SUBN ? n : 0][SUBN ? j / 2 : 0], up, down, up, down, b0, b1);
+                            }
                         }
                     }
                 }
             }
         }
+        return true;
     }
     // A word's 8 codes as four pairs.
     __device__ __forceinline__ static void codes4(uint32_t *f, uint32_t x) {
@@ -695,10 +703,10 @@ struct Worker {
     }
 
     // A tile whose scales the window does not hold: its values' products by sixteen exponents at a time, each level's brought up to the
-    // window (or down to it, where bf16 results meet q4_0 scales of 32 and more) and added to the sums in 32 bits. So no scale is
+    // window (or down to it: q4_0 scales of 2 and more for bf16 results) and added to the sums in 32 bits. So no scale is
     // lost beside a larger one, of another block, another token, or one that some rows do not see. Two levels take about
     // twice a tile's time. There are eight levels: what is 2^-112 of the block's largest scale counts as 0, and the sums' 32 bits keep no more.
-    template <bool EDGE> __device__ __forceinline__ void far_values(const uint8_t *tl, const float (&zz)[NT][4], int tok0, int lo_any, int hi_any) {
+    __device__ __forceinline__ void far_values(const uint8_t *tl, const float (&zz)[NT][4], int tok0, int lo_any, int hi_any) {
         const int ra = tau(g), t1 = 4 + (t ^ 1);
         constexpr int VS = 512 * NG + 16 * NG * SB;
         uint32_t pb[NT][2];
@@ -717,16 +725,16 @@ struct Worker {
             // A scale brought to the window, as a float; 0 outside this level
             auto scale = [&](int row, int j) -> float {
                 const int low = (MX ? (int)(base4[MX ? j / 4 : 0] >> (8 * (j % 4)) & 0xff) : base) - 16 * lev;      // exponents low .. low + 15
-                if (EDGE && (tok0 + row < lo_any || tok0 + row >= hi_any)) return 0.0f;
+                if (tok0 + row < lo_any || tok0 + row >= hi_any) return 0.0f;
                 if (MX) {
                     const int e = tl[VS + row * NG + j];
-                    if (EDGE && e == 255) return 0.0f;
+                    if (e == 255) return 0.0f;
                     more |= e > 0 && e < low;
                     return e >= low && e <= low + 15 ? exp2i(e - low - 14) : 0.0f;
                 }
                 const uint32_t x = *(const uint16_t *)(tl + VS + (row * NG + j) * 2);
                 const int e = x >> 10 & 31;
-                if (EDGE && e == 31) return 0.0f;
+                if (e == 31) return 0.0f;
                 more |= (x & 0x7fff) && e < low;
                 return e >= low && e <= low + 15 ? __half2float(__ushort_as_half((unsigned short)x)) * up : 0.0f;
             };
@@ -788,6 +796,23 @@ struct Worker {
 
     // Cache tiles [a, b) of request r's head h into the rows' sums.
     __device__ __forceinline__ void run(int r, int h, int rt, const Queries &rq, int a, int b) {
+        tiles<false>(r, h, rt, rq, a, b);
+        if constexpr (SUBN) {
+            dump();
+            // The rows of a cache with such scales, rare as they are, take their tiles twice. As a case of the loop this cost all others 5% (64 requests to 8192
+            // tokens, 32 heads to 8 of 128), as a second loop in this function 3%, as it is 1.5%.
+            if (base > kMostBase) {
+                // (from a copy: a kernel that gives its parameters' address away reads them more slowly, 1.2% of the same case)
+                AttendArgs *copy = (AttendArgs *)(smem + BUF_AT + BUF) + warp;
+                if (lane == 0) *copy = p;
+                __syncwarp();
+                far_tiles<T, NG, NT>(*copy, smem, r, h, rt, rq, a, b);
+            }
+        }
+    }
+
+    // FAR: one tile at a time, all of them by far_values().
+    template <bool FAR> __device__ __forceinline__ void tiles(int r, int h, int rt, const Queries &rq, int a, int b) {
         const int32_t *table = p.a.tables + (size_t)r * p.a.max_blocks;
         const int i0 = rt * NR / p.group, i1 = min((rt * NR + NR - 1) / p.group, rq.nq - 1);
         const int first = rq.at + i0, last = rq.at + i1;                     // the rows' positions
@@ -835,23 +860,19 @@ struct Worker {
             __syncwarp();
             const int st = k % 2 * 2, tok0 = (a + 2 * (warp + k * kWarps)) * kKvTile;
             const uint32_t both = good >> st & 3;
-            if (both == 3 && tok0 >= whole_lo && tok0 + 2 * kKvTile <= whole_hi) {
-                step<false, 2>(ring + st * TB, tok0, lo_any, hi_any);
-            } else {
+            if (FAR || !(both == 3 && tok0 >= whole_lo && tok0 + 2 * kKvTile <= whole_hi && step<false, 2>(ring + st * TB, tok0, lo_any, hi_any))) {
 #pragma unroll 1
                 for (int u = 0; u < 2; u++)
-                    if (both >> u & 1) step<true, 1>(ring + (st + u) * TB, tok0 + u * kKvTile, lo_any, hi_any);
+                    if (both >> u & 1) step<true, 1, FAR>(ring + (st + u) * TB, tok0 + u * kKvTile, lo_any, hi_any);
             }
             __syncwarp();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
 
-    // The warps' results joined; the rows' outputs, or a partial result.
-    __device__ __forceinline__ void finish(int start, int nq, int h, int rt, float *part) {
-        float *buf = (float *)smem;                                          // [warp][row][DP + 4]: values, reference, sum
-        constexpr int LD = DP + 4;
-        __syncthreads();                                                     // every warp is done with the ring
+    // This warp's results for the join.
+    __device__ __forceinline__ void dump() const {
+        float *buf = (float *)(smem + BUF_AT);
 #pragma unroll
         for (int n = 0; n < NT; n++) {
 #pragma unroll
@@ -880,6 +901,15 @@ struct Worker {
                     *(float4 *)(row + 32 * j + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
                 }
             }
+        }
+    }
+
+    // The warps' results joined; the rows' outputs, or a partial result.
+    __device__ __forceinline__ void finish(int start, int nq, int h, int rt, float *part) {
+        const float *buf = (const float *)(smem + BUF_AT);
+        if constexpr (!SUBN) {
+            __syncthreads();                                                 // every warp is done with the ring
+            dump();
         }
         __syncthreads();
         constexpr int PER = DP / 4;
@@ -919,6 +949,14 @@ struct Worker {
         store_f32(dst + 3, v.w * f);
     }
 };
+
+// A warp's share of a piece again, all of it by far_values(): q4_0 and bf16 results.
+template <typename T, int NG, int NT>
+__device__ __noinline__ void far_tiles(const AttendArgs &p, uint8_t *smem, int r, int h, int rt, Queries rq, int a, int b) {
+    Worker<T, 0, NG, NT> w(p, smem);
+    w.template tiles<true>(r, h, rt, rq, a, b);
+    w.dump();
+}
 
 struct Request : Queries { int lo, tiles, rts; };                 // cache tiles [lo, lo + tiles), row tiles
 
