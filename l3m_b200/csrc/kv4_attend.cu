@@ -143,7 +143,8 @@ constexpr int kMostBase = 4;             // bf16 results over q4_0: the window's
 // nibble in the low byte of a half is an f16 subnormal, n * 2^-24 (or n * 2^-20 four bits higher): one mask, no conversion. Its offset
 // of 8 is taken off the sum instead: scores start at -8 sum(q), and the sum of P times scale, which the values' offset multiplies,
 // comes from one more product with ones. Float results use n - 8 itself (one more f16 operation), so that nothing cancels.
-// (The sums then hold numbers of 255 P scale, so 2^-23 of those, not of the values, is what a step of 16 tokens loses.)
+// (The sums then hold numbers of 15 P scale, or 255 for 16 times a value, and 2^-23 of those, not of the values, is what a step of 16 tokens loses:
+// settle() bounds it.)
 // A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
 // them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
 // split in two f16 for float ones.
@@ -618,10 +619,10 @@ struct Worker {
             f[0] = prmt(x0, y0, 0x5410); f[1] = prmt(x0, y0, 0x7632);
             f[2] = prmt(x1, y1, 0x5410); f[3] = prmt(x1, y1, 0x7632);
         } else {
-            if (SUBN) {                                                      // y = n0 + 16 n1 and 16 n1 of the low bytes, then of the high ones
+            if (SUBN) {                                                      // y = n0 + 16 n1 and n0 of the low bytes, then of the high ones
                 const uint32_t x = pair_of(a, b, j);
-                f[0] = x & 0x00ff00ffu; f[1] = x & 0x00f000f0u;
-                f[2] = prmt(x, 0, 0x4341); f[3] = f[2] & 0x00f000f0u;
+                f[0] = x & 0x00ff00ffu; f[1] = x & 0x000f000fu;
+                f[2] = prmt(x, 0, 0x4341); f[3] = f[2] & 0x000f000fu;
             } else {
                 const uint32_t x = pair_of(a, b, j), y = x >> 8;
                 f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
@@ -866,8 +867,28 @@ struct Worker {
                     if (both >> u & 1) step<true, 1, FAR>(ring + (st + u) * TB, tok0 + u * kKvTile, lo_any, hi_any);
             }
             __syncwarp();
+            if (SUBN && k % 32 == 31) settle();
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+
+    // The offset of the codes so far taken off the sums. A product truncates what it adds to, by up to 2^-23 of it: sums that held the codes of a whole
+    // share would lose more the longer it is. So they hold values, and the codes (up to 255 where a value has 8) of 32 steps at most.
+    __device__ __forceinline__ void settle() {
+#pragma unroll
+        for (int n = 0; n < NT; n++)
+#pragma unroll
+            for (int j = 0; j < NG; j++)
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    float &sum8 = w[SUBN ? n : 0][SUBN ? j / 2 : 0][j % 2 * 2 + c];
+#pragma unroll
+                    for (int m = 0; m < 2; m++) {
+                        o[n][j][m][c] = fmaf(sum8, -8.0f * 17.0f * 0x1p-24f, o[n][j][m][c]);
+                        o[n][j][m][2 + c] = fmaf(sum8, -8.0f * 0x1p-24f, o[n][j][m][2 + c]);
+                    }
+                    sum8 = 0.0f;
+                }
     }
 
     // This warp's results for the join.
@@ -891,8 +912,9 @@ struct Worker {
                     float v[4] = {o[n][j][0][c], o[n][j][0][2 + c], o[n][j][1][c], o[n][j][1][2 + c]};
                     if (SUBN) {
                         const float off = w[SUBN ? n : 0][SUBN ? j / 2 : 0][j % 2 * 2 + c] * 8.0f;
-                        v[0] = fmaf(v[0] - v[1], 0x1p24f, -off); v[1] = fmaf(v[1], 0x1p20f, -off);
-                        v[2] = fmaf(v[2] - v[3], 0x1p24f, -off); v[3] = fmaf(v[3], 0x1p20f, -off);
+                        const float hi0 = fmaf(v[0] - v[1], 0x1p20f, -off), hi1 = fmaf(v[2] - v[3], 0x1p20f, -off);
+                        v[0] = fmaf(v[1], 0x1p24f, -off); v[1] = hi0;
+                        v[2] = fmaf(v[3], 0x1p24f, -off); v[3] = hi1;
                     }
                     if (MX) {
                         const float unit = exp2i((int)(base4[MX ? j / 4 : 0] >> (8 * (j % 4)) & 0xff) - 113);

@@ -491,3 +491,29 @@ def test_rotations_that_cancel(api, cdtype, factor, norm):
         want = ref.values(codes, bits, cdtype)
         for h in range(2):
             assert np.array_equal(ref.get_rows(data, c["slot"], h, is_v, cdtype, 64, 64), want[:, h])
+
+
+# ---- sums over long contexts
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("heads,dim,flat", [(1, 32, True), (2, 32, False), (8, 64, True)])
+def test_many_tokens_in_every_share(api, dtype, cdtype, heads, dim, flat):
+    """16 requests of up to four million tokens, the same 16 pages over and over, so that a warp sums thousands of tiles: the result is that of
+    the 16 pages once, within the tolerance of short contexts. Scores are all alike (scale 0) or random."""
+    rng, page, times = np.random.default_rng(90 + heads), 4096, 64 if dim == 32 else 32
+    host = random_cache(rng, cdtype, 16, 1, page, dim)
+    tables = np.stack([np.concatenate([rng.permutation(16) for _ in range(times)]) for _ in range(16)]).astype(np.int32)
+    lens, q_start = [16 * times * page] * 16, np.arange(17)
+    q, q64 = queries(api, rng, 16, heads, dim, dtype)
+    scale = 0.0 if flat else 0.25
+    out, st = api.attend(api.cache(api.put(host), cdtype, page, 1, dim), q, q_start, lens, tables, scale)
+    assert st.item() == 0
+    once = [16 * page] * 16
+    want, spread = ref.attend(q64, q_start, once, tables[:, :16], host, cdtype, dim, page, 1, scale)
+    check_attend(out, want, spread, dtype)
+    # and not further off, over all, than the 16 pages once: sums in 32 bits, rounded to nearest, of a few thousand terms a warp lose 2^-24 of themselves
+    # each, 2^-12 at the very worst, and the values' sum is 200 times smaller than the spread that this is relative to
+    short, _ = api.attend(api.cache(api.put(host), cdtype, page, 1, dim), q, q_start, once, tables, scale)
+    off = [np.linalg.norm(x.double().cpu().numpy() - want) for x in (out, short)]
+    assert off[0] <= 1.1 * off[1] + (2.0 ** -20 * np.linalg.norm(spread) if dtype == F32 else 0), off
