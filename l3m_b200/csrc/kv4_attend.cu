@@ -221,14 +221,13 @@ struct Worker {
 #pragma unroll
                 for (int e = 0; e < 8; e++) x[j][e] = x[j][e] * up0 * up1;
                 if (SUBN) {
-                    // The fragments hold nibbles 2k and 2k + 4 ... as r = n0 and y = n0 + 16 n1, so q0 n0 + q1 n1 = (q0 - q1 / 16) r + q1 / 16 y.
+                    // The fragments hold nibbles 2k and 2k + 4, then 16 times nibbles 2k + 1 and 2k + 5.
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
+                        q[0][n][j][2 * k] = pack_f16(x[j][2 * k], x[j][2 * k + 4]);
                         q[0][n][j][2 * k + 1] = pack_f16(x[j][2 * k + 1] * 0.0625f, x[j][2 * k + 5] * 0.0625f);
-                        const float2 y = unpack_f16(q[0][n][j][2 * k + 1]);
-                        q[0][n][j][2 * k] = pack_f16(x[j][2 * k] - y.x, x[j][2 * k + 4] - y.y);
-                        const float2 r = unpack_f16(q[0][n][j][2 * k]);
-                        s += r.x + r.y + 17.0f * (y.x + y.y);
+                        const float2 a = unpack_f16(q[0][n][j][2 * k]), b = unpack_f16(q[0][n][j][2 * k + 1]);
+                        s += a.x + a.y + 16.0f * (b.x + b.y);
                     }
                 } else {
 #pragma unroll
@@ -599,15 +598,10 @@ struct Worker {
             f[0] = e2m1_pair<0>(x); f[1] = e2m1_pair<1>(x);
             f[2] = e2m1_pair<2>(x); f[3] = e2m1_pair<3>(x);
         } else {
-            if (SUBN) {                                                      // r and y of the low bytes, then of the high ones
-                f[1] = x & 0x00ff00ffu; f[0] = x & 0x000f000fu;
-                f[3] = prmt(x, 0, 0x4341); f[2] = f[3] & 0x000f000fu;
-            } else {
-                const uint32_t y = x >> 8;
-                f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
-                f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
-                whole(f);
-            }
+            const uint32_t y = x >> 8;                                       // n0 and 16 n1 of the low bytes, then of the high ones
+            f[0] = x & 0x000f000fu; f[1] = x & 0x00f000f0u;
+            f[2] = y & 0x000f000fu; f[3] = y & 0x00f000f0u;
+            if (!SUBN) whole(f);
         }
     }
     // Block j's 4 codes of two tokens as four pairs of the same dim.

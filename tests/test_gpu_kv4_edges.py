@@ -517,3 +517,27 @@ def test_many_tokens_in_every_share(api, dtype, cdtype, heads, dim, flat):
     short, _ = api.attend(api.cache(api.put(host), cdtype, page, 1, dim), q, q_start, once, tables, scale)
     off = [np.linalg.norm(x.double().cpu().numpy() - want) for x in (out, short)]
     assert off[0] <= 1.1 * off[1] + (2.0 ** -20 * np.linalg.norm(spread) if dtype == F32 else 0), off
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_bf16_queries_enter_the_scores_whole(api, torch, dim):
+    """Neighbouring query values of 8 bits whose combinations have more than 11: scores are those of the queries themselves. One query whose large values
+    cancel exactly over keys of one code, but for a few dims: a query off by 2^-12 would move the scores by far more than is left."""
+    rng, page, n = np.random.default_rng(95), 16, 400
+    tables, q_start, n_pages = batch(rng, [n], [1], page)
+    host = random_cache(rng, ref.Q4, n_pages, 1, page, dim)
+    ng = ref.blocks(dim)
+    host[..., :256 * ng] = 0xFF                                              # key codes 15: 7 times the scale
+    scale_cells(host, ref.Q4, dim, False)[...] = rng.integers(1, 33, (n_pages, 1, 1, 16, 1)).astype(np.float16)      # one for all blocks of a token
+    big = rng.integers(128, 256, (8, dim // 4)) * np.exp2(rng.integers(-3, 3, (8, dim // 4)))
+    q64 = np.zeros((1, 8, dim))
+    q64[0, :, 0::4], q64[0, :, 1::4] = big, rng.integers(128, 256, big.shape) * np.exp2(rng.integers(-3, 3, big.shape))
+    q64[0, :, 2::4], q64[0, :, 3::4] = -q64[0, :, 1::4], -q64[0, :, 0::4]
+    q64[0, :, 0] += np.where(q64[0, :, 0] >= 256, 2.0, 1.0)
+    q = torch.from_numpy(q64).to(torch.bfloat16).cuda()
+    q64 = q.double().cpu().numpy()
+    out, _ = api.attend(api.cache(api.put(host), ref.Q4, page, 1, dim), q, q_start, [n], tables, 0.02)
+    want, spread = ref.attend(q64, q_start, [n], tables, host, ref.Q4, dim, page, 1, 0.02)
+    # Products of whole numbers below 2^22 in units of 2^-3: sums in 32 bits are exact up to 2^21, and lose 2^-24 of sum |q k| = 2^18 at the
+    # most per block and step; scores are off by 2^-4 * 0.02 then, P by 2^-9.
+    assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -10) * spread).all()
