@@ -169,7 +169,7 @@ L3M_API int l3m_kv4_plan_dev(const l3m_kv4_plan *a, void *stream);
 // k_out (may be NULL) and, with a cache, keys and values to the cache's slot[token] in 4 bits (a negative slot:
 // not stored). A token with pos < 0 is padding: nothing of it is read or written. Tensors are
 // [n_tokens][heads][head_dim], heads contiguous, ld elements from token to token, so slices of one qkv matrix serve; q_out may be q
-// and k_out may be k. Codes and scales are those of exact arithmetic: as ggml's rule gives them for the
+// and k_out may be k, at the same stride; otherwise results overlap no input. Codes and scales are those of exact arithmetic: as ggml's rule gives them for the
 // normed, rotated values in 64 bits (scales in f16: rounded to f32 first, at most 65504); a NaN is stored as 0. The tokens of a call
 // have different slots (the plan's do): where two share one, its row holds a mixture of both.
 typedef struct {

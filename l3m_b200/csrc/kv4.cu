@@ -816,6 +816,9 @@ L3M_API int l3m_qkv_rope_dev(const l3m_kv4 *cache, const l3m_qkv *a, void *strea
         return refuse(me, "a pointer is not aligned to its type");
     if (!a->n_heads && !with_k && !with_v) return 0;
     if (a->rope && ((uintptr_t)a->rope_table & 7)) return refuse(me, "rope_table must be 8-byte aligned");
+    // In place a row may take only its own place: with another stride it would take rows that other warps still read.
+    if (a->n_tokens > 1 && ((a->n_heads && a->q_out == a->q && a->q_out_ld != a->q_ld) || (with_k && a->k_out == a->k && a->k_out_ld != a->k_ld)))
+        return refuse(me, "in place, a result needs its input's token stride");
     QkvArgs p = {*a, {}, with_v, cache && cache->dtype == L3M_DT_MXFP4, 0, 0, 0, 1, 1};
     if (cache) p.c = kv4_dev(cache);
     // 16-byte accesses where every row of every tensor starts on 16 bytes.

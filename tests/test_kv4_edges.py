@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import kv4_ref as ref
-from test_kv4 import attend, cache, lib  # noqa: F401
+from test_kv4 import attend, cache, lib, qkv  # noqa: F401
 
 
 def test_a_plan_without_room_counts_rows_past_its_tensors():
@@ -20,3 +20,12 @@ def test_attend_refuses_a_negative_row_count(lib):  # noqa: F811
     assert lib.l3m_kv4_attend_dev(C.byref(c), C.byref(attend(max_rows=-1)), None) == -1 and b"negative" in lib.l3m_cuda_error()
     assert lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend(max_rows=-1))) == 0
     assert lib.l3m_kv4_attend_scratch(C.byref(c), C.byref(attend(max_rows=3))) >= 16
+
+
+@pytest.mark.parametrize("change", [dict(q_out=64, q_out_ld=256, q_ld=512), dict(q_out=64, q_out_ld=768), dict(q_out=4096, k_out=64, k_out_ld=128)])
+def test_qkv_in_place_refuses_another_stride(lib, change):  # noqa: F811
+    """A row's result would land on rows that are still to be read."""
+    c = cache()
+    base = dict(q=64, q_out=4096, k=64, k_out=8192, k_ld=512)
+    assert lib.l3m_qkv_rope_dev(C.byref(c), C.byref(qkv(**{**base, **change})), None) == -1
+    assert b"in place" in lib.l3m_cuda_error(), lib.l3m_cuda_error()
