@@ -143,8 +143,9 @@ constexpr int kMostBase = 4;             // bf16 results over q4_0: the window's
 // nibble in the low byte of a half is an f16 subnormal, n * 2^-24 (or n * 2^-20 four bits higher): one mask, no conversion. Its offset
 // of 8 is taken off the sum instead: scores start at -8 sum(q), and the sum of P times scale, which the values' offset multiplies,
 // comes from one more product with ones. Float results use n - 8 itself (one more f16 operation), so that nothing cancels.
-// (The sums then hold numbers of 15 P scale, or 255 for 16 times a value, and 2^-23 of those, not of the values, is what a step of 16 tokens loses:
-// settle() bounds it.)
+// What that costs: the tensor cores align a product's terms by their exponents and cut them off 24 bits below the largest, and a subnormal's exponent counts as
+// -14, so a step of 16 tokens loses up to 2^-14 of P times scale (in units of a code, most often 2^-15), 2^-17 of the codes' sums; settle() keeps what
+// the sums themselves lose from growing with the context.
 // A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
 // them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
 // split in two f16 for float ones.

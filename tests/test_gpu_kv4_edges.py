@@ -541,3 +541,37 @@ def test_bf16_queries_enter_the_scores_whole(api, torch, dim):
     # Products of whole numbers below 2^22 in units of 2^-3: sums in 32 bits are exact up to 2^21, and lose 2^-24 of sum |q k| = 2^18 at the
     # most per block and step; scores are off by 2^-4 * 0.02 then, P by 2^-9.
     assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -8 * np.abs(want) + (2.0 ** -8 + 2.0 ** -10) * spread).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("cdtype", [ref.Q4, ref.MX])
+@pytest.mark.parametrize("dim,heads,kh,wide", [(dim, 8, 1, wide) for dim in (24, 64, 96, 128) for wide in (False, True)] + [(160, 7, 1, False), (192, 4, 2, False), (224, 8, 1, False), (256, 3, 1, False)])
+def test_scales_far_apart_in_every_variant(api, dtype, cdtype, dim, heads, kh, wide):
+    """Each number of blocks, 8 and 16 rows to a tile (the call's bounds decide, lengths are short): blocks 2^10 apart, some tokens 2^16 (q4_0: 2^9) above their
+    neighbours, in a context with a window and without, through pages in any order."""
+    rng, page, lens, news = np.random.default_rng(dim), 16, [333, 40, 1200], [20, 3, 33]
+    ng = ref.blocks(dim)
+    width = 40000 // page * 16 if wide else 80
+    for window in (0, 100):
+        tables, q_start, n_pages = batch(rng, lens, news, page, width=width)
+        host = random_cache(rng, cdtype, n_pages, kh, page, dim)
+        v = scale_cells(host, cdtype, dim, True)
+        up = (rng.random(v.shape[:4] + (1,)) < 0.1) * 1
+        if cdtype == ref.MX:
+            v[...] = 200 - 10 * np.arange(ng) + 16 * up + rng.integers(0, 3, v.shape)
+        else:
+            v[...] = (np.exp2(5.0 - np.minimum(10 * np.arange(ng), 16) + 9 * up) * rng.uniform(1, 2, v.shape)).astype(np.float16)
+        q, q64 = queries(api, rng, int(q_start[-1]), heads, dim, dtype)
+        out, st = api.attend(api.cache(api.put(host), cdtype, page, kh, dim), q, q_start, lens, tables, dim ** -0.5, window, max_kv=width * page)
+        want, spread = ref.attend(q64, q_start, lens, tables, host, cdtype, dim, page, kh, dim ** -0.5, window)
+        if dtype == BF16 and cdtype == ref.Q4:
+            # q4_0's codes enter bf16 results as f16 subnormals, n * 2^-24, and 8 is taken off behind. A product's 17 terms (16 tokens and the sum so
+            # far) are aligned by their exponents, a subnormal's being -14, and cut off 24 bits below: by 2^-14 of the largest p * scale of the 16 tokens
+            # each, in units of a code. So a result is off by 17 * 2^-14 < 1.1 * 2^-10 of sum p * scale, a token whose value is 0 included, which the
+            # spread does not know.
+            ones = host.copy()
+            ones[..., 256 * ng:512 * ng] = 0x99
+            scale = ref.attend(q64, q_start, lens, tables, ones, cdtype, dim, page, kh, dim ** -0.5, window)[0]
+            spread = spread + 1.1 * scale
+        check_attend(out, want, spread, dtype)
+        assert st.item() == 0
