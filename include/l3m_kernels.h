@@ -204,7 +204,8 @@ typedef struct {
     int   dtype;                 // of q and out: L3M_DT_F32 or L3M_DT_BF16
     int   n_heads;               // a multiple of n_kv_heads: query head h reads kv head h / (n_heads / n_kv_heads)
     int   n_req, max_blocks;
-    int   max_q;                 // at least every request's number of queries (more are not looked at); max_q * n_heads <= 2^30
+    int   max_q;                 // at least every request's number of queries (more are not looked at); max_q * n_heads <= 2^30. The bounds, not the
+                                 // lengths, choose the kernel: single tokens beside a prompt, or under a prompt's max_q, take a prompt's time each
     int   max_kv;                // at least every kv_len; at most max_blocks * page
     int   window;                // 0: none
     float scale;                 // of the scores, below 2^127 in magnitude

@@ -635,8 +635,9 @@ struct RowWorker {
 };
 
 // LPR lanes a row, 8 values a lane, so that a row is one access wide and its sums are shuffles; queries first, then keys, then
-// values, the next rows' loads under way. Bound: instructions (norm, rotation, bounds and two roundings of each value to codes)
-// beside memory, at the 24 warps an SM that 80 registers allow: 8191 tokens of 32 + 8 + 8 heads of 128, bf16 to mxfp4, 75 us for 170 MB, 2.3 TB/s.
+// values, the next rows' loads under way. Bound: bytes under way. A warp has one group of rows ahead of it, 512 bytes of bf16 at 128 dims, so the 24
+// warps an SM that 80 registers allow have 12 KB, which at 0.8 us of latency is 2.3 TB/s; instructions (norm, rotation, bounds and two roundings of
+// each value to codes) take 2.4 issue slots of 4. 8191 tokens of 32 + 8 + 8 heads of 128, bf16 to mxfp4: 76 us for 170 MB, 2.2 TB/s.
 // 3 CTAs an SM of 80 registers; with fewer registers the bounds spill.
 template <typename T, int LPR, int ROPE, bool VEC>
 __global__ void __launch_bounds__(kQkvThreads, 3) qkv_kernel(const __grid_constant__ QkvArgs p) {
@@ -697,7 +698,7 @@ __device__ __forceinline__ float scale_value(const uint8_t *p, int mx) {
 }
 
 // One warp, or several, per row: the lanes go over its keys' and values' pieces of 8. 8191 rows of 8 heads of 128 to bf16: 20 us,
-// 43 MB, bound by the pieces' unpacking and short rows.
+// 43 MB, bound by its short reads: 4 or 8 bytes of codes and a scale a lane.
 template <typename T>
 __global__ void __launch_bounds__(256) load_kernel(const __grid_constant__ LoadArgs p) {
     const int lane = threadIdx.x & 31, per = p.c.n_kv * p.parts, ng = p.c.ng;

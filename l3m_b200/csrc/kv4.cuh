@@ -2,7 +2,7 @@
 // that write it (kv4.cu) and read it (kv4_attend.cu).
 //
 // Why this layout: one tile of 16 tokens of one head is one contiguous piece (2304 bytes for q4_0 at
-// head_dim 128), so a warp fetches it with a single bulk copy and a page of one head is a run of tiles.
+// head_dim 128), so a warp fetches it with 16-byte copies side by side and a page of one head is a run of tiles.
 // Inside it the codes of one token are contiguous, so appending a token writes whole bytes of its own
 // and never shares one with a neighbour. The order within a token's row is the order in which the
 // tensor-core fragments of m16n8k16 want them: lane 4*g + t of a warp reads, for the key row of its

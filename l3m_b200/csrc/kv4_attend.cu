@@ -698,10 +698,11 @@ struct Worker {
         }
     }
 
-    // A tile whose scales the window does not hold: its values' products by sixteen exponents at a time, each level's brought up to the
-    // window (or down to it: q4_0 scales of 2 and more for bf16 results) and added to the sums in 32 bits. So no scale is
-    // lost beside a larger one, of another block, another token, or one that some rows do not see. Two levels take about
-    // twice a tile's time. There are eight levels: what is 2^-112 of the block's largest scale counts as 0, and the sums' 32 bits keep no more.
+    // A tile whose scales the window does not hold: its values' products by sixteen exponents at a time, each level's scales brought up to the
+    // window (or down to it: q4_0 scales of 2 and more for bf16 results) and its sums added in 32 bits. So no scale is lost beside
+    // a larger one of another token, or one that some rows do not see (mxfp4's blocks have windows of their own). 64 requests to 8192 tokens, 32 heads
+    // to 8 of 128, bf16, mxfp4: 133 us where no tile comes here (136 with blocks 2^40 apart), 516 where all do, a token in 16 being 2^20 above the
+    // others. There are eight levels: what is 2^-112 of the block's largest scale counts as 0, and the sums' 32 bits keep no more.
     __device__ __forceinline__ void far_values(const uint8_t *tl, const float (&zz)[NT][4], int tok0, int lo_any, int hi_any) {
         const int ra = tau(g), t1 = 4 + (t ^ 1);
         constexpr int VS = 512 * NG + 16 * NG * SB;
@@ -1005,8 +1006,9 @@ template <int kWarps> __device__ long long block_sum_scan(long long v, long long
     return v;
 }
 
-// Bound: instructions beside memory. 64 requests to 8192 tokens, 32 heads to 8 of 128, bf16, q4_0: 105 us for 403 MB, 3.9 TB/s (the
-// same loads without the arithmetic 75 us, the arithmetic on one tile over and over 99); one request of 250001, 16 heads to 2: 34 us for 72 MB.
+// Bound: instructions beside memory. 64 requests to 8192 tokens, 32 heads to 8 of 128, bf16, q4_0: 107 us for 403 MB, 3.8 TB/s (the
+// same loads without the arithmetic took 75 us, the arithmetic on one tile over and over 99, before it had the codes' exact halves and settle());
+// one request of 250001, 16 heads to 2: 34.6 us for 72 MB, of which 19 at the rate above and the rest the fixed chain of shares and join.
 template <typename T, int MX, int NG, int NT>
 __global__ void __launch_bounds__(32 * warps_of(NG, NT), kCtas) attend_kernel(const __grid_constant__ AttendArgs p) {
     typedef Worker<T, MX, NG, NT> W;

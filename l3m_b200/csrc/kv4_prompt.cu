@@ -19,7 +19,7 @@
 // passes it by 14 (then to 10 below the largest), which multiplies O by a power of two.
 //
 // Bound: the tensor pipe inside a CTA (75% of its rate while one runs), the last wave of CTAs outside. 2 chunks of 1024 over up to
-// 6000 tokens, 32 heads to 8 of 128, q4_0: 218 to 238 us for 144 GFLOP, 600 to 660 TFLOP/s, on 256 CTAs in two waves. Even shares of the context
+// 6000 tokens, 32 heads to 8 of 128, q4_0: 226 to 242 us for 144 GFLOP, 600 to 640 TFLOP/s, on 256 CTAs in two waves. Even shares of the context
 // for one CTA an SM, joined behind, took 336 us: their loop leaves the softmax too few registers, and each share starts anew.
 //
 // Every wait has a limit; a wait that gives up sets a status bit and the CTA's rows become NaN.
@@ -32,7 +32,7 @@
 namespace l3m {
 namespace {
 
-constexpr int kSms = 148;
+constexpr int kSms = 148;                               // of a B200; not asked of the device, so that the scratch's size is the arguments' alone
 constexpr int kRows = 128, kStep = 128, kHalf = 64;     // rows of a tile, tokens that are widened at a time, tokens of a product
 constexpr int kSoftWarps = 8, kWideWarps = 8;          // half of the latter for keys, half for values
 constexpr int kPromptThreads = 32 * (kSoftWarps + kWideWarps + 2);
