@@ -134,6 +134,9 @@ constexpr int warps_of(int ng, int nt) { return ng * nt <= 5 ? 6 : 4; }
 
 constexpr int kMostBase = 4;             // bf16 results over q4_0: the window's base up to which one pass serves, scales below 32
 
+template <typename T, int NG, int NT>
+__device__ __noinline__ void far_tiles(const AttendArgs &p, uint8_t *smem, int r, int h, int rt, Queries rq, int a, int b);
+
 // One piece of a segment (request r, kv head h, row tile rt): cache tiles [a, b), by the CTA's warps. Scores are
 // computed transposed, S^T = K Q^T (16 tokens x 8 rows a product), so that a decode step's few rows pad to 8, not 16, and
 // O^T = V^T P^T follows from it with one 8x8 transposition per 8 tokens. Each warp keeps its own softmax reference and
@@ -149,9 +152,6 @@ constexpr int kMostBase = 4;             // bf16 results over q4_0: the window's
 // A key's scale multiplies its block's score; a value's scale multiplies P. Queries are scaled to 2^10 by a power of two, so f16 holds
 // them (bf16 exactly, float as two f16 of 22 bits); P is held up to 2^14, rounded to f16 for bf16 results and
 // split in two f16 for float ones.
-template <typename T, int NG, int NT>
-__device__ __noinline__ void far_tiles(const AttendArgs &p, uint8_t *smem, int r, int h, int rt, Queries rq, int a, int b);
-
 template <typename T, int MX, int NG, int NT>
 struct Worker {
     static constexpr int kWarps = warps_of(NG, NT), kThreads = 32 * kWarps;
@@ -903,7 +903,7 @@ struct Worker {
                     row[DP] = ref[n][c];
                     row[DP + 1] = s;
                 }
-                #pragma unroll
+#pragma unroll
                 for (int j = 0; j < NG; j++) {
                     float v[4] = {o[n][j][0][c], o[n][j][0][2 + c], o[n][j][1][c], o[n][j][1][2 + c]};
                     if (SUBN) {
