@@ -199,7 +199,8 @@ L3M_API int l3m_kv4_load_dev(const l3m_kv4 *cache, int dtype, void *k, void *v, 
 // not finite (the store writes none) leave queries alone that do not see them; what sees them is not defined. Sums are held in 32 bits: a value
 // below 2^-100 of the largest that any of the request's new tokens sees in its block of 32 dims may count as 0, and scores are defined where sum |q| |k| |scale|
 // over a head's dims, a key of q4_0 taken as 8 of its scales, stays below 2^20 (beyond it a score's rounding is that of a factor in its probability),
-// a key's scale below 2^100. out may not overlap q.
+// a key's scale below 2^100. Where that sum is small (5 or so), f32 results are within 2^-16 of sum p |v| of exact arithmetic, bf16 results within their
+// rounding and 2^-10 of sum p |v| (over q4_0 of sum p (|v| + |scale|)), both within 2^-32 of the block's largest scale a token beside. out may not overlap q.
 typedef struct {
     int   dtype;                 // of q and out: L3M_DT_F32 or L3M_DT_BF16
     int   n_heads;               // a multiple of n_kv_heads: query head h reads kv head h / (n_heads / n_kv_heads)
